@@ -38,6 +38,7 @@ inline size_t dtype_bytes(dli_dtype d) {
     case DLI_DTYPE_BF16: return 2;
     case DLI_DTYPE_F16: return 2;
     case DLI_DTYPE_I32: return 4;
+    case DLI_DTYPE_FP4: break;
   }
   return 0;
 }
@@ -84,6 +85,8 @@ enum DeviceError : unsigned {
   kDevErrAttentionTimeout = 4,
   kDevErrKvCapacity = 5,
   kDevErrExchangeTimeout = 6,
+  kDevErrPageIndex = 7,
+  kDevErrRaggedRows = 8,
 };
 // Device address of the error word of the current device (resolved once per
 // device with cudaGetSymbolAddress); kernels receive it as an argument.

@@ -25,6 +25,8 @@ const char* device_error_name(unsigned code) {
     case kDevErrAttentionTimeout: return "attention pipeline wait exceeded its iteration limit";
     case kDevErrKvCapacity: return "KV-cache position outside the cache capacity";
     case kDevErrExchangeTimeout: return "tensor-parallel exchange: a peer's rows did not arrive within the wait limit";
+    case kDevErrPageIndex: return "page table entry outside the page pool";
+    case kDevErrRaggedRows: return "row starts of a packed batch out of order, past its rows or over max_new";
     default: return "unknown device error";
   }
 }

@@ -59,6 +59,11 @@ SIGNATURES = {
     "dli_sm100_attention_kvcache": (N, [P, P, P, P, P] + [I] * 6 + [F, D, P, Z, P]),
     "dli_sm100_attention_kvcache_noalloc_max_scratch": (Z, []),
     "dli_sm100_attention_kvcache_noalloc": (N, [P, P, P, P, P] + [I] * 6 + [F, D, P]),
+    "dli_sm100_paged_kv_page_bytes": (Z, [I, I, I, D]),
+    "dli_sm100_qkv_rotary_paged": (N, [P] * 9 + [I] * 11 + [F, F, D, D, P]),
+    "dli_sm100_attention_paged_workspace_size": (Z, [I] * 8 + [D, D]),
+    "dli_sm100_attention_paged": (N, [P] * 8 + [I] * 9 + [F, F, I, F, F, D, D, P, Z, P]),
+    "dli_sm100_paged_gather": (N, [P] * 7 + [I] * 7 + [F, F, D, D, P]),
     "dli_sm100_add": (N, [P, P, P, I, I, D, P]),
     "dli_sm100_mul": (N, [P, P, P, I, I, D, P]),
     "dli_sm100_silu": (N, [P, P, I, D, P]),
@@ -413,6 +418,157 @@ def attention_kvcache(q, cache_k, cache_v, positions, scale=0.0, out=None):
                                         _ptr(out), b, s, hq, hkv, cap, d, scale, _dt(q), _ptr(ws),
                                         ws_bytes, _stream()), "attention_kvcache")
     return out
+
+
+# ---- paged KV cache -------------------------------------------------------------
+
+FP4 = 5  # kv_dtype code of 4-bit pages (uint8 tensors)
+
+
+def paged_kv_pages(num_pages, kv_heads, page_size, head_dim, dtype, device="cuda"):
+    """A zeroed (k_pages, v_pages) pool of a paged cache: [num_pages, kv_heads,
+    page_size, head_dim] of a float dtype, or for dtype "fp4" the 4-bit pages as
+    uint8 [num_pages, kv_heads, page_size * head_dim * 9 // 16]."""
+    code = FP4 if dtype == "fp4" else DTYPE_CODES.get(dtype)
+    if code is None or lib().dli_sm100_paged_kv_page_bytes(kv_heads, page_size, head_dim, code) == 0:
+        raise ValueError("paged_kv_pages: page_size 16, 32, 64 or 128; a float dtype, or \"fp4\" with head_dim % 16 == 0")
+    if dtype == "fp4":
+        shape, dtype = (num_pages, kv_heads, page_size * head_dim * 9 // 16), torch.uint8
+    else:
+        shape = (num_pages, kv_heads, page_size, head_dim)
+    return torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
+
+
+def _pages(what, k_pages, v_pages, page_table, head_dim, dtype):
+    """(num_pages, kv_heads, page_size, kv dtype code) of a pool, its tensors checked."""
+    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError(f"{what}: k_pages and v_pages differ in shape or dtype")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32:
+        raise ValueError(f"{what}: page_table must be int32 [batch, max_pages]")
+    if k_pages.dtype == torch.uint8:
+        if k_pages.dim() != 3 or head_dim % 16 or k_pages.shape[2] % (head_dim * 9 // 16):
+            raise ValueError(f"{what}: 4-bit pages must be uint8 [num_pages, kv_heads, page_size * head_dim * 9 / 16]")
+        return k_pages.shape[0], k_pages.shape[1], k_pages.shape[2] // (head_dim * 9 // 16), FP4
+    if k_pages.dim() != 4 or k_pages.shape[3] != head_dim or k_pages.dtype != dtype:
+        raise ValueError(f"{what}: pages must be [num_pages, kv_heads, page_size, {head_dim}] of {dtype}")
+    return k_pages.shape[0], k_pages.shape[1], k_pages.shape[2], DTYPE_CODES[dtype]
+
+
+def _rows(what, tokens, positions, page_table, starts, max_new):
+    """max_new of a packed batch, its tensors checked (starts None: equal shares of the rows)."""
+    b = page_table.shape[0]
+    if positions.dtype != torch.int64 or tuple(positions.shape) != (b,):
+        raise ValueError(f"{what}: positions must be int64 [batch]")
+    if starts is None:
+        if max_new is None:
+            if b == 0 or tokens % b:
+                raise ValueError(f"{what}: without starts the rows must divide among the sequences")
+            max_new = tokens // b
+        if tokens != b * max_new:
+            raise ValueError(f"{what}: without starts there must be batch * max_new rows")
+    else:
+        if starts.dtype != torch.int64 or tuple(starts.shape) != (b + 1,):
+            raise ValueError(f"{what}: starts must be int64 [batch + 1]")
+        if max_new is None:
+            max_new = tokens
+    return int(max_new)
+
+
+def _on(what, first, *ts):
+    """Every tensor contiguous on one CUDA device; returns (its guard, its current stream)."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError(f"{what}: expects CUDA tensors")
+    for t in (first, *ts):
+        if t is not None:
+            if t.device != dev:
+                raise ValueError(f"{what}: tensors on different devices")
+            if not t.is_contiguous():
+                raise ValueError("tensors must be contiguous")
+    return torch.cuda.device(dev), ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def qkv_rotary_paged(qkv, cos, sin, positions, page_table, k_pages, v_pages, q_heads, starts=None, max_new=None,
+                     q_out=None, k_scale=1.0, v_scale=1.0):
+    """Rotary embedding of a packed q|k|v projection [.., (Hq + 2 Hkv) * D], its k and
+    v appended to the pages at positions[b], positions[b] + 1, ...; returns rotated q
+    [rows, Hq, D]. `starts` (int64 [batch + 1]) gives the rows of every sequence, at
+    most `max_new` each; None: all sequences have the same number."""
+    kv_heads, width = k_pages.shape[1], qkv.shape[-1]
+    heads = q_heads + 2 * kv_heads
+    if q_heads <= 0 or width % heads:
+        raise ValueError("qkv_rotary_paged: qkv must be [.., (q_heads + 2 * kv_heads) * head_dim]")
+    d, tokens = width // heads, qkv.numel() // width
+    what = "qkv_rotary_paged"
+    num_pages, _, page_size, kv = _pages(what, k_pages, v_pages, page_table, d, qkv.dtype)
+    max_new = _rows(what, tokens, positions, page_table, starts, max_new)
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError("qkv_rotary_paged: cos and sin must be float32 [rows, pairs]")
+    if q_out is None:
+        q_out = torch.empty(tokens, q_heads, d, dtype=qkv.dtype, device=qkv.device)
+    elif q_out.dtype != qkv.dtype or q_out.numel() != tokens * q_heads * d:
+        raise ValueError("qkv_rotary_paged: q_out must be [rows, q_heads, head_dim] of qkv's dtype")
+    guard, stream = _on(what, qkv, cos, sin, positions, page_table, k_pages, v_pages, starts, q_out)
+    with guard:
+        check(lib().dli_sm100_qkv_rotary_paged(
+            _ptr(qkv), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(starts), _ptr(page_table), _ptr(q_out),
+            _ptr(k_pages), _ptr(v_pages), tokens, positions.shape[0], max_new, q_heads, kv_heads, d, cos.shape[1],
+            cos.shape[0], page_size, num_pages, page_table.shape[1], k_scale, v_scale, _dt(qkv), kv, stream), what)
+    return q_out
+
+
+def attention_paged(q, k_pages, v_pages, positions, page_table, starts=None, max_new=None, scale=0.0, softcap=0.0,
+                    window=0, slopes=None, k_scale=1.0, v_scale=1.0, out=None):
+    """Causal attention of packed q [rows, Hq, D] over a paged cache (after the append
+    of the rows' k and v). softcap > 0 caps the scores by a tanh, window > 0 limits a
+    row to its last `window` keys, slopes (float32 [Hq]) add slope * (j - i)."""
+    if q.dim() != 3:
+        raise ValueError("attention_paged: q must be [rows, q_heads, head_dim]")
+    tokens, hq, d = q.shape
+    what = "attention_paged"
+    num_pages, hkv, page_size, kv = _pages(what, k_pages, v_pages, page_table, d, q.dtype)
+    max_new = _rows(what, tokens, positions, page_table, starts, max_new)
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != hq):
+        raise ValueError("attention_paged: slopes must be float32 [q_heads]")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.dtype != q.dtype or out.numel() != q.numel():
+        raise ValueError("attention_paged: out must be like q")
+    guard, stream = _on(what, q, k_pages, v_pages, positions, page_table, starts, slopes, out)
+    L = lib()
+    b, max_pages = page_table.shape
+    with guard:
+        ws_bytes = L.dli_sm100_attention_paged_workspace_size(tokens, b, max_new, hq, hkv, d, page_size, max_pages,
+                                                              _dt(q), kv)
+        ws = _workspace(ws_bytes, q.device)
+        check(L.dli_sm100_attention_paged(
+            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(positions), _ptr(starts), _ptr(page_table), _ptr(slopes),
+            _ptr(out), tokens, b, max_new, hq, hkv, d, page_size, num_pages, max_pages, scale, softcap, window,
+            k_scale, v_scale, _dt(q), kv, _ptr(ws), ws_bytes, stream), what)
+    return out
+
+
+def paged_gather(k_pages, v_pages, page_table, count, head_dim, dtype, first=None, lengths=None, k_scale=1.0,
+                 v_scale=1.0):
+    """Rows first[b] .. first[b] + count - 1 of every sequence as dense (k, v)
+    [batch, Hkv, count, D] of `dtype`; rows at or past lengths[b] are zero."""
+    what = "paged_gather"
+    num_pages, hkv, page_size, kv = _pages(what, k_pages, v_pages, page_table, head_dim, dtype)
+    b = page_table.shape[0]
+    for t in (first, lengths):
+        if t is not None and (t.dtype != torch.int64 or tuple(t.shape) != (b,)):
+            raise ValueError("paged_gather: first and lengths must be int64 [batch]")
+    guard, stream = _on(what, k_pages, v_pages, page_table, first, lengths)
+    k = torch.empty(b, hkv, count, head_dim, dtype=dtype, device=k_pages.device)
+    v = torch.empty_like(k)
+    if dtype not in DTYPE_CODES:
+        raise ValueError(f"unsupported dtype {dtype}")
+    with guard:
+        check(lib().dli_sm100_paged_gather(
+            _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(first), _ptr(lengths), _ptr(k), _ptr(v), b, count,
+            hkv, head_dim, page_size, num_pages, page_table.shape[1], k_scale, v_scale, DTYPE_CODES[dtype], kv,
+            stream), what)
+    return k, v
 
 
 # ---- elementwise / data movement ------------------------------------------------

@@ -29,13 +29,15 @@ extern "C" {
 #define DLI_SM100_ABI_VERSION 1
 
 /* Element types. F32 and I64 are the reference's DType {Float32, Int64}
- * (include/dli/tensor.h:15); BF16/F16/I32 are additive. */
+ * (include/dli/tensor.h:15); BF16/F16/I32 are additive. FP4 names the 4-bit
+ * element type of paged KV caches and is accepted as `kv_dtype` only. */
 typedef enum dli_dtype {
   DLI_DTYPE_F32 = 0,
   DLI_DTYPE_I64 = 1,
   DLI_DTYPE_BF16 = 2,
   DLI_DTYPE_F16 = 3,
-  DLI_DTYPE_I32 = 4
+  DLI_DTYPE_I32 = 4,
+  DLI_DTYPE_FP4 = 5
 } dli_dtype;
 
 typedef enum dli_status {
@@ -265,6 +267,77 @@ dli_status dli_sm100_attention_kvcache_noalloc(const void* q, const void* cache_
                                                int64_t q_heads, int64_t kv_heads, int64_t capacity,
                                                int64_t head_dim, float scale, dli_dtype dtype,
                                                void* stream);
+
+/* ---- paged KV cache -----------------------------------------------------
+ * No counterpart in the reference, whose cache is one dense tensor per layer
+ * (src/kv_cache.cc:9-49). A pool of `num_pages` pages holds page_size rows
+ * (tokens) each; page_table[batch, max_pages] (int32) lists the pages of every
+ * sequence in order: row p of sequence b is row p mod page_size of page
+ * page_table[b, p / page_size]. page_size is 16, 32, 64 or 128. Sequences may
+ * share pages that no call appends to.
+ *
+ * k_pages / v_pages: [num_pages, kv_heads, page_size, head_dim] of kv_dtype ==
+ * dtype, or with kv_dtype = DLI_DTYPE_FP4 (head_dim a multiple of 16)
+ * [num_pages, kv_heads, page_size * head_dim * 9 / 16] bytes: per (page, head)
+ * the page_size rows of head_dim / 2 code bytes (E2M1, element 2i in the low
+ * half of byte i), then page_size rows of head_dim / 16 scale bytes (E4M3). A
+ * block of 16 elements with scale byte S stands for e2m1 * S * k_scale (v_scale
+ * for V). S is max|x / k_scale| / 6 rounded to E4M3 and the codes x / k_scale / S
+ * rounded to E2M1, both to nearest, ties to the even code, saturating; a block
+ * with a NaN stands for NaNs. k_scale and v_scale are ignored for other types.
+ *
+ * Batches are packed: the new tokens of sequence b are rows starts[b] ..
+ * starts[b+1]-1 of qkv / q / out (starts: int64 [batch + 1], at most max_new
+ * tokens each, none for an idle sequence), at positions positions[b],
+ * positions[b]+1, ... (positions: int64 [batch], the rows cached before the
+ * call). starts = NULL means max_new tokens of every sequence. `tokens` is the
+ * number of rows the buffers have; rows of no sequence are not touched.
+ * A sequence whose starts or positions are outside their bounds is skipped (its
+ * rows and pages are left as they were), and a page outside the pool is not
+ * written and read as zeros; both set the device error word. */
+
+/* Bytes of one page of K (or V) over all heads; 0 for unsupported arguments. */
+size_t dli_sm100_paged_kv_page_bytes(int64_t kv_heads, int64_t page_size, int64_t head_dim, dli_dtype kv_dtype);
+
+/* dli_sm100_qkv_rotary_cache for a packed batch and a paged cache: qkv[tokens,
+ * (Hq + 2 Hkv) * D] holds q heads, k heads, v heads per token; rotated q goes to
+ * q_out[tokens, Hq, D], rotated k and v into the pages. Into 4-bit pages k is
+ * rotated and both are quantised as if exactly (one rounding, to the codes). */
+dli_status dli_sm100_qkv_rotary_paged(const void* qkv, const float* cos_table, const float* sin_table,
+                                      const int64_t* positions, const int64_t* starts, const int32_t* page_table,
+                                      void* q_out, void* k_pages, void* v_pages, int64_t tokens, int64_t batch,
+                                      int64_t max_new, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                      int64_t pairs, int64_t table_rows, int64_t page_size, int64_t num_pages,
+                                      int64_t max_pages, float k_scale, float v_scale, dli_dtype dtype,
+                                      dli_dtype kv_dtype, void* stream);
+
+/* Attention over a paged cache: q/out [tokens, Hq, D], the token at position i
+ * of sequence b sees the cached rows j <= i (call it after the append), with
+ * window > 0 only i - window < j. Score of (i, j) in head h: x = scale * q . k;
+ * softcap > 0: x = softcap * tanh(x / softcap); slopes (float [Hq], NULL = none):
+ * x += slopes[h] * (j - i). scale <= 0 selects 1/sqrt(D). Hq must be a multiple
+ * of Hkv; head_dim <= 256. The workspace is scratch: nothing in it has to be
+ * initialised or kept, but calls that may overlap on the GPU need their own. */
+size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads,
+                                                int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                                int64_t max_pages, dli_dtype dtype, dli_dtype kv_dtype);
+dli_status dli_sm100_attention_paged(const void* q, const void* k_pages, const void* v_pages,
+                                     const int64_t* positions, const int64_t* starts, const int32_t* page_table,
+                                     const float* slopes, void* out, int64_t tokens, int64_t batch, int64_t max_new,
+                                     int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                     int64_t num_pages, int64_t max_pages, float scale, float softcap,
+                                     int64_t window, float k_scale, float v_scale, dli_dtype dtype,
+                                     dli_dtype kv_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows first[b] .. first[b] + count - 1 (first: int64 [batch], NULL = 0) of every
+ * sequence as dense k_out / v_out [batch, Hkv, count, D] of `dtype` (the values
+ * 4-bit pages stand for, rounded to dtype). Rows at or past lengths[b] (int64
+ * [batch], NULL = no limit but the table's) are written as zeros. */
+dli_status dli_sm100_paged_gather(const void* k_pages, const void* v_pages, const int32_t* page_table,
+                                  const int64_t* first, const int64_t* lengths, void* k_out, void* v_out,
+                                  int64_t batch, int64_t count, int64_t kv_heads, int64_t head_dim,
+                                  int64_t page_size, int64_t num_pages, int64_t max_pages, float k_scale,
+                                  float v_scale, dli_dtype dtype, dli_dtype kv_dtype, void* stream);
 
 /* ---- elementwise / data movement -------------------------------------- */
 
