@@ -38,6 +38,10 @@ bool fmha_required();
 dli_status make_map_4d(CUtensorMap* map, const void* base, bool bf16, const uint64_t (&dims)[4],
                        const uint64_t (&strides)[3], const uint32_t (&box)[4]);
 
+// The same over bytes, with the 64-byte swizzle or none.
+dli_status make_map_4d_bytes(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                             const uint32_t (&box)[4], bool swizzle64);
+
 // Launches the kernel on `stream` (fmha_supported() must hold). Returns
 // DLI_ERR_UNSUPPORTED, launching nothing, when a tensor map cannot be encoded.
 dli_status run_fmha_prefill(const FmhaArgs& a, dli_dtype dtype, cudaStream_t stream);

@@ -7,7 +7,7 @@
 #include <climits>
 #include <cmath>
 
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace dli_sm100 {
 namespace {
@@ -377,6 +377,9 @@ dli_status launch_attn_general(const PagedAttnArgs& a, cudaStream_t stream) {
   return check_launch("attention_paged");
 }
 
+// Query rows per KV head up to which the decode kernel serves a call.
+constexpr int64_t kDecodeRows = 32;
+
 // ---- argument checks -----------------------------------------------------------------
 int page_shift_of(int64_t page_size) {
   for (int s = 4; s <= 7; ++s)
@@ -543,9 +546,12 @@ extern "C" size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64
                                                            int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                            int64_t page_size, int64_t max_pages, dli_dtype dtype,
                                                            dli_dtype kv_dtype) {
-  (void)tokens, (void)batch, (void)max_new, (void)q_heads, (void)kv_heads, (void)head_dim, (void)page_size;
-  (void)max_pages, (void)dtype, (void)kv_dtype;
-  return 0;
+  (void)kv_dtype;
+  if (tokens <= 0 || batch <= 0 || max_new <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0) return 0;
+  if (page_shift_of(page_size) < 0 || max_pages <= 0 || max_pages > (1ll << 30) / page_size) return 0;
+  if ((dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) || (head_dim != 64 && head_dim != 128)) return 0;
+  if (q_heads / kv_heads * max_new > kDecodeRows) return 0;
+  return paged_decode_workspace(batch, kv_heads, q_heads / kv_heads, max_new, head_dim, max_pages * page_size);
 }
 
 extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pages, const void* v_pages,
@@ -569,7 +575,6 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
     return fail(DLI_ERR_INVALID_ARGUMENT, "attention_paged: softcap and window must not be negative, scale finite");
   if (head_dim > 256) return fail(DLI_ERR_UNSUPPORTED, "attention_paged: head_dim > 256");
   if (batch == 0 || max_new == 0 || tokens == 0) return ok();
-  (void)workspace, (void)workspace_bytes;
   PagedAttnArgs a{};
   a.seqs = make_seqs(positions, starts, page_table, tokens, batch, max_new, page_size, num_pages, max_pages);
   a.q = q;
@@ -586,6 +591,8 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
   a.scale = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim))) * (fp4 ? k_scale : 1.f);
   a.softcap = softcap;
   a.v_scale = fp4 ? v_scale : 1.f;
+  if (a.group * max_new <= kDecodeRows && paged_decode_serves(a, dtype, kv_dtype))
+    return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
   dli_status run = DLI_OK;
   st = dispatch_float(dtype, what, [&](auto tag) {
     using T = decltype(tag);

@@ -1,0 +1,876 @@
+// Attention of few new tokens over a paged KV cache (decode steps, short
+// speculative runs): tensor cores by mma.sync, K/V pages by TMA, 16-bit or 4-bit
+// pages, head dims 64 and 128.
+//
+// A unit is one row tile (8 or 16 query rows: the new tokens of a sequence times
+// the query heads of one KV head) over all its visible keys. S^T = K Q^T puts 16
+// keys on the m16 side and the rows on n8, O^T = V^T P^T likewise, so 7 heads
+// waste an eighth of the tensor work; each K/V byte is fetched once per tile.
+//
+// The work of a call is the list of all key blocks of all units, in order; CTA c
+// of G takes the c-th of G equal shares of it, whatever the sequences' lengths
+// are (a ragged batch keeps every SM busy to the end). A unit that lies within
+// one share is finished there; of the others each CTA stores its part's (max,
+// sum, O) in the workspace and a second kernel merges the parts in order
+// (deterministic). A call whose units cannot be long runs one CTA per unit and
+// needs no merge.
+//
+// One producer warp walks the page table and issues the TMA boxes of each block
+// (a page's rows of one head; boxes past the sequence or of a bad page read as
+// zeros) into a ring of stages; four consumer warps take 16 keys each of every
+// 64 keys. Every wait is bounded.
+//
+// 4-bit pages: codes arrive by TMA as bytes and become halves in registers, in
+// the order of the MMA fragments: E2M1 x E4M3 has 6 significant bits, so the
+// products are exact, and the MMA runs in f16 for every model type. q is scaled
+// by a power of two per row for that, which is exact too.
+#include <algorithm>
+#include <climits>
+#include <map>
+#include <mutex>
+#include <tuple>
+
+#include "mma_sync.cuh"
+#include "paged_attn.cuh"
+#include "tcgen05.cuh"
+
+namespace dli_sm100 {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kDecodeThreads = 160;  // 4 consumer warps and the producer
+
+struct DecodeArgs {
+  PagedAttnArgs a;
+  int tiles_max;        // row tiles of a sequence of max_new tokens
+  int split;            // 0: one CTA per unit
+  int min_blocks;       // split: no CTA takes fewer key blocks (but the last)
+  float* part_o;        // [2 G][rows][D]
+  float2* part_ml;      // [2 G][rows]: running maximum (log2) and sum
+  int2* unit_parts;     // [B * Hkv * tiles_max]: first slot, parts (0: finished in the main kernel)
+};
+
+template <typename T, typename KV, int D, int NT>
+struct DecodeLayout {
+  static constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
+  static constexpr int R = 8 * NT;
+  static constexpr int BN = kFp4 ? 128 : 64;  // keys per block
+  static constexpr int SUB = BN / 64;         // 16-key groups per warp and block
+  static constexpr int kCodes = kFp4 ? BN * D / 2 : BN * D * 2;  // code or element bytes of K (or V)
+  static constexpr int kScales = kFp4 ? BN * 8 : 0;  // a TMA box of 64 bytes (D 64, pages of 16) takes 128
+  static constexpr int kStage = 2 * (kCodes + kScales);
+  static constexpr int kStageTx = 2 * (kCodes + (kFp4 ? BN * D / 16 : 0));
+  static constexpr int kStages = kFp4 ? (D == 128 ? 5 : 8) : (D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 6 : 5));
+  static constexpr int DH = 64;  // dims that the four warps merge at a time
+  static constexpr int kMergeOff = kStages * kStage;
+  static constexpr int kMerge = 4 * R * DH * 4;
+  static constexpr int kMlOff = kMergeOff + kMerge;
+  static constexpr int kMl = 2 * 4 * R * 4;
+  static constexpr int kBarOff = kMlOff + kMl;
+  static constexpr int kBytes = kBarOff + 2 * kStages * 8 + 1024;  // the ring's base is rounded up to 1 KiB
+  static_assert(kStage % 1024 == 0, "stage alignment");
+};
+
+// What one sequence contributes to the list of key blocks.
+struct SeqWork {
+  SeqRows rows;
+  int tiles, blocks, block0, kv_len, key_lo;
+};
+
+template <int BN, int R>
+__device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int b, bool report) {
+  SeqWork w;
+  w.rows = seq_rows(a.seqs, b, report);
+  w.kv_len = w.rows.past + w.rows.n;
+  w.key_lo = a.window <= w.rows.past ? w.rows.past - a.window + 1 : 0;
+  w.tiles = (w.rows.n * a.group + R - 1) / R;
+  w.block0 = w.key_lo / BN;
+  w.blocks = (w.kv_len + BN - 1) / BN - w.block0;
+  return w;
+}
+
+struct Segment {
+  int b, kvh, rt, block, blocks;  // key blocks [block, block + blocks) of the unit
+  bool whole;
+  int slot;        // of the part, when not whole
+  SeqWork w;
+  int64_t unit_w;  // the unit's first place in the work list
+};
+
+// Walks the segments of a CTA's share; every warp runs its own copy.
+template <int BN, int R>
+struct Walker {
+  const DecodeArgs& d;
+  int64_t w, w_end, w0, base, total;
+  int64_t ctas;  // CTAs with work
+  int b, next;
+  SeqWork sw;
+
+  __device__ __forceinline__ int64_t work_of(const SeqWork& s) const {
+    return static_cast<int64_t>(d.a.hkv) * s.tiles * s.blocks;
+  }
+
+  __device__ Walker(const DecodeArgs& args, int lane) : d(args) {
+    base = 0;
+    b = -1;
+    next = 0;
+    total = 0;
+    if (!d.split) {
+      w = 0;
+      w_end = 1;
+      return;
+    }
+    const int batch = d.a.seqs.batch;
+    for (int c = 0; c < batch; c += 32) {
+      int64_t mine = 0;
+      if (c + lane < batch) mine = work_of(seq_work<BN, R>(d.a, c + lane, blockIdx.x == 0));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      total += mine;
+    }
+    const int64_t most = (total + d.min_blocks - 1) / d.min_blocks;
+    ctas = most < static_cast<int64_t>(gridDim.x) ? (most > 0 ? most : 1) : static_cast<int64_t>(gridDim.x);
+    w0 = w = begin_of(blockIdx.x);
+    w_end = begin_of(blockIdx.x + 1ll);
+    if (w >= w_end) return;
+    // the sequence that holds w
+    for (int c = 0; c < batch; c += 32) {
+      int64_t mine = 0;
+      if (c + lane < batch) mine = work_of(seq_work<BN, R>(d.a, c + lane, false));
+      int64_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, base + upto <= w);
+      const int k = __popc(past);  // sequences of this chunk that end before w
+      if (k < 32) {
+        const int64_t before = __shfl_sync(0xffffffffu, upto - mine, k);
+        b = c + k;
+        base += before;
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    sw = seq_work<BN, R>(d.a, b, false);
+  }
+  __device__ __forceinline__ int64_t begin_of(int64_t c) const {
+    return c >= ctas ? total : c * (total / ctas) + min(c, total % ctas);
+  }
+  __device__ __forceinline__ int64_t cta_of(int64_t at) const {  // the CTA whose share holds `at`
+    const int64_t q = total / ctas, r = total % ctas;
+    return at < r * (q + 1) ? at / (q + 1) : r + (at - r * (q + 1)) / q;
+  }
+
+  __device__ bool get(Segment& s) {
+    if (!d.split) {
+      if (w >= w_end) return false;
+      w = w_end;
+      const int per = d.a.hkv * d.tiles_max;
+      s.b = blockIdx.x / per;
+      const int u = blockIdx.x - s.b * per;
+      s.kvh = u / d.tiles_max;
+      s.rt = u - s.kvh * d.tiles_max;
+      s.w = seq_work<BN, R>(d.a, s.b, u == 0);
+      if (s.rt >= s.w.tiles) return false;
+      s.block = s.w.block0;
+      s.blocks = s.w.blocks;
+      s.whole = true;
+      return true;
+    }
+    if (w >= w_end) return false;
+    while (w >= base + work_of(sw)) {
+      base += work_of(sw);
+      ++b;
+      sw = seq_work<BN, R>(d.a, b, false);
+    }
+    const int64_t rel = w - base;
+    const int unit = static_cast<int>(rel / sw.blocks), blk = static_cast<int>(rel - static_cast<int64_t>(unit) * sw.blocks);
+    s.b = b;
+    s.kvh = unit / sw.tiles;
+    s.rt = unit - s.kvh * sw.tiles;
+    s.w = sw;
+    s.block = sw.block0 + blk;
+    s.blocks = static_cast<int>(min(static_cast<int64_t>(sw.blocks - blk), w_end - w));
+    s.whole = s.blocks == sw.blocks;
+    s.slot = 2 * blockIdx.x + (w == w0 ? 0 : 1);
+    s.unit_w = base + static_cast<int64_t>(unit) * sw.blocks;
+    w += s.blocks;
+    return true;
+  }
+};
+
+// Byte offset of (key row, 16-bit column) in a K or V stage of D/64 boxes of
+// [64 keys][64 elements] with the 128-byte swizzle.
+__device__ __forceinline__ int swz128(int row, int col) {
+  return (col >> 6) * (64 * 128) + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+
+template <typename T, typename KV, int D, int NT>
+__global__ void __launch_bounds__(kDecodeThreads)
+    attn_paged_decode_kernel(const DecodeArgs d, const __grid_constant__ CUtensorMap tk,
+                             const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tks,
+                             const __grid_constant__ CUtensorMap tvs) {
+  using L = DecodeLayout<T, KV, D, NT>;
+  using MT = typename std::conditional<L::kFp4, __half, T>::type;  // MMA operand type
+  constexpr int BN = L::BN, SUB = L::SUB, R = L::R, ST = L::kStages;
+  extern __shared__ uint8_t smem_base[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_base) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty = full + ST;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedAttnArgs& a = d.a;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4);
+    }
+    mbar_fence_init();
+  }
+  if (threadIdx.x == 128) {
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+  }
+  __syncthreads();
+  pdl_wait();
+  pdl_trigger();
+  Walker<BN, R> walk(d, lane);
+  Segment seg;
+  // scale bytes of row r: r * D/16 + (r / 16) * scale_pad
+  const int scale_pad = L::kFp4 && D == 64 && a.seqs.page_shift == 4 ? 64 : 0;
+
+  if (warp == 4) {
+    // ---- producer: page ids (32 at a time, the next 32 already asked for) and TMA boxes
+    const int shift = a.seqs.page_shift, page_rows = 1 << shift;
+    const int box_rows = min(page_rows, BN), boxes = BN / box_rows;
+    int it = 0, last_it = 0;
+    bool alive = true;
+    while (alive && walk.get(seg)) {
+      const int32_t* ids = a.seqs.page_table + seg.b * a.seqs.max_pages;
+      const int last_page = (seg.w.kv_len - 1) >> shift;
+      const int none = static_cast<int>(a.seqs.num_pages);  // outside the map: reads as zeros
+      auto fetch = [&](int chunk) {
+        const int i = chunk * 32 + lane;
+        return i <= last_page ? ids[i] : none;
+      };
+      int chunk = ((seg.block * BN) >> shift) >> 5;
+      int cur = fetch(chunk), nxt = fetch(chunk + 1);
+      for (int j = 0; j < seg.blocks; ++j, ++it) {
+        const int key0 = (seg.block + j) * BN;
+        const int first = key0 >> shift;
+        if ((first >> 5) != chunk) {
+          ++chunk;
+          cur = nxt;
+          nxt = fetch(chunk + 1);
+        }
+        int page = __shfl_sync(0xffffffffu, cur, (first + lane) & 31);
+        if (first + lane > last_page) page = none;
+        else if (lane < boxes && (page < 0 || page >= none)) {
+          set_device_error(a.seqs.err, kDevErrPageIndex);
+          page = none;
+        }
+        const int st = it % ST;
+        const bool free_stage = mbar_wait(&empty[st], ((it / ST) & 1) ^ 1);
+        if (!__all_sync(0xffffffffu, free_stage)) {
+          if (lane == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
+          alive = false;
+          break;
+        }
+        uint8_t* sk = smem + st * L::kStage;
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], L::kStageTx);
+        __syncwarp();
+        if (lane < boxes) {
+          const int row = key0 & (page_rows - 1);  // 0 unless a page holds several blocks
+          const int at = lane * box_rows;
+          if constexpr (L::kFp4) {
+            uint8_t* sv = sk + L::kCodes;
+            uint8_t* ss = sv + L::kCodes;
+            tma_load_4d(sk + at * (D / 2), &tk, 0, row, seg.kvh, page, &full[st]);
+            tma_load_4d(sv + at * (D / 2), &tv, 0, row, seg.kvh, page, &full[st]);
+            const int sat = at * (D / 16) + lane * scale_pad;
+            tma_load_4d(ss + sat, &tks, 0, 0, seg.kvh, page, &full[st]);
+            tma_load_4d(ss + L::kScales + sat, &tvs, 0, 0, seg.kvh, page, &full[st]);
+          } else {
+            uint8_t* sv = sk + L::kCodes;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              tma_load_4d(sk + c * (64 * 128) + at * 128, &tk, c * 64, row, seg.kvh, page, &full[st]);
+              tma_load_4d(sv + c * (64 * 128) + at * 128, &tv, c * 64, row, seg.kvh, page, &full[st]);
+            }
+          }
+        }
+        __syncwarp();
+        last_it = it + 1;
+      }
+    }
+    // no copy may still be writing shared memory when the CTA exits
+    for (int i = max(0, last_it - ST); i < last_it; ++i) mbar_wait(&full[i % ST], (i / ST) & 1);
+    return;
+  }
+
+  // ---- consumers
+  const int g = lane >> 2, t = lane & 3;
+  float* merge = reinterpret_cast<float*>(smem + L::kMergeOff);
+  float* wm = reinterpret_cast<float*>(smem + L::kMlOff);  // [4][R]
+  float* wl = wm + 4 * R;
+  // MMA key row x of a 16-key group holds key perm(x): 4-bit V reads of the four
+  // lanes of a quad then fall into different banks
+  auto perm = [](int x) { return L::kFp4 ? (D == 128 ? x ^ ((x >> 1) & 1) : (x & 8) | ((x & 6) >> 1) | ((x & 1) << 2)) : x; };
+  const float cap_out = a.softcap * kLog2e;
+  const float base_scale = a.softcap > 0.f ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
+  int it = 0;
+  bool alive = true;
+
+  while (walk.get(seg)) {
+    const int rows_left = seg.w.rows.n * a.group - seg.rt * R;
+    const int rows = min(rows_left, R);
+    // the two score columns of this thread in each n8 tile: rows nt * 8 + 2t + e
+    int pos[NT][2];
+    float slope[NT][2], rscale[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = nt * 8 + 2 * t + e;
+        const int rr = seg.rt * R + min(r, rows - 1);
+        const int tok = rr / a.group;
+        pos[nt][e] = seg.w.rows.past + tok;
+        slope[nt][e] = a.slopes ? a.slopes[seg.kvh * a.group + rr - tok * a.group] * kLog2e : 0.f;
+        rscale[nt][e] = base_scale;
+      }
+    // Q^T fragments, rows past the tile zero
+    constexpr int KK = D / 16;
+    uint32_t qf[NT][KK][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g;
+      const bool valid = r < rows;
+      const int rr = seg.rt * R + (valid ? r : 0);
+      const int tok = rr / a.group, h = seg.kvh * a.group + rr - tok * a.group;
+      const T* q = static_cast<const T*>(a.q) + ((seg.w.rows.row0 + tok) * a.hq + h) * D;
+      if constexpr (L::kFp4) {
+        // dims [t * D/4, (t + 1) * D/4) in order: the k order of the MMAs is that of the code bytes
+        float x[D / 4];
+        float big = 0.f;
+#pragma unroll
+        for (int v = 0; v < D / 32; ++v) {
+          const Vec16<T> in = load16(q + t * (D / 4) + v * 8);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[v * 8 + j] = valid ? to_f32(in.e[j]) : 0.f;
+            big = fmaxf(big, fabsf(x[v * 8 + j]));
+          }
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // 2^-e with 2^e <= max|q| < 2^(e+1), e within +-120
+        const int e = max(-120, min(120, static_cast<int>((__float_as_uint(big) >> 23) & 255u) - 127));
+        const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+        const float up = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+          qf[nt][j / 2][j & 1] = pack16<__half>(x[2 * j] * down, x[2 * j + 1] * down);
+        rscale[nt][0] *= __shfl_sync(0xffffffffu, up, (2 * t) * 4);
+        rscale[nt][1] *= __shfl_sync(0xffffffffu, up, (2 * t + 1) * 4);
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            qf[nt][kk][e] = valid ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + e * 8 + 2 * t) : 0u;
+      }
+    }
+    float o[NT][KK][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < KK; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+
+    for (int j = 0; j < seg.blocks; ++j, ++it) {
+      const int st = it % ST;
+      if (alive) {
+        const bool got = mbar_wait(&full[st], (it / ST) & 1);
+        if (!__all_sync(0xffffffffu, got)) {
+          if (lane == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
+          alive = false;  // the remaining blocks are skipped, every barrier is still met
+        }
+      }
+      if (!alive) continue;
+      uint8_t* sk = smem + st * L::kStage;
+      uint8_t* sv = sk + L::kCodes;
+      const int blk_key = (seg.block + j) * BN;
+
+      // S^T = K Q^T
+      float sc[SUB][NT][4];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const int kw = u * 64 + warp * 16;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[u][nt][0] = sc[u][nt][1] = sc[u][nt][2] = sc[u][nt][3] = 0.f;
+        if constexpr (L::kFp4) {
+          const int r0 = kw + perm(g), r1 = kw + perm(g + 8);
+          const uint8_t* ss = sv + L::kCodes;
+          uint32_t w0[D / 32], w1[D / 32], s0[D / 64], s1[D / 64];
+          if constexpr (D == 128) {
+            const uint4 c0 = *reinterpret_cast<const uint4*>(sk + r0 * 64 + ((t ^ ((r0 >> 1) & 3)) << 4));
+            const uint4 c1 = *reinterpret_cast<const uint4*>(sk + r1 * 64 + ((t ^ ((r1 >> 1) & 3)) << 4));
+            w0[0] = c0.x, w0[1] = c0.y, w0[2] = c0.z, w0[3] = c0.w;
+            w1[0] = c1.x, w1[1] = c1.y, w1[2] = c1.z, w1[3] = c1.w;
+            const uint32_t e0 = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(ss + r0 * 8 + 2 * t));
+            const uint32_t e1 = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(ss + r1 * 8 + 2 * t));
+            s0[0] = __byte_perm(e0, e0, 0x1010), s0[1] = __byte_perm(e0, e0, 0x3232);
+            s1[0] = __byte_perm(e1, e1, 0x1010), s1[1] = __byte_perm(e1, e1, 0x3232);
+          } else {
+            const uint2 c0 = *reinterpret_cast<const uint2*>(sk + r0 * 32 + t * 8);
+            const uint2 c1 = *reinterpret_cast<const uint2*>(sk + r1 * 32 + t * 8);
+            w0[0] = c0.x, w0[1] = c0.y;
+            w1[0] = c1.x, w1[1] = c1.y;
+            const uint32_t e =
+                e4m3x2_to_half2(static_cast<uint32_t>(ss[r0 * 4 + (r0 >> 4) * scale_pad + t]) |
+                                (static_cast<uint32_t>(ss[r1 * 4 + (r1 >> 4) * scale_pad + t]) << 8));
+            s0[0] = __byte_perm(e, e, 0x1010);
+            s1[0] = __byte_perm(e, e, 0x3232);
+          }
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {  // a code word: two MMAs
+            const uint32_t x0 = s0[i / 2], x1 = s1[i / 2];
+            const uint32_t a00 = mul_half2(e2m1x2_to_half2<0>(w0[i]), x0), a01 = mul_half2(e2m1x2_to_half2<1>(w0[i]), x0);
+            const uint32_t a02 = mul_half2(e2m1x2_to_half2<2>(w0[i]), x0), a03 = mul_half2(e2m1x2_to_half2<3>(w0[i]), x0);
+            const uint32_t a10 = mul_half2(e2m1x2_to_half2<0>(w1[i]), x1), a11 = mul_half2(e2m1x2_to_half2<1>(w1[i]), x1);
+            const uint32_t a12 = mul_half2(e2m1x2_to_half2<2>(w1[i]), x1), a13 = mul_half2(e2m1x2_to_half2<3>(w1[i]), x1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816<MT>(sc[u][nt], a00, a10, a01, a11, qf[nt][2 * i][0], qf[nt][2 * i][1]);
+              mma_16816<MT>(sc[u][nt], a02, a12, a03, a13, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+            }
+          }
+        } else {
+          const uint32_t ks = smem_u32(sk);
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            uint32_t f[4];
+            ldmatrix_x4(f, ks + swz128(kw + (lane & 15), kk * 16 + (lane >> 4) * 8));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816<MT>(sc[u][nt], f[0], f[1], f[2], f[3], qf[nt][kk][0], qf[nt][kk][1]);
+          }
+        }
+      }
+
+      // scores in log2 units, cap, bias and mask
+      float mx[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+      const bool edge = blk_key + BN > seg.w.rows.past + 1 || blk_key < seg.w.kv_len - a.window;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = i & 1;
+            const int key = blk_key + u * 64 + warp * 16 + perm(g + (i >> 1) * 8);
+            float x = sc[u][nt][i] * rscale[nt][e];
+            if (a.softcap > 0.f) x = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(x));
+            if (a.slopes) x = fmaf(slope[nt][e], static_cast<float>(key - pos[nt][e]), x);
+            if (edge && (key > pos[nt][e] || key <= pos[nt][e] - a.window)) x = -INFINITY;
+            sc[u][nt][i] = x;
+            mx[nt][e] = fmaxf(mx[nt][e], x);
+          }
+      bool moved = false;
+      float alpha[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], s));
+          const float top = fmaxf(m[nt][e], mx[nt][e]);
+          alpha[nt][e] = m[nt][e] == top ? 1.f : exp2_approx(m[nt][e] - top);  // m = -inf: 0
+          moved |= m[nt][e] != top;
+          m[nt][e] = top;
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          l[nt][0] *= alpha[nt][0];
+          l[nt][1] *= alpha[nt][1];
+#pragma unroll
+          for (int i = 0; i < KK; ++i) {
+            o[nt][i][0] *= alpha[nt][0];
+            o[nt][i][1] *= alpha[nt][1];
+            o[nt][i][2] *= alpha[nt][0];
+            o[nt][i][3] *= alpha[nt][1];
+          }
+        }
+      }
+
+      // O^T += V^T P^T
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const int kw = u * 64 + warp * 16;
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          // a row that has seen no key yet keeps m = -inf: its p are 0
+          const float n0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], n1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+          const float p00 = exp2_approx(sc[u][nt][0] - n0), p01 = exp2_approx(sc[u][nt][1] - n1);
+          const float p10 = exp2_approx(sc[u][nt][2] - n0), p11 = exp2_approx(sc[u][nt][3] - n1);
+          l[nt][0] += p00 + p10;  // this thread's keys; summed over the warp at the end
+          l[nt][1] += p01 + p11;
+          pb[nt][0] = movmatrix_trans(pack16<MT>(p00, p01));
+          pb[nt][1] = movmatrix_trans(pack16<MT>(p10, p11));
+        }
+        const int key_first = blk_key + kw;
+        const bool stale = key_first + 16 > seg.w.kv_len || key_first < seg.w.key_lo;
+        if constexpr (L::kFp4) {
+          const uint8_t* ss = sv + L::kCodes + L::kScales;
+          const int rw[4] = {kw + perm(2 * t), kw + perm(2 * t + 1), kw + perm(2 * t + 8), kw + perm(2 * t + 9)};
+          uint32_t c[4][D / 64], sb[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (D == 128) {
+              const uint2 v = *reinterpret_cast<const uint2*>(sv + rw[k] * 64 + (((g >> 1) ^ ((rw[k] >> 1) & 3)) << 4) + (g & 1) * 8);
+              c[k][0] = v.x;
+              c[k][1] = v.y;
+              sb[k] = ss[rw[k] * 8 + g];
+            } else {
+              c[k][0] = *reinterpret_cast<const uint32_t*>(sv + rw[k] * 32 + g * 4);
+              sb[k] = ss[rw[k] * 4 + (rw[k] >> 4) * scale_pad + (g >> 1)];
+            }
+            // a row that is not of the sequence may hold a NaN scale
+            if (stale && (blk_key + rw[k] >= seg.w.kv_len || blk_key + rw[k] < seg.w.key_lo)) sb[k] = 0u;
+          }
+          const uint32_t s01 = e4m3x2_to_half2(sb[0] | (sb[1] << 8)), s23 = e4m3x2_to_half2(sb[2] | (sb[3] << 8));
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            // nibble pairs (key 2t, key 2t+1) of the even and of the odd dims
+            const uint32_t ev0 = (c[0][i] & 0x0F0F0F0Fu) | ((c[1][i] << 4) & 0xF0F0F0F0u);
+            const uint32_t od0 = ((c[0][i] >> 4) & 0x0F0F0F0Fu) | (c[1][i] & 0xF0F0F0F0u);
+            const uint32_t ev1 = (c[2][i] & 0x0F0F0F0Fu) | ((c[3][i] << 4) & 0xF0F0F0F0u);
+            const uint32_t od1 = ((c[2][i] >> 4) & 0x0F0F0F0Fu) | (c[3][i] & 0xF0F0F0F0u);
+#define DLI_FP4_V(B)                                                                                                 \
+  {                                                                                                                  \
+    const uint32_t f0 = mul_half2(e2m1x2_to_half2<B>(ev0), s01), f1 = mul_half2(e2m1x2_to_half2<B>(od0), s01);      \
+    const uint32_t f2 = mul_half2(e2m1x2_to_half2<B>(ev1), s23), f3 = mul_half2(e2m1x2_to_half2<B>(od1), s23);      \
+    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt)                                                                \
+        mma_16816<MT>(o[nt][4 * i + B], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);                                       \
+  }
+            DLI_FP4_V(0)
+            DLI_FP4_V(1)
+            DLI_FP4_V(2)
+            DLI_FP4_V(3)
+#undef DLI_FP4_V
+          }
+        } else {
+          if (stale) {
+            // V rows that are not of the sequence may hold anything: a zero weight must meet a zero
+            for (int c = lane; c < 16 * (D / 8); c += 32) {
+              const int r = c / (D / 8), ch = c - r * (D / 8);
+              if (key_first + r >= seg.w.kv_len || key_first + r < seg.w.key_lo)
+                *reinterpret_cast<uint4*>(sv + swz128(kw + r, ch * 8)) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();  // before the stage is given back to the TMA
+            __syncwarp();
+          }
+          const uint32_t vs = smem_u32(sv);
+#pragma unroll
+          for (int i = 0; i < KK; ++i) {
+            uint32_t f[4];
+            ldmatrix_x4_trans(f, vs + swz128(kw + (lane & 7) + (lane >> 4) * 8, i * 16 + ((lane >> 3) & 1) * 8));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816<MT>(o[nt][i], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+
+    // ---- merge the four warps in order, then store the rows or the part
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], s);
+        if (g == 0) {
+          wm[warp * R + nt * 8 + 2 * t + e] = m[nt][e];
+          wl[warp * R + nt * 8 + 2 * t + e] = l[nt][e];
+        }
+      }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    constexpr int DH = L::DH;
+#pragma unroll
+    for (int half = 0; half < D / DH; ++half) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = nt * 8 + 2 * t + e;
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) top = fmaxf(top, wm[w * R + r]);
+          f[e] = m[nt][e] == -INFINITY ? 0.f : exp2_approx(m[nt][e] - top);
+        }
+#pragma unroll
+        for (int i = 0; i < KK; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // 16-bit: dims i * 16 + g (+ 8); 4-bit: g * D/8 + 2 i (+ 1)
+            const int dim = L::kFp4 ? g * (D / 8) + 2 * i + (k >> 1) : i * 16 + g + (k >> 1) * 8;
+            if (D == DH || dim / DH == half)
+              merge[(warp * R + nt * 8 + 2 * t + (k & 1)) * DH + (dim - half * DH)] = o[nt][i][k] * f[k & 1];
+          }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int c = threadIdx.x; c < rows * (DH / 4); c += 128) {
+        const int r = c / (DH / 4), x = (c - r * (DH / 4)) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = -INFINITY, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, wm[w * R + r]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(&merge[(w * R + r) * DH + x]);
+          sum.x += v.x;
+          sum.y += v.y;
+          sum.z += v.z;
+          sum.w += v.w;
+          const float mw = wm[w * R + r];
+          if (mw != -INFINITY) den += wl[w * R + r] * exp2_approx(mw - top);
+        }
+        const int dim = half * DH + x;
+        if (seg.whole) {
+          const int rr = seg.rt * R + r, tok = rr / a.group, h = seg.kvh * a.group + rr - tok * a.group;
+          const float inv = a.v_scale / den;
+          uint2 v;
+          v.x = pack16<T>(sum.x * inv, sum.y * inv);
+          v.y = pack16<T>(sum.z * inv, sum.w * inv);
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((seg.w.rows.row0 + tok) * a.hq + h) * D + dim) = v;
+        } else {
+          *reinterpret_cast<float4*>(d.part_o + (static_cast<int64_t>(seg.slot) * R + r) * D + dim) = sum;
+          if (dim == 0) d.part_ml[static_cast<int64_t>(seg.slot) * R + r] = make_float2(top, den);
+        }
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
+    if (d.split && threadIdx.x == 0 && seg.block == seg.w.block0) {
+      // the unit's first CTA says which slots hold its parts
+      int2 parts = make_int2(0, 0);
+      if (!seg.whole)
+        parts = make_int2(seg.slot, static_cast<int>(walk.cta_of(seg.unit_w + seg.w.blocks - 1) - blockIdx.x) + 1);
+      d.unit_parts[(static_cast<int64_t>(seg.b) * a.hkv + seg.kvh) * d.tiles_max + seg.rt] = parts;
+    }
+  }
+}
+
+// Merges the parts of the units that were split, in order: slot 0 of the parts is
+// the unit's first, the others are the first slots of the CTAs after it.
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(256) attn_paged_combine_kernel(const DecodeArgs d) {
+  DLI_PDL_ENTRY();
+  const PagedAttnArgs& a = d.a;
+  const int u = blockIdx.x, rt = u % d.tiles_max, kvh = u / d.tiles_max % a.hkv, b = u / d.tiles_max / a.hkv;
+  const SeqRows sr = seq_rows(a.seqs, b, false);
+  const int rows = min(sr.n * a.group - rt * R, R);
+  if (rows <= 0) return;
+  const int2 parts = d.unit_parts[u];
+  if (parts.y == 0) return;
+  const int cta = parts.x / 2;
+  for (int c = threadIdx.x; c < rows * (D / 4); c += 256) {
+    const int r = c / (D / 4), x = (c - r * (D / 4)) * 4;
+    float top = -INFINITY, den = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < parts.y; ++p) {
+      const int64_t slot = p == 0 ? parts.x : 2 * (cta + p);
+      top = fmaxf(top, d.part_ml[slot * R + r].x);
+    }
+#pragma unroll 4
+    for (int p = 0; p < parts.y; ++p) {
+      const int64_t slot = p == 0 ? parts.x : 2 * (cta + p);
+      const float2 ml = d.part_ml[slot * R + r];
+      const float4 v = *reinterpret_cast<const float4*>(d.part_o + (slot * R + r) * D + x);
+      const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+      den += ml.y * f;
+      sum.x += v.x * f;
+      sum.y += v.y * f;
+      sum.z += v.z * f;
+      sum.w += v.w * f;
+    }
+    const int rr = rt * R + r, tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
+    const float inv = a.v_scale / den;
+    uint2 v;
+    v.x = pack16<T>(sum.x * inv, sum.y * inv);
+    v.y = pack16<T>(sum.z * inv, sum.w * inv);
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((sr.row0 + tok) * a.hq + h) * D + x) = v;
+  }
+}
+
+// ---- host ------------------------------------------------------------------------
+
+// CTAs that are resident at once, per kernel and device.
+int resident_ctas(const void* kernel, int smem) {
+  static std::mutex mu;
+  static std::map<std::pair<int, const void*>, int> cache;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = cache.find({dev, kernel});
+  if (it != cache.end()) return it->second;
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kDecodeThreads, smem) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  n *= sm_count();
+  cache[{dev, kernel}] = n;
+  return n;
+}
+
+struct DecodePlan {
+  int nt, tiles_max;
+  bool split;
+  int64_t units, grid;
+  size_t part_o, part_ml, workspace;
+};
+
+// Shares of a split call are at least kMinKeys keys; a call whose sequences cannot
+// exceed kWholeKeys runs one CTA per unit.
+constexpr int kWholeKeys = 512;
+constexpr int kMinKeys = 256;
+constexpr int kMaxCtasPerSm = 2;
+
+DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys) {
+  DecodePlan p{};
+  const int64_t rows = group * max_new;
+  p.nt = rows <= 8 ? 1 : 2;
+  p.tiles_max = static_cast<int>(ceil_div(rows, 8 * p.nt));
+  p.units = batch * hkv * p.tiles_max;
+  p.split = max_keys > kWholeKeys;
+  p.grid = p.split ? static_cast<int64_t>(sm_count()) * kMaxCtasPerSm : p.units;
+  if (p.split) {
+    const int64_t r = 8 * p.nt;
+    p.part_o = static_cast<size_t>(2 * p.grid * r * head_dim) * 4;
+    p.part_ml = static_cast<size_t>(2 * p.grid * r) * 8;
+    p.workspace = p.part_o + p.part_ml + static_cast<size_t>(p.units) * 8;
+  }
+  return p;
+}
+
+template <typename T, typename KV, int D, int NT>
+dli_status launch_paged_decode(const PagedAttnArgs& a, const DecodePlan& plan, void* workspace, cudaStream_t stream) {
+  using L = DecodeLayout<T, KV, D, NT>;
+  CUtensorMap tk, tv, tks, tvs;
+  const int64_t page_rows = 1ll << a.seqs.page_shift;
+  dli_status st = make_page_maps(a, L::kFp4, D, static_cast<int>(std::min<int64_t>(page_rows, L::BN)), std::is_same<T, __nv_bfloat16>::value,
+                                 &tk, &tv, &tks, &tvs);
+  if (st != DLI_OK) return st;
+  auto kern = attn_paged_decode_kernel<T, KV, D, NT>;
+  st = ensure_smem(reinterpret_cast<const void*>(kern), L::kBytes, "attention_paged");
+  if (st != DLI_OK) return st;
+  DecodeArgs d{};
+  d.a = a;
+  d.tiles_max = plan.tiles_max;
+  d.split = plan.split ? 1 : 0;
+  d.min_blocks = kMinKeys / L::BN;
+  int64_t grid = plan.grid;
+  if (plan.split) {
+    d.part_o = static_cast<float*>(workspace);
+    d.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.part_o);
+    d.unit_parts = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + plan.part_o + plan.part_ml);
+    grid = std::min<int64_t>(grid, std::max(1, resident_ctas(reinterpret_cast<const void*>(kern), L::kBytes)));
+  }
+  launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kDecodeThreads), L::kBytes, stream, d, tk, tv, tks, tvs);
+  if (plan.split)
+    launch_pdl(attn_paged_combine_kernel<T, D, L::R>, dim3(static_cast<unsigned>(plan.units)), dim3(256), 0, stream, d);
+  return check_launch("attention_paged", plan.split ? 2 : 1);
+}
+
+template <typename T, typename KV>
+dli_status launch_paged_decode_nd(const PagedAttnArgs& a, const DecodePlan& plan, void* ws, cudaStream_t stream) {
+  if (a.head_dim == 64)
+    return plan.nt == 1 ? launch_paged_decode<T, KV, 64, 1>(a, plan, ws, stream) : launch_paged_decode<T, KV, 64, 2>(a, plan, ws, stream);
+  return plan.nt == 1 ? launch_paged_decode<T, KV, 128, 1>(a, plan, ws, stream) : launch_paged_decode<T, KV, 128, 2>(a, plan, ws, stream);
+}
+
+int64_t max_keys_of(const PagedAttnArgs& a) {
+  const int64_t cap = a.seqs.max_pages << a.seqs.page_shift;
+  return std::min<int64_t>(cap, static_cast<int64_t>(a.window) + a.seqs.max_new);
+}
+
+}  // namespace
+
+// 4-D maps over the pages: [num_pages, Hkv, page rows, D] elements, or the code and
+// scale bytes of 4-bit pages (scales as 16-byte chunks).
+dli_status make_page_maps(const PagedAttnArgs& a, bool fp4, int d, int box_rows, bool bf16, CUtensorMap* tk, CUtensorMap* tv,
+                          CUtensorMap* tks, CUtensorMap* tvs) {
+  const uint64_t page_rows = 1ull << a.seqs.page_shift, hkv = static_cast<uint64_t>(a.hkv);
+  const uint64_t pages = static_cast<uint64_t>(a.seqs.num_pages), ud = static_cast<uint64_t>(d);
+  if (!fp4) {
+    const uint64_t dims[4] = {ud, page_rows, hkv, pages};
+    const uint64_t strides[3] = {ud * 2, page_rows * ud * 2, hkv * page_rows * ud * 2};
+    const uint32_t box[4] = {64u, static_cast<uint32_t>(box_rows), 1u, 1u};
+    dli_status st = make_map_4d(tk, a.k_pages, bf16, dims, strides, box);
+    if (st == DLI_OK) st = make_map_4d(tv, a.v_pages, bf16, dims, strides, box);
+    *tks = *tk;
+    *tvs = *tv;
+    return st;
+  }
+  const uint64_t block = static_cast<uint64_t>(fp4_block_bytes(static_cast<int64_t>(page_rows), d));
+  const uint64_t dims[4] = {ud / 2, page_rows, hkv, pages};
+  const uint64_t strides[3] = {ud / 2, block, hkv * block};
+  const uint32_t box[4] = {static_cast<uint32_t>(d / 2), static_cast<uint32_t>(box_rows), 1u, 1u};
+  const uint64_t sdims[4] = {16, page_rows * ud / 256, hkv, pages};
+  const uint64_t sstrides[3] = {16, block, hkv * block};
+  const uint32_t sbox[4] = {16u, static_cast<uint32_t>(box_rows * d / 256), 1u, 1u};
+  const int64_t codes = static_cast<int64_t>(page_rows) * d / 2;
+  const void* base[2] = {a.k_pages, a.v_pages};
+  CUtensorMap* code[2] = {tk, tv};
+  CUtensorMap* scale[2] = {tks, tvs};
+  for (int i = 0; i < 2; ++i) {
+    dli_status st = make_map_4d_bytes(code[i], base[i], dims, strides, box, d == 128);
+    if (st == DLI_OK) st = make_map_4d_bytes(scale[i], static_cast<const uint8_t*>(base[i]) + codes, sdims, sstrides, sbox, false);
+    if (st != DLI_OK) return st;
+  }
+  return DLI_OK;
+}
+
+bool paged_decode_serves(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype) {
+  if (dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) return false;
+  if (a.head_dim != 64 && a.head_dim != 128) return false;
+  (void)kv_dtype;
+  if (a.seqs.num_pages < 1) return false;
+  for (const void* p : {a.q, a.k_pages, a.v_pages, static_cast<const void*>(a.out)})
+    if (!aligned(p, 16)) return false;
+  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a));
+  return plan.units <= INT_MAX;
+}
+
+size_t paged_decode_workspace(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys) {
+  return plan_paged_decode(batch, hkv, group, max_new, head_dim, max_keys).workspace;
+}
+
+dli_status run_paged_decode(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype, void* workspace,
+                            size_t workspace_bytes, cudaStream_t stream) {
+  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a));
+  if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace || !aligned(workspace, 16)))
+    return fail(DLI_ERR_WORKSPACE, "attention_paged: a 16-byte aligned workspace of " + std::to_string(plan.workspace) + " bytes is needed");
+  const bool fp4 = kv_dtype == DLI_DTYPE_FP4;
+  if (dtype == DLI_DTYPE_BF16)
+    return fp4 ? launch_paged_decode_nd<__nv_bfloat16, Fp4>(a, plan, workspace, stream)
+               : launch_paged_decode_nd<__nv_bfloat16, __nv_bfloat16>(a, plan, workspace, stream);
+  return fp4 ? launch_paged_decode_nd<__half, Fp4>(a, plan, workspace, stream)
+             : launch_paged_decode_nd<__half, __half>(a, plan, workspace, stream);
+}
+
+}  // namespace dli_sm100

@@ -1,0 +1,90 @@
+// Warp-level matrix and conversion wrappers (mma.sync, ldmatrix, movmatrix, ex2)
+// used by the paged decode attention.
+#pragma once
+
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace dli_sm100 {
+
+// D[16x8] += A[16x16] B[16x8], 16-bit operands, fp32 accumulators.
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+// Transposes an 8x8 matrix of 16-bit values held one row pair per lane.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Byte I of `w` (two E2M1 codes) as two halves, the low code in the low half.
+template <int I>
+__device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t w) {
+  uint32_t r;
+  if constexpr (I == 0)
+    asm("{.reg .b8 a,b,c,d; mov.b32 {a,b,c,d}, %1; cvt.rn.f16x2.e2m1x2 %0, a;}" : "=r"(r) : "r"(w));
+  else if constexpr (I == 1)
+    asm("{.reg .b8 a,b,c,d; mov.b32 {a,b,c,d}, %1; cvt.rn.f16x2.e2m1x2 %0, b;}" : "=r"(r) : "r"(w));
+  else if constexpr (I == 2)
+    asm("{.reg .b8 a,b,c,d; mov.b32 {a,b,c,d}, %1; cvt.rn.f16x2.e2m1x2 %0, c;}" : "=r"(r) : "r"(w));
+  else
+    asm("{.reg .b8 a,b,c,d; mov.b32 {a,b,c,d}, %1; cvt.rn.f16x2.e2m1x2 %0, d;}" : "=r"(r) : "r"(w));
+  return r;
+}
+// Two E4M3 bytes (low 16 bits of `w`) as two halves.
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t w) {
+  uint32_t r;
+  asm("{.reg .b16 a; cvt.u16.u32 a, %1; cvt.rn.f16x2.e4m3x2 %0, a;}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+
+}  // namespace dli_sm100
