@@ -546,12 +546,13 @@ extern "C" size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64
                                                            int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                            int64_t page_size, int64_t max_pages, dli_dtype dtype,
                                                            dli_dtype kv_dtype) {
-  (void)kv_dtype;
   if (tokens <= 0 || batch <= 0 || max_new <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0) return 0;
   if (page_shift_of(page_size) < 0 || max_pages <= 0 || max_pages > (1ll << 30) / page_size) return 0;
   if ((dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) || (head_dim != 64 && head_dim != 128)) return 0;
-  if (q_heads / kv_heads * max_new > kDecodeRows) return 0;
-  return paged_decode_workspace(batch, kv_heads, q_heads / kv_heads, max_new, head_dim, max_pages * page_size);
+  const int64_t group = q_heads / kv_heads, max_keys = max_pages * page_size;
+  if (group * max_new <= kDecodeRows) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
+  if (group > 128 || kv_dtype != dtype) return 0;
+  return paged_prefill_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
 }
 
 extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pages, const void* v_pages,
@@ -593,6 +594,8 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
   a.v_scale = fp4 ? v_scale : 1.f;
   if (a.group * max_new <= kDecodeRows && paged_decode_serves(a, dtype, kv_dtype))
     return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
+  if (a.group * max_new > kDecodeRows && paged_prefill_serves(a, dtype, kv_dtype))
+    return run_paged_prefill(a, dtype, workspace, workspace_bytes, as_stream(stream));
   dli_status run = DLI_OK;
   st = dispatch_float(dtype, what, [&](auto tag) {
     using T = decltype(tag);

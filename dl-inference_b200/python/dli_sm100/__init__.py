@@ -11,6 +11,7 @@ missing.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -441,51 +442,64 @@ def paged_kv_pages(num_pages, kv_heads, page_size, head_dim, dtype, device="cuda
 
 def _pages(what, k_pages, v_pages, page_table, head_dim, dtype):
     """(num_pages, kv_heads, page_size, kv dtype code) of a pool, its tensors checked."""
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    shape, kind = k_pages.shape, k_pages.dtype
+    if shape != v_pages.shape or kind != v_pages.dtype:
         raise ValueError(f"{what}: k_pages and v_pages differ in shape or dtype")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
         raise ValueError(f"{what}: page_table must be int32 [batch, max_pages]")
-    if k_pages.dtype == torch.uint8:
-        if k_pages.dim() != 3 or head_dim % 16 or k_pages.shape[2] % (head_dim * 9 // 16):
+    if kind == torch.uint8:
+        if len(shape) != 3 or head_dim % 16 or shape[2] % (head_dim * 9 // 16):
             raise ValueError(f"{what}: 4-bit pages must be uint8 [num_pages, kv_heads, page_size * head_dim * 9 / 16]")
-        return k_pages.shape[0], k_pages.shape[1], k_pages.shape[2] // (head_dim * 9 // 16), FP4
-    if k_pages.dim() != 4 or k_pages.shape[3] != head_dim or k_pages.dtype != dtype:
+        return shape[0], shape[1], shape[2] // (head_dim * 9 // 16), FP4
+    if len(shape) != 4 or shape[3] != head_dim or kind != dtype or kind not in DTYPE_CODES:
         raise ValueError(f"{what}: pages must be [num_pages, kv_heads, page_size, {head_dim}] of {dtype}")
-    return k_pages.shape[0], k_pages.shape[1], k_pages.shape[2], DTYPE_CODES[dtype]
+    return shape[0], shape[1], shape[2], DTYPE_CODES[kind]
 
 
-def _rows(what, tokens, positions, page_table, starts, max_new):
+def _rows(what, tokens, b, positions, starts, max_new):
     """max_new of a packed batch, its tensors checked (starts None: equal shares of the rows)."""
-    b = page_table.shape[0]
-    if positions.dtype != torch.int64 or tuple(positions.shape) != (b,):
+    if positions.dtype != torch.int64 or positions.dim() != 1 or positions.numel() != b:
         raise ValueError(f"{what}: positions must be int64 [batch]")
     if starts is None:
         if max_new is None:
             if b == 0 or tokens % b:
                 raise ValueError(f"{what}: without starts the rows must divide among the sequences")
-            max_new = tokens // b
+            return tokens // b
         if tokens != b * max_new:
             raise ValueError(f"{what}: without starts there must be batch * max_new rows")
-    else:
-        if starts.dtype != torch.int64 or tuple(starts.shape) != (b + 1,):
-            raise ValueError(f"{what}: starts must be int64 [batch + 1]")
-        if max_new is None:
-            max_new = tokens
-    return int(max_new)
+    elif starts.dtype != torch.int64 or starts.dim() != 1 or starts.numel() != b + 1:
+        raise ValueError(f"{what}: starts must be int64 [batch + 1]")
+    return int(max_new) if max_new is not None else tokens
 
 
-def _on(what, first, *ts):
-    """Every tensor contiguous on one CUDA device; returns (its guard, its current stream)."""
-    dev = first.device
-    if dev.type != "cuda":
+def _device(what, *ts):
+    """Index of the one CUDA device that holds every (contiguous) tensor."""
+    dev = ts[0].get_device()
+    if dev < 0:
         raise ValueError(f"{what}: expects CUDA tensors")
-    for t in (first, *ts):
+    for t in ts:
         if t is not None:
-            if t.device != dev:
+            if t.get_device() != dev:
                 raise ValueError(f"{what}: tensors on different devices")
             if not t.is_contiguous():
                 raise ValueError("tensors must be contiguous")
-    return torch.cuda.device(dev), ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    return dev
+
+
+def _launch(what, dev, fn, *args):
+    """fn(*args, stream) with `dev` current, on its current stream."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
+        st = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, stream)
+    if st != DLI_OK:
+        check(st, what)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def qkv_rotary_paged(qkv, cos, sin, positions, page_table, k_pages, v_pages, q_heads, starts=None, max_new=None,
@@ -494,27 +508,33 @@ def qkv_rotary_paged(qkv, cos, sin, positions, page_table, k_pages, v_pages, q_h
     v appended to the pages at positions[b], positions[b] + 1, ...; returns rotated q
     [rows, Hq, D]. `starts` (int64 [batch + 1]) gives the rows of every sequence, at
     most `max_new` each; None: all sequences have the same number."""
+    what = "qkv_rotary_paged"
     kv_heads, width = k_pages.shape[1], qkv.shape[-1]
     heads = q_heads + 2 * kv_heads
-    if q_heads <= 0 or width % heads:
+    if q_heads <= 0 or width % heads or width == 0:
         raise ValueError("qkv_rotary_paged: qkv must be [.., (q_heads + 2 * kv_heads) * head_dim]")
     d, tokens = width // heads, qkv.numel() // width
-    what = "qkv_rotary_paged"
     num_pages, _, page_size, kv = _pages(what, k_pages, v_pages, page_table, d, qkv.dtype)
-    max_new = _rows(what, tokens, positions, page_table, starts, max_new)
+    b, max_pages = page_table.shape
+    max_new = _rows(what, tokens, b, positions, starts, max_new)
     if cos.shape != sin.shape or cos.dim() != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("qkv_rotary_paged: cos and sin must be float32 [rows, pairs]")
     if q_out is None:
-        q_out = torch.empty(tokens, q_heads, d, dtype=qkv.dtype, device=qkv.device)
+        q_out = torch.empty((tokens, q_heads, d), dtype=qkv.dtype, device=qkv.device)
     elif q_out.dtype != qkv.dtype or q_out.numel() != tokens * q_heads * d:
         raise ValueError("qkv_rotary_paged: q_out must be [rows, q_heads, head_dim] of qkv's dtype")
-    guard, stream = _on(what, qkv, cos, sin, positions, page_table, k_pages, v_pages, starts, q_out)
-    with guard:
-        check(lib().dli_sm100_qkv_rotary_paged(
-            _ptr(qkv), _ptr(cos), _ptr(sin), _ptr(positions), _ptr(starts), _ptr(page_table), _ptr(q_out),
-            _ptr(k_pages), _ptr(v_pages), tokens, positions.shape[0], max_new, q_heads, kv_heads, d, cos.shape[1],
-            cos.shape[0], page_size, num_pages, page_table.shape[1], k_scale, v_scale, _dt(qkv), kv, stream), what)
+    dev = _device(what, qkv, cos, sin, positions, page_table, k_pages, v_pages, starts, q_out)
+    table_rows, pairs = cos.shape
+    _launch(what, dev, lib().dli_sm100_qkv_rotary_paged, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+            positions.data_ptr(), _at(starts), page_table.data_ptr(), q_out.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), tokens, b, max_new, q_heads, kv_heads, d, pairs, table_rows, page_size, num_pages,
+            max_pages, k_scale, v_scale, _dt(qkv), kv)
     return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_paged_workspace(*sizes):
+    return lib().dli_sm100_attention_paged_workspace_size(*sizes)
 
 
 def attention_paged(q, k_pages, v_pages, positions, page_table, starts=None, max_new=None, scale=0.0, softcap=0.0,
@@ -522,29 +542,27 @@ def attention_paged(q, k_pages, v_pages, positions, page_table, starts=None, max
     """Causal attention of packed q [rows, Hq, D] over a paged cache (after the append
     of the rows' k and v). softcap > 0 caps the scores by a tanh, window > 0 limits a
     row to its last `window` keys, slopes (float32 [Hq]) add slope * (j - i)."""
+    what = "attention_paged"
     if q.dim() != 3:
         raise ValueError("attention_paged: q must be [rows, q_heads, head_dim]")
     tokens, hq, d = q.shape
-    what = "attention_paged"
     num_pages, hkv, page_size, kv = _pages(what, k_pages, v_pages, page_table, d, q.dtype)
-    max_new = _rows(what, tokens, positions, page_table, starts, max_new)
+    b, max_pages = page_table.shape
+    max_new = _rows(what, tokens, b, positions, starts, max_new)
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != hq):
         raise ValueError("attention_paged: slopes must be float32 [q_heads]")
     if out is None:
         out = torch.empty_like(q)
     elif out.dtype != q.dtype or out.numel() != q.numel():
         raise ValueError("attention_paged: out must be like q")
-    guard, stream = _on(what, q, k_pages, v_pages, positions, page_table, starts, slopes, out)
-    L = lib()
-    b, max_pages = page_table.shape
-    with guard:
-        ws_bytes = L.dli_sm100_attention_paged_workspace_size(tokens, b, max_new, hq, hkv, d, page_size, max_pages,
-                                                              _dt(q), kv)
-        ws = _workspace(ws_bytes, q.device)
-        check(L.dli_sm100_attention_paged(
-            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(positions), _ptr(starts), _ptr(page_table), _ptr(slopes),
-            _ptr(out), tokens, b, max_new, hq, hkv, d, page_size, num_pages, max_pages, scale, softcap, window,
-            k_scale, v_scale, _dt(q), kv, _ptr(ws), ws_bytes, stream), what)
+    dev = _device(what, q, k_pages, v_pages, positions, page_table, starts, slopes, out)
+    dt = _dt(q)
+    ws_bytes = _attention_paged_workspace(tokens, b, max_new, hq, hkv, d, page_size, max_pages, dt, kv)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _launch(what, dev, lib().dli_sm100_attention_paged, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            positions.data_ptr(), _at(starts), page_table.data_ptr(), _at(slopes), out.data_ptr(), tokens, b, max_new,
+            hq, hkv, d, page_size, num_pages, max_pages, scale, softcap, window, k_scale, v_scale, dt, kv, _at(ws),
+            ws_bytes)
     return out
 
 
@@ -553,21 +571,19 @@ def paged_gather(k_pages, v_pages, page_table, count, head_dim, dtype, first=Non
     """Rows first[b] .. first[b] + count - 1 of every sequence as dense (k, v)
     [batch, Hkv, count, D] of `dtype`; rows at or past lengths[b] are zero."""
     what = "paged_gather"
-    num_pages, hkv, page_size, kv = _pages(what, k_pages, v_pages, page_table, head_dim, dtype)
-    b = page_table.shape[0]
-    for t in (first, lengths):
-        if t is not None and (t.dtype != torch.int64 or tuple(t.shape) != (b,)):
-            raise ValueError("paged_gather: first and lengths must be int64 [batch]")
-    guard, stream = _on(what, k_pages, v_pages, page_table, first, lengths)
-    k = torch.empty(b, hkv, count, head_dim, dtype=dtype, device=k_pages.device)
-    v = torch.empty_like(k)
     if dtype not in DTYPE_CODES:
         raise ValueError(f"unsupported dtype {dtype}")
-    with guard:
-        check(lib().dli_sm100_paged_gather(
-            _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(first), _ptr(lengths), _ptr(k), _ptr(v), b, count,
-            hkv, head_dim, page_size, num_pages, page_table.shape[1], k_scale, v_scale, DTYPE_CODES[dtype], kv,
-            stream), what)
+    num_pages, hkv, page_size, kv = _pages(what, k_pages, v_pages, page_table, head_dim, dtype)
+    b, max_pages = page_table.shape
+    for t in (first, lengths):
+        if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or t.numel() != b):
+            raise ValueError("paged_gather: first and lengths must be int64 [batch]")
+    dev = _device(what, k_pages, v_pages, page_table, first, lengths)
+    both = torch.empty((2, b, hkv, count, head_dim), dtype=dtype, device=k_pages.device)
+    k, v = both.unbind(0)
+    _launch(what, dev, lib().dli_sm100_paged_gather, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+            _at(first), _at(lengths), k.data_ptr(), v.data_ptr(), b, count, hkv, head_dim, page_size, num_pages,
+            max_pages, k_scale, v_scale, DTYPE_CODES[dtype], kv)
     return k, v
 
 
