@@ -551,7 +551,7 @@ extern "C" size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64
   if ((dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) || (head_dim != 64 && head_dim != 128)) return 0;
   const int64_t group = q_heads / kv_heads, max_keys = max_pages * page_size;
   if (group * max_new <= kDecodeRows) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
-  if (group > 128 || kv_dtype != dtype) return 0;
+  if (group > 128) return 0;
   return paged_prefill_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
 }
 
@@ -595,7 +595,7 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
   if (a.group * max_new <= kDecodeRows && paged_decode_serves(a, dtype, kv_dtype))
     return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
   if (a.group * max_new > kDecodeRows && paged_prefill_serves(a, dtype, kv_dtype))
-    return run_paged_prefill(a, dtype, workspace, workspace_bytes, as_stream(stream));
+    return run_paged_prefill(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
   dli_status run = DLI_OK;
   st = dispatch_float(dtype, what, [&](auto tag) {
     using T = decltype(tag);

@@ -1,6 +1,6 @@
 // Attention of many new tokens over a paged KV cache on tcgen05 tensor cores:
-// prompts and chunks of prompts, packed ragged batches, 16-bit pages, head dims
-// 64 and 128, up to 128 query heads per KV head.
+// prompts and chunks of prompts, packed ragged batches, 16-bit or 4-bit pages, head
+// dims 64 and 128, up to 128 query heads per KV head.
 //
 // A tile is 128 / group consecutive tokens of a sequence with all `group` query
 // heads of one KV head (row = token * group + head; 126 of 128 rows at 7 heads),
@@ -20,6 +20,11 @@
 //              so O is seldom rescaled) and sum in fp32, P as 16 bits over S's own
 //              columns; at the end O / sum through shared memory to the rows, or
 //              the share's (max, sum, O) to the workspace.
+// 4-bit pages: no producer warp; four converter warps read codes and scales a
+// block ahead into registers and write the K and V stages as halves (E2M1 x E4M3
+// has 6 significant bits: exact), and the MMAs run in f16 for every model type. The
+// softmax warps then write the Q tile, each row scaled by a power of two (exact), and
+// undo the scale on the scores.
 // Every wait is bounded; one that runs out sets the device error word.
 #include <algorithm>
 #include <climits>
@@ -32,7 +37,18 @@
 namespace dli_sm100 {
 namespace {
 
-constexpr int kThreads = 192;
+// warps: producer, MMA, 4 softmax; for 4-bit pages 4 softmax, 4 converters, MMA.
+// The softmax warps hold a row of S: with converters in the CTA they take 32
+// registers a thread from those (launched with 96: 128 x 128 + 128 x 64 + 32 x 96).
+template <bool FP4>
+struct Roles {
+  static constexpr int kThreads = FP4 ? 288 : 192;
+  static constexpr int kMma = FP4 ? 8 : 1;
+  static constexpr int kSoftmax = FP4 ? 0 : 2;
+  static constexpr int kConvert = 4;  // FP4 only
+  static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 128, kConvertRegs = 64;
+  static_assert(128 * kSoftmaxRegs + 128 * kConvertRegs + 32 * kLaunchRegs <= 288 * kLaunchRegs, "register split");
+};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2: P <= 2^8 before O is rescaled
 constexpr int BM = 128, BN = 64;
@@ -119,13 +135,22 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, done && *abort_flag == 0);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2)
+// Halves of the codes in `w` (8 elements) times the scale pair `s`.
+__device__ __forceinline__ uint4 fp4_halves(uint32_t w, uint32_t s) {
+  return make_uint4(mul_half2(e2m1x2_to_half2<0>(w), s), mul_half2(e2m1x2_to_half2<1>(w), s),
+                    mul_half2(e2m1x2_to_half2<2>(w), s), mul_half2(e2m1x2_to_half2<3>(w), s));
+}
+
+template <typename T, typename KV, int D>
+__global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads, 2)
     attn_paged_prefill_kernel(const PrefillArgs p, const __grid_constant__ CUtensorMap tq,
                               const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
   using L = PrefillLayout<D>;
   constexpr int KST = L::KST, VST = L::VST;
-  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
+  using MT = typename std::conditional<kFp4, __half, T>::type;  // MMA operand type
+  using W = Roles<kFp4>;
+  constexpr bool kBf16 = std::is_same<MT, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem[];
   const PagedAttnArgs& a = p.a;
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -162,13 +187,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int nblocks = x.block0 + static_cast<int>(static_cast<int64_t>(share + 1) * x.blocks / shares) - block_first;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
+    constexpr int kWriters = kFp4 ? 4 : 1;  // warps that fill Q, K and V, or TMA
+    mbar_init(q_full, kWriters);
     for (int s = 0; s < KST; ++s) {
-      mbar_init(&k_full[s], 1);
+      mbar_init(&k_full[s], kWriters);
       mbar_init(&k_empty[s], 1);
     }
     for (int s = 0; s < VST; ++s) {
-      mbar_init(&v_full[s], 1);
+      mbar_init(&v_full[s], kWriters);
       mbar_init(&v_empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -181,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 1) {
+  if (warp == W::kMma) {
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
@@ -192,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int rows = x.tokens * a.group;  // of the 128
   const int pos0 = x.rows.past + x.t0;
 
-  if (warp == 0) {
+  if (!kFp4 && warp == 0) {
     // ---- Q tile, then K and V blocks in the order the MMAs use them: K0, K1, V0, K2, V1, ...
     const int shift = a.seqs.page_shift, page_rows = 1 << shift;
     const int box_rows = min(page_rows, BN), boxes = BN / box_rows;
@@ -257,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_wait(q_full, 0);
     for (int j = max(0, k_issued - KST); j < k_issued; ++j) mbar_wait(&k_full[j % KST], (j / KST) & 1);
     for (int j = max(0, v_issued - VST); j < v_issued; ++j) mbar_wait(&v_full[j % VST], (j / VST) & 1);
-  } else if (warp == 1) {
+  } else if (warp == W::kMma) {
     if (lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, BM, BN);
       constexpr uint32_t idesc_o = umma_idesc_f16_bmn(kBf16, BM, D);
@@ -309,7 +335,88 @@ __global__ void __launch_bounds__(kThreads, 2)
       umma_commit(mma_done);
       mbar_wait(mma_done, 0);
     }
+  } else if (kFp4 && warp >= W::kConvert) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::kConvertRegs));
+    // ---- converters: thread = half a key row; loads a block ahead, then K0, K1, V0, ...
+    const int ct = threadIdx.x - W::kConvert * 32;
+    const int key_row = ct & 63, half = ct >> 6;
+    constexpr int WORDS = D / 16;  // code words of half a row
+    constexpr int SB = D / 32;     // scale bytes
+    const int shift = a.seqs.page_shift, page_rows = 1 << shift;
+    const int32_t* ids = a.seqs.page_table + b * a.seqs.max_pages;
+    const int64_t block_bytes = fp4_block_bytes(page_rows, D);
+    const uint8_t* pages[2] = {static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages)};
+    auto page_for = [&](int j) {
+      const int key = (block_first + j) * BN + key_row;
+      if (j >= nblocks || key >= x.kv_len || key < x.key_lo) return -1;
+      const int page = ids[key >> shift];
+      if (page < 0 || page >= a.seqs.num_pages) {
+        set_device_error(a.seqs.err, kDevErrPageIndex);
+        return -1;
+      }
+      return page;
+    };
+    auto fetch = [&](int j, int page, int which, uint32_t (&w)[WORDS], uint32_t& sc) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+      sc = 0u;  // rows that are not of the tile's keys: zeros
+      if (page < 0) return;
+      const int r = ((block_first + j) * BN + key_row) & (page_rows - 1);
+      const uint8_t* base = pages[which] + (static_cast<int64_t>(page) * a.hkv + kvh) * block_bytes;
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(base + r * (D / 2) + half * (D / 4) + i * 4);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+      const uint8_t* s = base + page_rows * (D / 2) + r * (D / 16) + half * SB;
+      sc = SB == 4 ? *reinterpret_cast<const uint32_t*>(s) : static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(s));
+    };
+    // the half row as swizzled 16-byte chunks of halves, then the warp's arrival
+    auto put = [&](uint8_t* stage, const uint32_t (&w)[WORDS], uint32_t sc, uint64_t* full) {
+      uint8_t* row = stage + (D == 128 ? half * (BN * 128) : 0) + key_row * 128;
+      uint32_t s2 = 0u;
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) {
+        if (i % 4 == 0) s2 = e4m3x2_to_half2(sc >> (4 * i));
+        const uint32_t s = i % 4 < 2 ? __byte_perm(s2, s2, 0x1010) : __byte_perm(s2, s2, 0x3232);
+        const int ch = (D == 128 ? 0 : half * 4) + i;
+        *reinterpret_cast<uint4*>(row + ((ch ^ (key_row & 7)) << 4)) = fp4_halves(w[i], s);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
+    };
+    uint32_t kw[WORDS], vw[WORDS], ks, vs;
+    int page0 = page_for(0), page1 = page_for(1);
+    fetch(0, page0, 0, kw, ks);
+    fetch(0, page0, 1, vw, vs);
+    bool ok = true;
+    // V of block j is converted after K of block j + 1: the order of the MMAs
+    for (int j = 0; j <= nblocks && ok; ++j) {
+      const int page2 = page_for(j + 2);
+      if (j < nblocks) {
+        const int st = j % KST;
+        ok = warp_wait(&k_empty[st], ((j / KST) & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        put(smem + L::kKOff + st * L::kKVBytes, kw, ks, &k_full[st]);
+        fetch(j + 1, page1, 0, kw, ks);
+      }
+      if (j > 0) {
+        const int st = (j - 1) % VST;
+        ok = warp_wait(&v_empty[st], (((j - 1) / VST) & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        put(smem + L::kVOff + st * L::kKVBytes, vw, vs, &v_full[st]);
+        fetch(j, page0, 1, vw, vs);
+      }
+      page0 = page1;
+      page1 = page2;
+    }
+    if (!ok && lane == 0) {
+      set_device_error(a.seqs.err, kDevErrAttentionTimeout);
+      *abort_flag = 1;
+    }
   } else {
+    if constexpr (kFp4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(W::kSoftmaxRegs));
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // tensor-memory lane = row of the tile
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -319,7 +426,38 @@ __global__ void __launch_bounds__(kThreads, 2)
     const float slope = a.slopes && row < rows ? a.slopes[head] * kLog2e : 0.f;
     const bool cap = a.softcap > 0.f, bias = a.slopes != nullptr;
     const float cap_out = a.softcap * kLog2e;
-    const float in_scale = cap ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
+    float in_scale = cap ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
+    if constexpr (kFp4) {
+      // this thread's row of the Q tile, scaled by 2^-e with 2^e <= max|q| < 2^(e+1)
+      const T* q = static_cast<const T*>(a.q) + ((x.rows.row0 + x.t0 + tok) * a.hq + head) * D;
+      float big = 0.f;
+      if (row < rows) {
+#pragma unroll 4
+        for (int c = 0; c < D; c += 8) {
+          const Vec16<T> in = load16(q + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(to_f32(in.e[i])));
+        }
+      }
+      const int e = max(-120, min(120, static_cast<int>((__float_as_uint(big) >> 23) & 255u) - 127));
+      const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+      in_scale *= __uint_as_float(static_cast<unsigned>(127 + e) << 23);
+#pragma unroll 4
+      for (int c = 0; c < D; c += 8) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows) {
+          const Vec16<T> in = load16(q + c);
+          v.x = pack16<MT>(to_f32(in.e[0]) * down, to_f32(in.e[1]) * down);
+          v.y = pack16<MT>(to_f32(in.e[2]) * down, to_f32(in.e[3]) * down);
+          v.z = pack16<MT>(to_f32(in.e[4]) * down, to_f32(in.e[5]) * down);
+          v.w = pack16<MT>(to_f32(in.e[6]) * down, to_f32(in.e[7]) * down);
+        }
+        *reinterpret_cast<uint4*>(smem + (c >> 6) * L::kBox + row * 128 + ((((c >> 3) & 7) ^ (row & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
     const float mul = cap || bias ? 1.f : in_scale;  // what the scores still want when the maximum is taken
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
@@ -345,9 +483,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int i = 0; i < BN; ++i) s[i] = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(s[i] * in_scale));
       }
       if (bias) {
-        const float first = cap ? 1.f : in_scale;
+        const float first = cap ? 1.f : in_scale, at = slope * static_cast<float>(key0 - pos);
 #pragma unroll
-        for (int i = 0; i < BN; ++i) s[i] = fmaf(s[i], first, slope * static_cast<float>(key0 + i - pos));
+        for (int i = 0; i < BN; i += 2) {
+          const float2 far = fma2(make_float2(slope, slope), make_float2(i, i + 1), make_float2(at, at));
+          const float2 y = fma2(make_float2(s[i], s[i + 1]), make_float2(first, first), far);
+          s[i] = y.x;
+          s[i + 1] = y.y;
+        }
       }
       if (key0 + BN - 1 > pos0 || key0 <= pos0 + x.tokens - 1 - a.window) {
         const int end = pos - key0, begin = lo - key0;
@@ -401,13 +544,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         e.x = exp2_approx(e.x);
         e.y = exp2_approx(e.y);
         rs[(i / 2) & 3] = add2(rs[(i / 2) & 3], e);
-        pk[i / 2] = pack16<T>(e.x, e.y);
+        pk[i / 2] = pack16<MT>(e.x, e.y);
       }
       const float2 sum = add2(add2(rs[0], rs[1]), add2(rs[2], rs[3]));
       l += sum.x + sum.y;
       // V rows that no row of the tile sees may hold anything: a zero weight must meet a zero
       const int z_end = x.kv_len - key0, z_begin = x.key_lo - key0;
-      const bool stale = z_end < BN || z_begin > 0;
+      const bool stale = !kFp4 && (z_end < BN || z_begin > 0);  // the converters write zeros there
       if (stale) {
         if (!warp_wait(&v_full[j % VST], (j / VST) & 1, abort_flag)) {
           ok = false;
@@ -491,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == W::kMma) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, L::kTmemCols);
@@ -558,19 +701,20 @@ PrefillPlan plan_prefill(int64_t batch, int64_t hkv, int64_t group, int64_t max_
   return p;
 }
 
-template <typename T, int D>
+template <typename T, typename KV, int D>
 dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void* workspace, cudaStream_t stream) {
   using L = PrefillLayout<D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  CUtensorMap tq, tk, tv, tks, tvs;
+  constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
+  CUtensorMap tq{}, tk{}, tv{}, tks, tvs;  // not used for 4-bit pages
   const int page_rows = 1 << a.seqs.page_shift;
-  dli_status st = make_page_maps(a, false, D, std::min(page_rows, BN), kBf16, &tk, &tv, &tks, &tvs);
+  dli_status st = kFp4 ? DLI_OK : make_page_maps(a, false, D, std::min(page_rows, BN), kBf16, &tk, &tv, &tks, &tvs);
   if (st != DLI_OK) return st;
   const uint64_t qd[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.hq), static_cast<uint64_t>(a.seqs.tokens), 1ull};
   const uint64_t row_bytes = static_cast<uint64_t>(a.hq) * D * 2;
   const uint64_t qs[3] = {static_cast<uint64_t>(D * 2), row_bytes, row_bytes * static_cast<uint64_t>(a.seqs.tokens)};
   const uint32_t qb[4] = {64u, static_cast<uint32_t>(a.group), static_cast<uint32_t>(plan.tile_tokens), 1u};
-  st = make_map_4d(&tq, a.q, kBf16, qd, qs, qb);
+  if (!kFp4) st = make_map_4d(&tq, a.q, kBf16, qd, qs, qb);
   if (st != DLI_OK) return st;
   PrefillArgs p{};
   p.a = a;
@@ -581,12 +725,20 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.part_o);
   }
-  auto kern = attn_paged_prefill_kernel<T, D>;
+  auto kern = attn_paged_prefill_kernel<T, KV, D>;
   st = ensure_smem(reinterpret_cast<const void*>(kern), L::kBytes, "attention_paged");
   if (st != DLI_OK) return st;
+  if (kFp4) {
+    // the register split draws on what the CTA is launched with
+    static const int regs = [&] {
+      cudaFuncAttributes attr{};
+      return cudaFuncGetAttributes(&attr, kern) == cudaSuccess ? attr.numRegs : 0;
+    }();
+    if (regs < Roles<true>::kLaunchRegs) return fail(DLI_ERR_UNSUPPORTED, "attention_paged: built with too few registers a thread");
+  }
   const dim3 grid(static_cast<unsigned>(plan.tiles * plan.splits), static_cast<unsigned>(a.hkv),
                   static_cast<unsigned>(a.seqs.batch));
-  launch_pdl(kern, grid, dim3(kThreads), L::kBytes, stream, p, tq, tk, tv);
+  launch_pdl(kern, grid, dim3(Roles<kFp4>::kThreads), L::kBytes, stream, p, tq, tk, tv);
   if (plan.splits > 1)
     launch_pdl(attn_paged_prefill_combine_kernel<T, D>,
                dim3(static_cast<unsigned>(plan.tiles), static_cast<unsigned>(a.hkv), static_cast<unsigned>(a.seqs.batch)),
@@ -601,7 +753,7 @@ int64_t keys_of(const PagedAttnArgs& a) {
 }  // namespace
 
 bool paged_prefill_serves(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype) {
-  if ((dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) || kv_dtype != dtype) return false;
+  if ((dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) || (kv_dtype != dtype && kv_dtype != DLI_DTYPE_FP4)) return false;
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (a.group > BM || a.hkv > 65535 || a.seqs.num_pages < 1 || a.seqs.tokens > INT_MAX) return false;
   for (const void* p : {a.q, a.k_pages, a.v_pages, static_cast<const void*>(a.out)})
@@ -613,15 +765,23 @@ size_t paged_prefill_workspace(int64_t batch, int64_t hkv, int64_t group, int64_
   return plan_prefill(batch, hkv, group, max_new, head_dim, max_keys).workspace;
 }
 
-dli_status run_paged_prefill(const PagedAttnArgs& a, dli_dtype dtype, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+dli_status run_paged_prefill(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype, void* workspace,
+                             size_t workspace_bytes, cudaStream_t stream) {
   const PrefillPlan plan = plan_prefill(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, keys_of(a));
   if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace || !aligned(workspace, 16)))
     return fail(DLI_ERR_WORKSPACE, "attention_paged: a 16-byte aligned workspace of " + std::to_string(plan.workspace) + " bytes is needed");
+  if (kv_dtype == DLI_DTYPE_FP4) {
+    if (dtype == DLI_DTYPE_BF16)
+      return a.head_dim == 64 ? launch_prefill<__nv_bfloat16, Fp4, 64>(a, plan, workspace, stream)
+                              : launch_prefill<__nv_bfloat16, Fp4, 128>(a, plan, workspace, stream);
+    return a.head_dim == 64 ? launch_prefill<__half, Fp4, 64>(a, plan, workspace, stream)
+                            : launch_prefill<__half, Fp4, 128>(a, plan, workspace, stream);
+  }
   if (dtype == DLI_DTYPE_BF16)
-    return a.head_dim == 64 ? launch_prefill<__nv_bfloat16, 64>(a, plan, workspace, stream)
-                            : launch_prefill<__nv_bfloat16, 128>(a, plan, workspace, stream);
-  return a.head_dim == 64 ? launch_prefill<__half, 64>(a, plan, workspace, stream)
-                          : launch_prefill<__half, 128>(a, plan, workspace, stream);
+    return a.head_dim == 64 ? launch_prefill<__nv_bfloat16, __nv_bfloat16, 64>(a, plan, workspace, stream)
+                            : launch_prefill<__nv_bfloat16, __nv_bfloat16, 128>(a, plan, workspace, stream);
+  return a.head_dim == 64 ? launch_prefill<__half, __half, 64>(a, plan, workspace, stream)
+                          : launch_prefill<__half, __half, 128>(a, plan, workspace, stream);
 }
 
 }  // namespace dli_sm100

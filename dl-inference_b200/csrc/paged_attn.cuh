@@ -19,12 +19,11 @@ size_t paged_decode_workspace(int64_t batch, int64_t hkv, int64_t group, int64_t
 dli_status run_paged_decode(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype, void* workspace,
                             size_t workspace_bytes, cudaStream_t stream);
 
-// Many query rows (k_paged_prefill.cu): bf16/f16 pages of the model's type, head_dim
-// 64 or 128, at most 128 query heads per KV head, 16-byte aligned tensors.
+// Many query rows (k_paged_prefill.cu): bf16/f16, head_dim 64 or 128, at most 128 query heads per KV head, 16-byte aligned tensors.
 bool paged_prefill_serves(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype);
 size_t paged_prefill_workspace(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim,
                                int64_t max_keys);
-dli_status run_paged_prefill(const PagedAttnArgs& a, dli_dtype dtype, void* workspace, size_t workspace_bytes,
-                             cudaStream_t stream);
+dli_status run_paged_prefill(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype, void* workspace,
+                             size_t workspace_bytes, cudaStream_t stream);
 
 }  // namespace dli_sm100
