@@ -377,8 +377,11 @@ dli_status launch_attn_general(const PagedAttnArgs& a, cudaStream_t stream) {
   return check_launch("attention_paged");
 }
 
-// Query rows per KV head up to which the decode kernel serves a call.
-constexpr int64_t kDecodeRows = 32;
+// Calls of the decode kernel (the others go to the tcgen05 kernel): up to 32 query rows
+// per KV head, float32, and more heads per KV head than a tcgen05 tile has rows.
+bool few_rows(dli_dtype dtype, int64_t group, int64_t max_new) {
+  return dtype == DLI_DTYPE_F32 || group > 128 || group * max_new <= 32;
+}
 
 // ---- argument checks -----------------------------------------------------------------
 int page_shift_of(int64_t page_size) {
@@ -548,10 +551,10 @@ extern "C" size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64
                                                            dli_dtype kv_dtype) {
   if (tokens <= 0 || batch <= 0 || max_new <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0) return 0;
   if (page_shift_of(page_size) < 0 || max_pages <= 0 || max_pages > (1ll << 30) / page_size) return 0;
-  if ((dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) || (head_dim != 64 && head_dim != 128)) return 0;
+  if (!is_float_dtype(dtype) || (head_dim != 64 && head_dim != 128)) return 0;
   const int64_t group = q_heads / kv_heads, max_keys = max_pages * page_size;
-  if (group * max_new <= kDecodeRows) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
-  if (group > 128) return 0;
+  (void)kv_dtype;
+  if (few_rows(dtype, group, max_new)) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys, dtype);
   return paged_prefill_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
 }
 
@@ -592,10 +595,11 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
   a.scale = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim))) * (fp4 ? k_scale : 1.f);
   a.softcap = softcap;
   a.v_scale = fp4 ? v_scale : 1.f;
-  if (a.group * max_new <= kDecodeRows && paged_decode_serves(a, dtype, kv_dtype))
-    return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
-  if (a.group * max_new > kDecodeRows && paged_prefill_serves(a, dtype, kv_dtype))
+  if (few_rows(dtype, a.group, max_new)) {
+    if (paged_decode_serves(a, dtype)) return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
+  } else if (paged_prefill_serves(a, dtype, kv_dtype)) {
     return run_paged_prefill(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
+  }
   dli_status run = DLI_OK;
   st = dispatch_float(dtype, what, [&](auto tag) {
     using T = decltype(tag);

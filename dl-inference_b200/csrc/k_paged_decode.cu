@@ -1,6 +1,6 @@
 // Attention of few new tokens over a paged KV cache (decode steps, short
-// speculative runs): tensor cores by mma.sync, K/V pages by TMA, 16-bit or 4-bit
-// pages, head dims 64 and 128.
+// speculative runs; float32 calls of any length): tensor cores by mma.sync, K/V
+// pages by TMA, 16-bit, float32 or 4-bit pages, head dims 64 and 128.
 //
 // A unit is one row tile (8 or 16 query rows: the new tokens of a sequence times
 // the query heads of one KV head) over all its visible keys. S^T = K Q^T puts 16
@@ -23,7 +23,13 @@
 // 4-bit pages: codes arrive by TMA as bytes and become halves in registers, in
 // the order of the MMA fragments: E2M1 x E4M3 has 6 significant bits, so the
 // products are exact, and the MMA runs in f16 for every model type. q is scaled
-// by a power of two per row for that, which is exact too.
+// by a power of two per row for that, which is exact too; a float32 q, and its P,
+// enter as two halves each (22 bits).
+//
+// float32 pages: every operand is split into two TF32 numbers and three of the four
+// products are summed (2^-23 relative, like an fp32 product), so the call stays bound
+// by memory instead of by FFMA. MMAs cut their sums off, which would bias long
+// chains: scores are summed in four, O in one per 16 keys, and added up in fp32.
 #include <algorithm>
 #include <climits>
 #include <map>
@@ -53,14 +59,19 @@ struct DecodeArgs {
 template <typename T, typename KV, int D, int NT>
 struct DecodeLayout {
   static constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
+  static constexpr bool kF32 = std::is_same<KV, float>::value;
   static constexpr int R = 8 * NT;
   static constexpr int BN = kFp4 ? 128 : 64;  // keys per block
   static constexpr int SUB = BN / 64;         // 16-key groups per warp and block
-  static constexpr int kCodes = kFp4 ? BN * D / 2 : BN * D * 2;  // code or element bytes of K (or V)
+  static constexpr int kRowBytes = kFp4 ? D / 2 : kF32 ? D * 4 : D * 2;
+  static constexpr int kCodes = BN * kRowBytes;  // code or element bytes of K (or V)
   static constexpr int kScales = kFp4 ? BN * 8 : 0;  // a TMA box of 64 bytes (D 64, pages of 16) takes 128
   static constexpr int kStage = 2 * (kCodes + kScales);
   static constexpr int kStageTx = 2 * (kCodes + (kFp4 ? BN * D / 16 : 0));
-  static constexpr int kStages = kFp4 ? (D == 128 ? 5 : 8) : (D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 6 : 5));
+  // 16-bit and 4-bit: two CTAs per SM; float32: one
+  static constexpr int kStages = kFp4   ? (D == 128 ? 5 : 8)
+                                 : kF32 ? (D == 128 ? 3 : 6)
+                                        : (D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 6 : 5));
   static constexpr int DH = 64;  // dims that the four warps merge at a time
   static constexpr int kMergeOff = kStages * kStage;
   static constexpr int kMerge = 4 * R * DH * 4;
@@ -69,6 +80,7 @@ struct DecodeLayout {
   static constexpr int kBarOff = kMlOff + kMl;
   static constexpr int kBytes = kBarOff + 2 * kStages * 8 + 1024;  // the ring's base is rounded up to 1 KiB
   static_assert(kStage % 1024 == 0, "stage alignment");
+  static_assert(kBytes <= 232448, "shared memory");
 };
 
 // What one sequence contributes to the list of key blocks.
@@ -201,6 +213,13 @@ struct Walker {
   }
 };
 
+// Four output values as T.
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, float x, float y, float z, float w) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(x, y, z, w);
+  else *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(x, y), pack16<T>(z, w));
+}
+
 // Byte offset of (key row, 16-bit column) in a K or V stage of D/64 boxes of
 // [64 keys][64 elements] with the 128-byte swizzle.
 __device__ __forceinline__ int swz128(int row, int col) {
@@ -213,7 +232,9 @@ __global__ void __launch_bounds__(kDecodeThreads)
                              const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tks,
                              const __grid_constant__ CUtensorMap tvs) {
   using L = DecodeLayout<T, KV, D, NT>;
-  using MT = typename std::conditional<L::kFp4, __half, T>::type;  // MMA operand type
+  using MT = typename std::conditional<L::kFp4, __half, T>::type;  // MMA operand type of 16-bit MMAs
+  constexpr bool kF32 = L::kF32;
+  constexpr int QS = L::kFp4 && std::is_same<T, float>::value ? 2 : 1;  // halves that make up a q or p
   constexpr int BN = L::BN, SUB = L::SUB, R = L::R, ST = L::kStages;
   extern __shared__ uint8_t smem_base[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_base) + 1023) &
@@ -294,10 +315,11 @@ __global__ void __launch_bounds__(kDecodeThreads)
             tma_load_4d(ss + L::kScales + sat, &tvs, 0, 0, seg.kvh, page, &full[st]);
           } else {
             uint8_t* sv = sk + L::kCodes;
+            constexpr int kBoxWidth = kF32 ? 128 : 64;  // in the map's units: bytes or 16-bit elements
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-              tma_load_4d(sk + c * (64 * 128) + at * 128, &tk, c * 64, row, seg.kvh, page, &full[st]);
-              tma_load_4d(sv + c * (64 * 128) + at * 128, &tv, c * 64, row, seg.kvh, page, &full[st]);
+            for (int c = 0; c < L::kRowBytes / 128; ++c) {
+              tma_load_4d(sk + c * (64 * 128) + at * 128, &tk, c * kBoxWidth, row, seg.kvh, page, &full[st]);
+              tma_load_4d(sv + c * (64 * 128) + at * 128, &tv, c * kBoxWidth, row, seg.kvh, page, &full[st]);
             }
           }
         }
@@ -315,9 +337,12 @@ __global__ void __launch_bounds__(kDecodeThreads)
   float* merge = reinterpret_cast<float*>(smem + L::kMergeOff);
   float* wm = reinterpret_cast<float*>(smem + L::kMlOff);  // [4][R]
   float* wl = wm + 4 * R;
-  // MMA key row x of a 16-key group holds key perm(x): 4-bit V reads of the four
-  // lanes of a quad then fall into different banks
-  auto perm = [](int x) { return L::kFp4 ? (D == 128 ? x ^ ((x >> 1) & 1) : (x & 8) | ((x & 6) >> 1) | ((x & 1) << 2)) : x; };
+  // MMA key row x of a 16-key group holds key perm(x): the fragment reads of 4-bit V
+  // and of float32 K and V then fall into different banks
+  auto perm = [](int x) {
+    if (L::kFp4 && D == 128) return x ^ ((x >> 1) & 1);
+    return L::kFp4 || kF32 ? (x & 8) | ((x & 6) >> 1) | ((x & 1) << 2) : x;
+  };
   const float cap_out = a.softcap * kLog2e;
   const float base_scale = a.softcap > 0.f ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
   int it = 0;
@@ -342,7 +367,8 @@ __global__ void __launch_bounds__(kDecodeThreads)
       }
     // Q^T fragments, rows past the tile zero
     constexpr int KK = D / 16;
-    uint32_t qf[NT][KK][2];
+    constexpr int QR = kF32 ? 4 : 2 * QS;  // registers per 16 dims
+    uint32_t qf[NT][KK][QR];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 8 + g;
@@ -355,12 +381,12 @@ __global__ void __launch_bounds__(kDecodeThreads)
         float x[D / 4];
         float big = 0.f;
 #pragma unroll
-        for (int v = 0; v < D / 32; ++v) {
-          const Vec16<T> in = load16(q + t * (D / 4) + v * 8);
+        for (int v = 0; v < D / 4; v += Vec16<T>::N) {
+          const Vec16<T> in = load16(q + t * (D / 4) + v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            x[v * 8 + j] = valid ? to_f32(in.e[j]) : 0.f;
-            big = fmaxf(big, fabsf(x[v * 8 + j]));
+          for (int j = 0; j < Vec16<T>::N; ++j) {
+            x[v + j] = valid ? to_f32(in.e[j]) : 0.f;
+            big = fmaxf(big, fabsf(x[v + j]));
           }
         }
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
@@ -370,10 +396,24 @@ __global__ void __launch_bounds__(kDecodeThreads)
         const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
         const float up = __uint_as_float(static_cast<unsigned>(127 + e) << 23);
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j)
-          qf[nt][j / 2][j & 1] = pack16<__half>(x[2 * j] * down, x[2 * j + 1] * down);
+        for (int j = 0; j < D / 8; ++j) {
+          const float u = x[2 * j] * down, w = x[2 * j + 1] * down;
+          qf[nt][j / 2][j & 1] = pack16<__half>(u, w);
+          if constexpr (QS == 2)
+            qf[nt][j / 2][2 + (j & 1)] = pack16<__half>(u - __half2float(__float2half_rn(u)), w - __half2float(__float2half_rn(w)));
+        }
         rscale[nt][0] *= __shfl_sync(0xffffffffu, up, (2 * t) * 4);
         rscale[nt][1] *= __shfl_sync(0xffffffffu, up, (2 * t + 1) * 4);
+      } else if constexpr (kF32) {
+        // MMA pair kk: dims kk * 16 + 4t .. + 3
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint4 v = *reinterpret_cast<const uint4*>(q + kk * 16 + 4 * t);
+          qf[nt][kk][0] = valid ? v.x : 0u;
+          qf[nt][kk][1] = valid ? v.y : 0u;
+          qf[nt][kk][2] = valid ? v.z : 0u;
+          qf[nt][kk][3] = valid ? v.w : 0u;
+        }
       } else {
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
@@ -448,8 +488,46 @@ __global__ void __launch_bounds__(kDecodeThreads)
             for (int nt = 0; nt < NT; ++nt) {
               mma_16816<MT>(sc[u][nt], a00, a10, a01, a11, qf[nt][2 * i][0], qf[nt][2 * i][1]);
               mma_16816<MT>(sc[u][nt], a02, a12, a03, a13, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
+              if constexpr (QS == 2) {
+                mma_16816<MT>(sc[u][nt], a00, a10, a01, a11, qf[nt][2 * i][2], qf[nt][2 * i][3]);
+                mma_16816<MT>(sc[u][nt], a02, a12, a03, a13, qf[nt][2 * i + 1][2], qf[nt][2 * i + 1][3]);
+              }
             }
           }
+        } else if constexpr (kF32) {
+          const int r0 = kw + perm(g), r1 = kw + perm(g + 8);
+          float part[NT][4][4], low[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) low[nt][i] = part[nt][0][i] = part[nt][1][i] = part[nt][2][i] = part[nt][3][i] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            const uint8_t* box = sk + (kk >> 1) * (64 * 128);
+            const int ch = (kk & 1) * 4 + t;
+            const float4 k0 = *reinterpret_cast<const float4*>(box + r0 * 128 + ((ch ^ (r0 & 7)) << 4));
+            const float4 k1 = *reinterpret_cast<const float4*>(box + r1 * 128 + ((ch ^ (r1 & 7)) << 4));
+            uint32_t h[2][4], l2[2][4];
+            split_tf32(k0.x, h[0][0], l2[0][0]);
+            split_tf32(k1.x, h[0][1], l2[0][1]);
+            split_tf32(k0.y, h[0][2], l2[0][2]);
+            split_tf32(k1.y, h[0][3], l2[0][3]);
+            split_tf32(k0.z, h[1][0], l2[1][0]);
+            split_tf32(k1.z, h[1][1], l2[1][1]);
+            split_tf32(k0.w, h[1][2], l2[1][2]);
+            split_tf32(k1.w, h[1][3], l2[1][3]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float(&acc)[4] = part[nt][kk & 3];
+              mma_1688_f32(acc, low[nt], h[0], l2[0], __uint_as_float(qf[nt][kk][0]), __uint_as_float(qf[nt][kk][1]));
+              mma_1688_f32(acc, low[nt], h[1], l2[1], __uint_as_float(qf[nt][kk][2]), __uint_as_float(qf[nt][kk][3]));
+            }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              sc[u][nt][i] = low[nt][i] + ((part[nt][0][i] + part[nt][1][i]) + (part[nt][2][i] + part[nt][3][i]));
         } else {
           const uint32_t ks = smem_u32(sk);
 #pragma unroll
@@ -514,7 +592,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
         const int kw = u * 64 + warp * 16;
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][kF32 ? 4 : 2 * QS];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           // a row that has seen no key yet keeps m = -inf: its p are 0
@@ -523,8 +601,26 @@ __global__ void __launch_bounds__(kDecodeThreads)
           const float p10 = exp2_approx(sc[u][nt][2] - n0), p11 = exp2_approx(sc[u][nt][3] - n1);
           l[nt][0] += p00 + p10;  // this thread's keys; summed over the warp at the end
           l[nt][1] += p01 + p11;
-          pb[nt][0] = movmatrix_trans(pack16<MT>(p00, p01));
-          pb[nt][1] = movmatrix_trans(pack16<MT>(p10, p11));
+          if constexpr (kF32) {
+            // P^T as the B operand: lane (g, t) gets rows g of the keys 2t, 2t + 1 (+ 8)
+            const int s0 = 8 * t + (g >> 1), s1 = s0 + 4;
+            const float x0 = __shfl_sync(0xffffffffu, p00, s0), y0 = __shfl_sync(0xffffffffu, p01, s0);
+            const float x1 = __shfl_sync(0xffffffffu, p00, s1), y1 = __shfl_sync(0xffffffffu, p01, s1);
+            const float x2 = __shfl_sync(0xffffffffu, p10, s0), y2 = __shfl_sync(0xffffffffu, p11, s0);
+            const float x3 = __shfl_sync(0xffffffffu, p10, s1), y3 = __shfl_sync(0xffffffffu, p11, s1);
+            pb[nt][0] = __float_as_uint((g & 1) ? y0 : x0);
+            pb[nt][1] = __float_as_uint((g & 1) ? y1 : x1);
+            pb[nt][2] = __float_as_uint((g & 1) ? y2 : x2);
+            pb[nt][3] = __float_as_uint((g & 1) ? y3 : x3);
+          } else {
+            pb[nt][0] = movmatrix_trans(pack16<MT>(p00, p01));
+            pb[nt][1] = movmatrix_trans(pack16<MT>(p10, p11));
+            if constexpr (QS == 2) {
+              auto rest = [](float p) { return p - __half2float(__float2half_rn(p)); };
+              pb[nt][2] = movmatrix_trans(pack16<MT>(rest(p00), rest(p01)));
+              pb[nt][3] = movmatrix_trans(pack16<MT>(rest(p10), rest(p11)));
+            }
+          }
         }
         const int key_first = blk_key + kw;
         const bool stale = key_first + 16 > seg.w.kv_len || key_first < seg.w.key_lo;
@@ -558,8 +654,16 @@ __global__ void __launch_bounds__(kDecodeThreads)
   {                                                                                                                  \
     const uint32_t f0 = mul_half2(e2m1x2_to_half2<B>(ev0), s01), f1 = mul_half2(e2m1x2_to_half2<B>(od0), s01);      \
     const uint32_t f2 = mul_half2(e2m1x2_to_half2<B>(ev1), s23), f3 = mul_half2(e2m1x2_to_half2<B>(od1), s23);      \
-    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt)                                                                \
+    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) {                                                              \
+      if constexpr (QS == 2) {                                                                                       \
+        float part[4] = {0.f, 0.f, 0.f, 0.f};                                                                        \
+        mma_16816<MT>(part, f0, f1, f2, f3, pb[nt][2 * QS - 2], pb[nt][2 * QS - 1]);                                 \
+        mma_16816<MT>(part, f0, f1, f2, f3, pb[nt][0], pb[nt][1]);                                                   \
+        _Pragma("unroll") for (int k = 0; k < 4; ++k) o[nt][4 * i + B][k] += part[k];                                \
+      } else {                                                                                                       \
         mma_16816<MT>(o[nt][4 * i + B], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);                                       \
+      }                                                                                                              \
+    }                                                                                                                \
   }
             DLI_FP4_V(0)
             DLI_FP4_V(1)
@@ -570,14 +674,55 @@ __global__ void __launch_bounds__(kDecodeThreads)
         } else {
           if (stale) {
             // V rows that are not of the sequence may hold anything: a zero weight must meet a zero
-            for (int c = lane; c < 16 * (D / 8); c += 32) {
-              const int r = c / (D / 8), ch = c - r * (D / 8);
+            for (int c = lane; c < 16 * (L::kRowBytes / 16); c += 32) {
+              const int r = (c >> 3) & 15, box = c >> 7;
               if (key_first + r >= seg.w.kv_len || key_first + r < seg.w.key_lo)
-                *reinterpret_cast<uint4*>(sv + swz128(kw + r, ch * 8)) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(sv + box * (64 * 128) + (kw + r) * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async_smem();  // before the stage is given back to the TMA
             __syncwarp();
           }
+          if constexpr (kF32) {
+            // lane (g, t): 4 dims 4 * chunk of each 32, of the keys 2t and 2t + 1 of each 8
+            const int chunk = ((g & 1) << 2) | (g >> 1);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+              const uint8_t* box = sv + i * (64 * 128);
+              float part[NT][2][4], low[NT][2][4];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) part[nt][0][k] = part[nt][1][k] = low[nt][0][k] = low[nt][1][k] = 0.f;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int ra = kw + h * 8 + t, rb = ra + 4;
+                const float4 va = *reinterpret_cast<const float4*>(box + ra * 128 + ((chunk ^ (ra & 7)) << 4));
+                const float4 vb = *reinterpret_cast<const float4*>(box + rb * 128 + ((chunk ^ (rb & 7)) << 4));
+                uint32_t hi[2][4], lo[2][4];
+                split_tf32(va.x, hi[0][0], lo[0][0]);
+                split_tf32(va.y, hi[0][1], lo[0][1]);
+                split_tf32(vb.x, hi[0][2], lo[0][2]);
+                split_tf32(vb.y, hi[0][3], lo[0][3]);
+                split_tf32(va.z, hi[1][0], lo[1][0]);
+                split_tf32(va.w, hi[1][1], lo[1][1]);
+                split_tf32(vb.z, hi[1][2], lo[1][2]);
+                split_tf32(vb.w, hi[1][3], lo[1][3]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  const float b0 = __uint_as_float(pb[nt][2 * h]), b1 = __uint_as_float(pb[nt][2 * h + 1]);
+                  mma_1688_f32(part[nt][0], low[nt][0], hi[0], lo[0], b0, b1);
+                  mma_1688_f32(part[nt][1], low[nt][1], hi[1], lo[1], b0, b1);
+                }
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  o[nt][2 * i][k] += part[nt][0][k] + low[nt][0][k];
+                  o[nt][2 * i + 1][k] += part[nt][1][k] + low[nt][1][k];
+                }
+            }
+          } else {
           const uint32_t vs = smem_u32(sv);
 #pragma unroll
           for (int i = 0; i < KK; ++i) {
@@ -585,6 +730,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
             ldmatrix_x4_trans(f, vs + swz128(kw + (lane & 7) + (lane >> 4) * 8, i * 16 + ((lane >> 3) & 1) * 8));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_16816<MT>(o[nt][i], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
+          }
           }
         }
       }
@@ -623,8 +769,10 @@ __global__ void __launch_bounds__(kDecodeThreads)
         for (int i = 0; i < KK; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            // 16-bit: dims i * 16 + g (+ 8); 4-bit: g * D/8 + 2 i (+ 1)
-            const int dim = L::kFp4 ? g * (D / 8) + 2 * i + (k >> 1) : i * 16 + g + (k >> 1) * 8;
+            // 16-bit: dims i * 16 + g (+ 8); 4-bit: g * D/8 + 2 i (+ 1); float32: see the reads of V
+            const int dim = L::kFp4 ? g * (D / 8) + 2 * i + (k >> 1)
+                            : kF32  ? 32 * (i >> 1) + 4 * (((g & 1) << 2) | (g >> 1)) + 2 * (i & 1) + (k >> 1)
+                                    : i * 16 + g + (k >> 1) * 8;
             if (D == DH || dim / DH == half)
               merge[(warp * R + nt * 8 + 2 * t + (k & 1)) * DH + (dim - half * DH)] = o[nt][i][k] * f[k & 1];
           }
@@ -650,10 +798,8 @@ __global__ void __launch_bounds__(kDecodeThreads)
         if (seg.whole) {
           const int rr = seg.rt * R + r, tok = rr / a.group, h = seg.kvh * a.group + rr - tok * a.group;
           const float inv = a.v_scale / den;
-          uint2 v;
-          v.x = pack16<T>(sum.x * inv, sum.y * inv);
-          v.y = pack16<T>(sum.z * inv, sum.w * inv);
-          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((seg.w.rows.row0 + tok) * a.hq + h) * D + dim) = v;
+          store4(static_cast<T*>(a.out) + ((seg.w.rows.row0 + tok) * a.hq + h) * D + dim, sum.x * inv, sum.y * inv,
+                 sum.z * inv, sum.w * inv);
         } else {
           *reinterpret_cast<float4*>(d.part_o + (static_cast<int64_t>(seg.slot) * R + r) * D + dim) = sum;
           if (dim == 0) d.part_ml[static_cast<int64_t>(seg.slot) * R + r] = make_float2(top, den);
@@ -706,10 +852,8 @@ __global__ void __launch_bounds__(256) attn_paged_combine_kernel(const DecodeArg
     }
     const int rr = rt * R + r, tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
     const float inv = a.v_scale / den;
-    uint2 v;
-    v.x = pack16<T>(sum.x * inv, sum.y * inv);
-    v.y = pack16<T>(sum.z * inv, sum.w * inv);
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((sr.row0 + tok) * a.hq + h) * D + x) = v;
+    store4(static_cast<T*>(a.out) + ((sr.row0 + tok) * a.hq + h) * D + x, sum.x * inv, sum.y * inv, sum.z * inv,
+           sum.w * inv);
   }
 }
 
@@ -750,10 +894,11 @@ constexpr int kWholeKeys = 512;
 constexpr int kMinKeys = 256;
 constexpr int kMaxCtasPerSm = 2;
 
-DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys) {
+DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys,
+                             bool f32) {
   DecodePlan p{};
   const int64_t rows = group * max_new;
-  p.nt = rows <= 8 ? 1 : 2;
+  p.nt = rows <= 8 || f32 ? 1 : 2;  // two row tiles of split operands do not fit the registers
   p.tiles_max = static_cast<int>(ceil_div(rows, 8 * p.nt));
   p.units = batch * hkv * p.tiles_max;
   p.split = max_keys > kWholeKeys;
@@ -772,8 +917,11 @@ dli_status launch_paged_decode(const PagedAttnArgs& a, const DecodePlan& plan, v
   using L = DecodeLayout<T, KV, D, NT>;
   CUtensorMap tk, tv, tks, tvs;
   const int64_t page_rows = 1ll << a.seqs.page_shift;
-  dli_status st = make_page_maps(a, L::kFp4, D, static_cast<int>(std::min<int64_t>(page_rows, L::BN)), std::is_same<T, __nv_bfloat16>::value,
-                                 &tk, &tv, &tks, &tvs);
+  const dli_dtype kv_dtype = L::kFp4                                   ? DLI_DTYPE_FP4
+                             : L::kF32                                 ? DLI_DTYPE_F32
+                             : std::is_same<T, __nv_bfloat16>::value ? DLI_DTYPE_BF16
+                                                                       : DLI_DTYPE_F16;
+  dli_status st = make_page_maps(a, kv_dtype, D, static_cast<int>(std::min<int64_t>(page_rows, L::BN)), &tk, &tv, &tks, &tvs);
   if (st != DLI_OK) return st;
   auto kern = attn_paged_decode_kernel<T, KV, D, NT>;
   st = ensure_smem(reinterpret_cast<const void*>(kern), L::kBytes, "attention_paged");
@@ -798,9 +946,10 @@ dli_status launch_paged_decode(const PagedAttnArgs& a, const DecodePlan& plan, v
 
 template <typename T, typename KV>
 dli_status launch_paged_decode_nd(const PagedAttnArgs& a, const DecodePlan& plan, void* ws, cudaStream_t stream) {
-  if (a.head_dim == 64)
-    return plan.nt == 1 ? launch_paged_decode<T, KV, 64, 1>(a, plan, ws, stream) : launch_paged_decode<T, KV, 64, 2>(a, plan, ws, stream);
-  return plan.nt == 1 ? launch_paged_decode<T, KV, 128, 1>(a, plan, ws, stream) : launch_paged_decode<T, KV, 128, 2>(a, plan, ws, stream);
+  if constexpr (!std::is_same<T, float>::value)
+    if (plan.nt == 2)
+      return a.head_dim == 64 ? launch_paged_decode<T, KV, 64, 2>(a, plan, ws, stream) : launch_paged_decode<T, KV, 128, 2>(a, plan, ws, stream);
+  return a.head_dim == 64 ? launch_paged_decode<T, KV, 64, 1>(a, plan, ws, stream) : launch_paged_decode<T, KV, 128, 1>(a, plan, ws, stream);
 }
 
 int64_t max_keys_of(const PagedAttnArgs& a) {
@@ -810,62 +959,67 @@ int64_t max_keys_of(const PagedAttnArgs& a) {
 
 }  // namespace
 
-// 4-D maps over the pages: [num_pages, Hkv, page rows, D] elements, or the code and
-// scale bytes of 4-bit pages (scales as 16-byte chunks).
-dli_status make_page_maps(const PagedAttnArgs& a, bool fp4, int d, int box_rows, bool bf16, CUtensorMap* tk, CUtensorMap* tv,
+// 4-D maps over the pages: [num_pages, Hkv, page rows, D] 16-bit elements or bytes,
+// and the scale bytes of 4-bit pages as 16-byte chunks.
+dli_status make_page_maps(const PagedAttnArgs& a, dli_dtype kv_dtype, int d, int box_rows, CUtensorMap* tk, CUtensorMap* tv,
                           CUtensorMap* tks, CUtensorMap* tvs) {
   const uint64_t page_rows = 1ull << a.seqs.page_shift, hkv = static_cast<uint64_t>(a.hkv);
   const uint64_t pages = static_cast<uint64_t>(a.seqs.num_pages), ud = static_cast<uint64_t>(d);
-  if (!fp4) {
-    const uint64_t dims[4] = {ud, page_rows, hkv, pages};
-    const uint64_t strides[3] = {ud * 2, page_rows * ud * 2, hkv * page_rows * ud * 2};
-    const uint32_t box[4] = {64u, static_cast<uint32_t>(box_rows), 1u, 1u};
-    dli_status st = make_map_4d(tk, a.k_pages, bf16, dims, strides, box);
-    if (st == DLI_OK) st = make_map_4d(tv, a.v_pages, bf16, dims, strides, box);
-    *tks = *tk;
-    *tvs = *tv;
-    return st;
-  }
-  const uint64_t block = static_cast<uint64_t>(fp4_block_bytes(static_cast<int64_t>(page_rows), d));
-  const uint64_t dims[4] = {ud / 2, page_rows, hkv, pages};
-  const uint64_t strides[3] = {ud / 2, block, hkv * block};
-  const uint32_t box[4] = {static_cast<uint32_t>(d / 2), static_cast<uint32_t>(box_rows), 1u, 1u};
-  const uint64_t sdims[4] = {16, page_rows * ud / 256, hkv, pages};
-  const uint64_t sstrides[3] = {16, block, hkv * block};
-  const uint32_t sbox[4] = {16u, static_cast<uint32_t>(box_rows * d / 256), 1u, 1u};
-  const int64_t codes = static_cast<int64_t>(page_rows) * d / 2;
+  const uint32_t rows = static_cast<uint32_t>(box_rows);
   const void* base[2] = {a.k_pages, a.v_pages};
-  CUtensorMap* code[2] = {tk, tv};
+  CUtensorMap* map[2] = {tk, tv};
   CUtensorMap* scale[2] = {tks, tvs};
   for (int i = 0; i < 2; ++i) {
-    dli_status st = make_map_4d_bytes(code[i], base[i], dims, strides, box, d == 128);
-    if (st == DLI_OK) st = make_map_4d_bytes(scale[i], static_cast<const uint8_t*>(base[i]) + codes, sdims, sstrides, sbox, false);
+    dli_status st = DLI_OK;
+    if (kv_dtype == DLI_DTYPE_FP4) {
+      const uint64_t block = static_cast<uint64_t>(fp4_block_bytes(static_cast<int64_t>(page_rows), d));
+      const uint64_t dims[4] = {ud / 2, page_rows, hkv, pages}, sdims[4] = {16, page_rows * ud / 256, hkv, pages};
+      const uint64_t strides[3] = {ud / 2, block, hkv * block}, sstrides[3] = {16, block, hkv * block};
+      const uint32_t box[4] = {static_cast<uint32_t>(d / 2), rows, 1u, 1u}, sbox[4] = {16u, rows * d / 256, 1u, 1u};
+      st = make_map_4d_bytes(map[i], base[i], dims, strides, box, d == 128 ? 64 : 0);
+      if (st == DLI_OK)
+        st = make_map_4d_bytes(scale[i], static_cast<const uint8_t*>(base[i]) + page_rows * ud / 2, sdims, sstrides, sbox, 0);
+    } else if (kv_dtype == DLI_DTYPE_F32) {
+      const uint64_t dims[4] = {ud * 4, page_rows, hkv, pages};
+      const uint64_t strides[3] = {ud * 4, page_rows * ud * 4, hkv * page_rows * ud * 4};
+      const uint32_t box[4] = {128u, rows, 1u, 1u};
+      st = make_map_4d_bytes(map[i], base[i], dims, strides, box, 128);
+      *scale[i] = *map[i];
+    } else {
+      const uint64_t dims[4] = {ud, page_rows, hkv, pages};
+      const uint64_t strides[3] = {ud * 2, page_rows * ud * 2, hkv * page_rows * ud * 2};
+      const uint32_t box[4] = {64u, rows, 1u, 1u};
+      st = make_map_4d(map[i], base[i], kv_dtype == DLI_DTYPE_BF16, dims, strides, box);
+      *scale[i] = *map[i];
+    }
     if (st != DLI_OK) return st;
   }
   return DLI_OK;
 }
 
-bool paged_decode_serves(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype) {
-  if (dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) return false;
-  if (a.head_dim != 64 && a.head_dim != 128) return false;
-  (void)kv_dtype;
+bool paged_decode_serves(const PagedAttnArgs& a, dli_dtype dtype) {
+  if (!is_float_dtype(dtype) || (a.head_dim != 64 && a.head_dim != 128)) return false;
   if (a.seqs.num_pages < 1) return false;
   for (const void* p : {a.q, a.k_pages, a.v_pages, static_cast<const void*>(a.out)})
     if (!aligned(p, 16)) return false;
-  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a));
+  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a), dtype == DLI_DTYPE_F32);
   return plan.units <= INT_MAX;
 }
 
-size_t paged_decode_workspace(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys) {
-  return plan_paged_decode(batch, hkv, group, max_new, head_dim, max_keys).workspace;
+size_t paged_decode_workspace(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys,
+                              dli_dtype dtype) {
+  return plan_paged_decode(batch, hkv, group, max_new, head_dim, max_keys, dtype == DLI_DTYPE_F32).workspace;
 }
 
 dli_status run_paged_decode(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype, void* workspace,
                             size_t workspace_bytes, cudaStream_t stream) {
-  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a));
+  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a), dtype == DLI_DTYPE_F32);
   if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace || !aligned(workspace, 16)))
     return fail(DLI_ERR_WORKSPACE, "attention_paged: a 16-byte aligned workspace of " + std::to_string(plan.workspace) + " bytes is needed");
   const bool fp4 = kv_dtype == DLI_DTYPE_FP4;
+  if (dtype == DLI_DTYPE_F32)
+    return fp4 ? launch_paged_decode_nd<float, Fp4>(a, plan, workspace, stream)
+               : launch_paged_decode_nd<float, float>(a, plan, workspace, stream);
   if (dtype == DLI_DTYPE_BF16)
     return fp4 ? launch_paged_decode_nd<__nv_bfloat16, Fp4>(a, plan, workspace, stream)
                : launch_paged_decode_nd<__nv_bfloat16, __nv_bfloat16>(a, plan, workspace, stream);

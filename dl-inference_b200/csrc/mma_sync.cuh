@@ -26,6 +26,32 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
 }
+// D[16x8] += A[16x8] B[8x8], operands fp32 bits of which the MMA reads the top 19 (TF32).
+__device__ __forceinline__ void mma_1688_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// x = hi + lo to 2^-24: both rounded to nearest (ties away) at TF32's 11 significant
+// bits. lo is left for the MMA to cut off: half a unit is added to its magnitude.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
+}
+// A B to fp32's accuracy as three TF32 products, lo * lo (2^-24 of it) left out. The
+// MMA cuts its sums off instead of rounding them, so the caller keeps its chains
+// short: the leading product goes to `main`, the small ones to `low`.
+__device__ __forceinline__ void mma_1688_f32(float (&main)[4], float (&low)[4], const uint32_t (&ah)[4],
+                                             const uint32_t (&al)[4], float b0, float b1) {
+  uint32_t h0, l0, h1, l1;
+  split_tf32(b0, h0, l0);
+  split_tf32(b1, h1, l1);
+  mma_1688_tf32(low, al[0], al[1], al[2], al[3], h0, h1);
+  mma_1688_tf32(low, ah[0], ah[1], ah[2], ah[3], l0, l1);
+  mma_1688_tf32(main, ah[0], ah[1], ah[2], ah[3], h0, h1);
+}
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])

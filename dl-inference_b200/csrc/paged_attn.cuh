@@ -6,16 +6,17 @@
 
 namespace dli_sm100 {
 
-// Tensor maps over the K and V pages with boxes of box_rows rows of one (page,
-// head); for 4-bit pages tk/tv cover the code bytes and tks/tvs the scale bytes.
-dli_status make_page_maps(const PagedAttnArgs& a, bool fp4, int d, int box_rows, bool bf16, CUtensorMap* tk, CUtensorMap* tv,
+// Tensor maps over the K and V pages with boxes of box_rows rows x 128 bytes of one
+// (page, head); for 4-bit pages tk/tv cover the code bytes (whole rows) and tks/tvs
+// the scale bytes.
+dli_status make_page_maps(const PagedAttnArgs& a, dli_dtype kv_dtype, int d, int box_rows, CUtensorMap* tk, CUtensorMap* tv,
                           CUtensorMap* tks, CUtensorMap* tvs);
 
-// Few query rows per KV head (k_paged_decode.cu): bf16/f16, head_dim 64 or 128,
-// 16-byte aligned tensors.
-bool paged_decode_serves(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype);
+// Few query rows per KV head, and every float32 call (k_paged_decode.cu): head_dim 64
+// or 128, 16-byte aligned tensors.
+bool paged_decode_serves(const PagedAttnArgs& a, dli_dtype dtype);
 size_t paged_decode_workspace(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim,
-                              int64_t max_keys);
+                              int64_t max_keys, dli_dtype dtype);
 dli_status run_paged_decode(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype, void* workspace,
                             size_t workspace_bytes, cudaStream_t stream);
 
