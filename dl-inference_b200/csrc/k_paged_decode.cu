@@ -17,8 +17,8 @@
 //
 // One producer warp walks the page table and issues the TMA boxes of each block
 // (a page's rows of one head; boxes past the sequence or of a bad page read as
-// zeros) into a ring of stages; four consumer warps take 16 keys each of every
-// 64 keys. Every wait is bounded.
+// zeros), K and V as entries of one ring; the consumer warps take 16 keys of the
+// block each. Every wait is bounded.
 //
 // 4-bit pages: codes arrive by TMA as bytes and become halves in registers, in
 // the order of the MMA fragments: E2M1 x E4M3 has 6 significant bits, so the
@@ -44,42 +44,44 @@ namespace dli_sm100 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kDecodeThreads = 160;  // 4 consumer warps and the producer
-
 struct DecodeArgs {
   PagedAttnArgs a;
-  int tiles_max;        // row tiles of a sequence of max_new tokens
-  int split;            // 0: one CTA per unit
-  int min_blocks;       // split: no CTA takes fewer key blocks (but the last)
-  float* part_o;        // [2 G][rows][D]
-  float2* part_ml;      // [2 G][rows]: running maximum (log2) and sum
-  int2* unit_parts;     // [B * Hkv * tiles_max]: first slot, parts (0: finished in the main kernel)
+  int tiles_max;   // row tiles of a sequence of max_new tokens
+  int split;       // 0: one CTA per unit
+  int min_blocks;  // split: the shares are no smaller, with fewer CTAs at work
+  int ctas;        // split: CTAs of the main kernel
+  float* part_o;   // [2 ctas][rows][D]
+  float2* part_ml; // [2 ctas][rows]: running maximum (log2) and sum
 };
 
+// W consumer warps: 4, or 8 where the ring's entries are small enough. Two CTAs per
+// SM (float32 and two row tiles of 4-bit pages: one).
 template <typename T, typename KV, int D, int NT>
 struct DecodeLayout {
   static constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
   static constexpr bool kF32 = std::is_same<KV, float>::value;
+  static constexpr int W = kFp4 || kF32 || (D == 64 && NT == 1) ? 8 : 4;
+  static constexpr int kThreads = 32 * W + 32;
   static constexpr int R = 8 * NT;
-  static constexpr int BN = kFp4 ? 128 : 64;  // keys per block
-  static constexpr int SUB = BN / 64;         // 16-key groups per warp and block
+  static constexpr int BN = 16 * W;  // keys per block
+  static constexpr int kCtas = kF32 || (kFp4 && (NT == 2 || std::is_same<T, float>::value)) ? 1 : 2;
   static constexpr int kRowBytes = kFp4 ? D / 2 : kF32 ? D * 4 : D * 2;
-  static constexpr int kCodes = BN * kRowBytes;  // code or element bytes of K (or V)
+  static constexpr int kBox = BN * 128;          // bytes of one 128-byte-wide column of boxes
+  static constexpr int kCodes = BN * kRowBytes;  // code or element bytes of a K (or V) block
   static constexpr int kScales = kFp4 ? BN * 8 : 0;  // a TMA box of 64 bytes (D 64, pages of 16) takes 128
-  static constexpr int kStage = 2 * (kCodes + kScales);
-  static constexpr int kStageTx = 2 * (kCodes + (kFp4 ? BN * D / 16 : 0));
-  // 16-bit and 4-bit: two CTAs per SM; float32: one
-  static constexpr int kStages = kFp4   ? (D == 128 ? 5 : 8)
-                                 : kF32 ? (D == 128 ? 3 : 6)
-                                        : (D == 128 ? (NT == 1 ? 3 : 2) : (NT == 1 ? 6 : 5));
-  static constexpr int DH = 64;  // dims that the four warps merge at a time
-  static constexpr int kMergeOff = kStages * kStage;
-  static constexpr int kMerge = 4 * R * DH * 4;
+  static constexpr int kEntry = kCodes + kScales;
+  static constexpr int kEntryTx = kCodes + (kFp4 ? BN * D / 16 : 0);
+  static constexpr int DH = 64;  // dims that the warps merge at a time
+  static constexpr int kMerge = W * R * DH * 4;
+  static constexpr int kMl = 2 * W * R * 4;
+  static constexpr int kRoom = (kCtas == 2 ? 113 : 227) * 1024 - kMerge - kMl - 1024 - 256;
+  static constexpr int kEntries = (kRoom / kEntry) < 16 ? (kRoom / kEntry) : 16;
+  static constexpr int kMergeOff = kEntries * kEntry;
   static constexpr int kMlOff = kMergeOff + kMerge;
-  static constexpr int kMl = 2 * 4 * R * 4;
   static constexpr int kBarOff = kMlOff + kMl;
-  static constexpr int kBytes = kBarOff + 2 * kStages * 8 + 1024;  // the ring's base is rounded up to 1 KiB
-  static_assert(kStage % 1024 == 0, "stage alignment");
+  static constexpr int kBytes = kBarOff + 2 * kEntries * 8 + 1024;  // the ring's base is rounded up to 1 KiB
+  static_assert(kEntry % 1024 == 0, "entry alignment");
+  static_assert(kEntries >= 3, "a ring that overlaps loads with work");
   static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -101,83 +103,90 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int b, bool 
   return w;
 }
 
+// The equal shares of `total` blocks among the CTAs that get any.
+struct Shares {
+  int total, ctas, q, r;
+  __device__ __forceinline__ Shares(int total_blocks, int grid, int min_blocks) : total(total_blocks) {
+    ctas = max(1, min(grid, (total + min_blocks - 1) / min_blocks));
+    q = total / ctas;
+    r = total - q * ctas;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c >= ctas ? total : c * q + min(c, r); }
+  __device__ __forceinline__ int cta_of(int at) const { return at < r * (q + 1) ? at / (q + 1) : r + (at - r * (q + 1)) / max(q, 1); }
+};
+
+// The blocks of all sequences (a whole warp).
+template <int BN, int R>
+__device__ __forceinline__ int list_total(const PagedAttnArgs& a, int lane, bool report) {
+  int total = 0;
+  for (int c = 0; c < a.seqs.batch; c += 32) {
+    if (c + lane < a.seqs.batch) {
+      const SeqWork s = seq_work<BN, R>(a, c + lane, report);
+      total += a.hkv * s.tiles * s.blocks;
+    }
+  }
+  return __reduce_add_sync(0xffffffffu, total);
+}
+
 struct Segment {
   int b, kvh, rt, block, blocks;  // key blocks [block, block + blocks) of the unit
   bool whole;
-  int slot;        // of the part, when not whole
+  int slot;  // of the part, when not whole
   SeqWork w;
-  int64_t unit_w;  // the unit's first place in the work list
 };
 
 // Walks the segments of a CTA's share; every warp runs its own copy.
 template <int BN, int R>
 struct Walker {
   const DecodeArgs& d;
-  int64_t w, w_end, w0, base, total;
-  int64_t ctas;  // CTAs with work
-  int b, next;
+  int w, w_end, w0, base, work, b;
   SeqWork sw;
 
-  __device__ __forceinline__ int64_t work_of(const SeqWork& s) const {
-    return static_cast<int64_t>(d.a.hkv) * s.tiles * s.blocks;
+  __device__ __forceinline__ void take(int seq) {
+    b = seq;
+    sw = seq_work<BN, R>(d.a, seq, false);
+    work = d.a.hkv * sw.tiles * sw.blocks;
   }
 
   __device__ Walker(const DecodeArgs& args, int lane) : d(args) {
-    base = 0;
-    b = -1;
-    next = 0;
-    total = 0;
+    base = b = work = 0;
     if (!d.split) {
       w = 0;
       w_end = 1;
       return;
     }
+    const int total = list_total<BN, R>(d.a, lane, blockIdx.x == 0);
+    const Shares shares(total, d.ctas, d.min_blocks);
+    w0 = w = shares.begin(blockIdx.x);
+    w_end = shares.begin(blockIdx.x + 1);
+    if (w >= w_end) return;
+    // the sequence that holds w (the loads are the first pass's: they hit L1)
     const int batch = d.a.seqs.batch;
     for (int c = 0; c < batch; c += 32) {
-      int64_t mine = 0;
-      if (c + lane < batch) mine = work_of(seq_work<BN, R>(d.a, c + lane, blockIdx.x == 0));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-      total += mine;
-    }
-    const int64_t most = (total + d.min_blocks - 1) / d.min_blocks;
-    ctas = most < static_cast<int64_t>(gridDim.x) ? (most > 0 ? most : 1) : static_cast<int64_t>(gridDim.x);
-    w0 = w = begin_of(blockIdx.x);
-    w_end = begin_of(blockIdx.x + 1ll);
-    if (w >= w_end) return;
-    // the sequence that holds w
-    for (int c = 0; c < batch; c += 32) {
-      int64_t mine = 0;
-      if (c + lane < batch) mine = work_of(seq_work<BN, R>(d.a, c + lane, false));
-      int64_t upto = mine;
+      int mine = 0;
+      if (c + lane < batch) {
+        const SeqWork s = seq_work<BN, R>(d.a, c + lane, false);
+        mine = d.a.hkv * s.tiles * s.blocks;
+      }
+      int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, base + upto <= w);
-      const int k = __popc(past);  // sequences of this chunk that end before w
+      const int k = __popc(__ballot_sync(0xffffffffu, base + upto <= w));  // sequences that end before w
       if (k < 32) {
-        const int64_t before = __shfl_sync(0xffffffffu, upto - mine, k);
-        b = c + k;
-        base += before;
-        break;
+        base += __shfl_sync(0xffffffffu, upto - mine, k);
+        take(c + k);
+        return;
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
     }
-    sw = seq_work<BN, R>(d.a, b, false);
-  }
-  __device__ __forceinline__ int64_t begin_of(int64_t c) const {
-    return c >= ctas ? total : c * (total / ctas) + min(c, total % ctas);
-  }
-  __device__ __forceinline__ int64_t cta_of(int64_t at) const {  // the CTA whose share holds `at`
-    const int64_t q = total / ctas, r = total % ctas;
-    return at < r * (q + 1) ? at / (q + 1) : r + (at - r * (q + 1)) / q;
   }
 
   __device__ bool get(Segment& s) {
+    if (w >= w_end) return false;
     if (!d.split) {
-      if (w >= w_end) return false;
       w = w_end;
       const int per = d.a.hkv * d.tiles_max;
       s.b = blockIdx.x / per;
@@ -189,25 +198,23 @@ struct Walker {
       s.block = s.w.block0;
       s.blocks = s.w.blocks;
       s.whole = true;
+      s.slot = 0;
       return true;
     }
-    if (w >= w_end) return false;
-    while (w >= base + work_of(sw)) {
-      base += work_of(sw);
-      ++b;
-      sw = seq_work<BN, R>(d.a, b, false);
+    while (w >= base + work) {
+      base += work;
+      take(b + 1);
     }
-    const int64_t rel = w - base;
-    const int unit = static_cast<int>(rel / sw.blocks), blk = static_cast<int>(rel - static_cast<int64_t>(unit) * sw.blocks);
+    const int rel = w - base;
+    const int unit = rel / sw.blocks, blk = rel - unit * sw.blocks;
     s.b = b;
     s.kvh = unit / sw.tiles;
     s.rt = unit - s.kvh * sw.tiles;
     s.w = sw;
     s.block = sw.block0 + blk;
-    s.blocks = static_cast<int>(min(static_cast<int64_t>(sw.blocks - blk), w_end - w));
+    s.blocks = min(sw.blocks - blk, w_end - w);
     s.whole = s.blocks == sw.blocks;
     s.slot = 2 * blockIdx.x + (w == w0 ? 0 : 1);
-    s.unit_w = base + static_cast<int64_t>(unit) * sw.blocks;
     w += s.blocks;
     return true;
   }
@@ -220,14 +227,14 @@ __device__ __forceinline__ void store4(T* dst, float x, float y, float z, float 
   else *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(x, y), pack16<T>(z, w));
 }
 
-// Byte offset of (key row, 16-bit column) in a K or V stage of D/64 boxes of
-// [64 keys][64 elements] with the 128-byte swizzle.
-__device__ __forceinline__ int swz128(int row, int col) {
-  return (col >> 6) * (64 * 128) + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4) + (col & 7) * 2;
+// Byte offset of (key row, 16-bit column) in a K or V block of columns of `box` bytes:
+// [keys][64 elements] with the 128-byte swizzle.
+__device__ __forceinline__ int swz128(int box, int row, int col) {
+  return (col >> 6) * box + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4) + (col & 7) * 2;
 }
 
 template <typename T, typename KV, int D, int NT>
-__global__ void __launch_bounds__(kDecodeThreads)
+__global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLayout<T, KV, D, NT>::kCtas)
     attn_paged_decode_kernel(const DecodeArgs d, const __grid_constant__ CUtensorMap tk,
                              const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tks,
                              const __grid_constant__ CUtensorMap tvs) {
@@ -235,22 +242,22 @@ __global__ void __launch_bounds__(kDecodeThreads)
   using MT = typename std::conditional<L::kFp4, __half, T>::type;  // MMA operand type of 16-bit MMAs
   constexpr bool kF32 = L::kF32;
   constexpr int QS = L::kFp4 && std::is_same<T, float>::value ? 2 : 1;  // halves that make up a q or p
-  constexpr int BN = L::BN, SUB = L::SUB, R = L::R, ST = L::kStages;
+  constexpr int BN = L::BN, R = L::R, E = L::kEntries, W = L::W;
   extern __shared__ uint8_t smem_base[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_base) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* empty = full + ST;
+  uint64_t* empty = full + E;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedAttnArgs& a = d.a;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
+    for (int s = 0; s < E; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 4);
+      mbar_init(&empty[s], W);
     }
     mbar_fence_init();
   }
-  if (threadIdx.x == 128) {
+  if (threadIdx.x == 32 * W) {
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tv);
   }
@@ -262,11 +269,11 @@ __global__ void __launch_bounds__(kDecodeThreads)
   // scale bytes of row r: r * D/16 + (r / 16) * scale_pad
   const int scale_pad = L::kFp4 && D == 64 && a.seqs.page_shift == 4 ? 64 : 0;
 
-  if (warp == 4) {
+  if (warp == W) {
     // ---- producer: page ids (32 at a time, the next 32 already asked for) and TMA boxes
     const int shift = a.seqs.page_shift, page_rows = 1 << shift;
     const int box_rows = min(page_rows, BN), boxes = BN / box_rows;
-    int it = 0, last_it = 0;
+    int at = 0;  // ring entries filled: 2 per block, K then V
     bool alive = true;
     while (alive && walk.get(seg)) {
       const int32_t* ids = a.seqs.page_table + seg.b * a.seqs.max_pages;
@@ -278,7 +285,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
       };
       int chunk = ((seg.block * BN) >> shift) >> 5;
       int cur = fetch(chunk), nxt = fetch(chunk + 1);
-      for (int j = 0; j < seg.blocks; ++j, ++it) {
+      for (int j = 0; j < seg.blocks && alive; ++j) {
         const int key0 = (seg.block + j) * BN;
         const int first = key0 >> shift;
         if ((first >> 5) != chunk) {
@@ -292,51 +299,46 @@ __global__ void __launch_bounds__(kDecodeThreads)
           set_device_error(a.seqs.err, kDevErrPageIndex);
           page = none;
         }
-        const int st = it % ST;
-        const bool free_stage = mbar_wait(&empty[st], ((it / ST) & 1) ^ 1);
-        if (!__all_sync(0xffffffffu, free_stage)) {
-          if (lane == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
-          alive = false;
-          break;
-        }
-        uint8_t* sk = smem + st * L::kStage;
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], L::kStageTx);
-        __syncwarp();
-        if (lane < boxes) {
-          const int row = key0 & (page_rows - 1);  // 0 unless a page holds several blocks
-          const int at = lane * box_rows;
-          if constexpr (L::kFp4) {
-            uint8_t* sv = sk + L::kCodes;
-            uint8_t* ss = sv + L::kCodes;
-            tma_load_4d(sk + at * (D / 2), &tk, 0, row, seg.kvh, page, &full[st]);
-            tma_load_4d(sv + at * (D / 2), &tv, 0, row, seg.kvh, page, &full[st]);
-            const int sat = at * (D / 16) + lane * scale_pad;
-            tma_load_4d(ss + sat, &tks, 0, 0, seg.kvh, page, &full[st]);
-            tma_load_4d(ss + L::kScales + sat, &tvs, 0, 0, seg.kvh, page, &full[st]);
-          } else {
-            uint8_t* sv = sk + L::kCodes;
-            constexpr int kBoxWidth = kF32 ? 128 : 64;  // in the map's units: bytes or 16-bit elements
+        const int row = key0 & (page_rows - 1);  // 0 unless a page holds several blocks
+        const int box_at = lane * box_rows;
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which, ++at) {
+          const int e = at % E;
+          const bool free_entry = mbar_wait(&empty[e], ((at / E) & 1) ^ 1);
+          if (!__all_sync(0xffffffffu, free_entry)) {
+            if (lane == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
+            alive = false;
+            break;
+          }
+          uint8_t* dst = smem + e * L::kEntry;
+          if (lane == 0) mbar_arrive_expect_tx(&full[e], L::kEntryTx);
+          __syncwarp();
+          if (lane < boxes) {
+            const CUtensorMap* map = which ? &tv : &tk;
+            if constexpr (L::kFp4) {
+              tma_load_4d(dst + box_at * (D / 2), map, 0, row, seg.kvh, page, &full[e]);
+              tma_load_4d(dst + L::kCodes + box_at * (D / 16) + lane * scale_pad, which ? &tvs : &tks, 0, 0, seg.kvh, page, &full[e]);
+            } else {
+              constexpr int kBoxWidth = kF32 ? 128 : 64;  // in the map's units: bytes or 16-bit elements
 #pragma unroll
-            for (int c = 0; c < L::kRowBytes / 128; ++c) {
-              tma_load_4d(sk + c * (64 * 128) + at * 128, &tk, c * kBoxWidth, row, seg.kvh, page, &full[st]);
-              tma_load_4d(sv + c * (64 * 128) + at * 128, &tv, c * kBoxWidth, row, seg.kvh, page, &full[st]);
+              for (int c = 0; c < L::kRowBytes / 128; ++c)
+                tma_load_4d(dst + c * L::kBox + box_at * 128, map, c * kBoxWidth, row, seg.kvh, page, &full[e]);
             }
           }
+          __syncwarp();
         }
-        __syncwarp();
-        last_it = it + 1;
       }
     }
     // no copy may still be writing shared memory when the CTA exits
-    for (int i = max(0, last_it - ST); i < last_it; ++i) mbar_wait(&full[i % ST], (i / ST) & 1);
+    for (int i = max(0, at - E); i < at; ++i) mbar_wait(&full[i % E], (i / E) & 1);
     return;
   }
 
   // ---- consumers
   const int g = lane >> 2, t = lane & 3;
   float* merge = reinterpret_cast<float*>(smem + L::kMergeOff);
-  float* wm = reinterpret_cast<float*>(smem + L::kMlOff);  // [4][R]
-  float* wl = wm + 4 * R;
+  float* wm = reinterpret_cast<float*>(smem + L::kMlOff);  // [W][R]
+  float* wl = wm + W * R;
   // MMA key row x of a 16-key group holds key perm(x): the fragment reads of 4-bit V
   // and of float32 K and V then fall into different banks
   auto perm = [](int x) {
@@ -345,8 +347,9 @@ __global__ void __launch_bounds__(kDecodeThreads)
   };
   const float cap_out = a.softcap * kLog2e;
   const float base_scale = a.softcap > 0.f ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
-  int it = 0;
+  int at = 0;  // ring entries consumed
   bool alive = true;
+  const int kw = warp * 16;  // this warp's keys of every block
 
   while (walk.get(seg)) {
     const int rows_left = seg.w.rows.n * a.group - seg.rt * R;
@@ -432,30 +435,35 @@ __global__ void __launch_bounds__(kDecodeThreads)
       l[nt][0] = l[nt][1] = 0.f;
     }
 
-    for (int j = 0; j < seg.blocks; ++j, ++it) {
-      const int st = it % ST;
-      if (alive) {
-        const bool got = mbar_wait(&full[st], (it / ST) & 1);
+    for (int j = 0; j < seg.blocks; ++j) {
+      // waits for ring entry `at`; one that runs out skips the remaining blocks, with
+      // every barrier of the CTA still met
+      auto arrived = [&]() {
+        const bool got = mbar_wait(&full[at % E], (at / E) & 1);
         if (!__all_sync(0xffffffffu, got)) {
           if (lane == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
-          alive = false;  // the remaining blocks are skipped, every barrier is still met
+          alive = false;
         }
-      }
-      if (!alive) continue;
-      uint8_t* sk = smem + st * L::kStage;
-      uint8_t* sv = sk + L::kCodes;
+        return alive;
+      };
+      auto release = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[at % E]);
+        ++at;
+      };
+      if (!alive || !arrived()) continue;
+      const uint8_t* sk = smem + (at % E) * L::kEntry;
       const int blk_key = (seg.block + j) * BN;
 
       // S^T = K Q^T
-      float sc[SUB][NT][4];
-#pragma unroll
-      for (int u = 0; u < SUB; ++u) {
-        const int kw = u * 64 + warp * 16;
+      float sc[1][NT][4];
+      {
+        constexpr int u = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sc[u][nt][0] = sc[u][nt][1] = sc[u][nt][2] = sc[u][nt][3] = 0.f;
         if constexpr (L::kFp4) {
           const int r0 = kw + perm(g), r1 = kw + perm(g + 8);
-          const uint8_t* ss = sv + L::kCodes;
+          const uint8_t* ss = sk + L::kCodes;
           uint32_t w0[D / 32], w1[D / 32], s0[D / 64], s1[D / 64];
           if constexpr (D == 128) {
             const uint4 c0 = *reinterpret_cast<const uint4*>(sk + r0 * 64 + ((t ^ ((r0 >> 1) & 3)) << 4));
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
             for (int i = 0; i < 4; ++i) low[nt][i] = part[nt][0][i] = part[nt][1][i] = part[nt][2][i] = part[nt][3][i] = 0.f;
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
-            const uint8_t* box = sk + (kk >> 1) * (64 * 128);
+            const uint8_t* box = sk + (kk >> 1) * L::kBox;
             const int ch = (kk & 1) * 4 + t;
             const float4 k0 = *reinterpret_cast<const float4*>(box + r0 * 128 + ((ch ^ (r0 & 7)) << 4));
             const float4 k1 = *reinterpret_cast<const float4*>(box + r1 * 128 + ((ch ^ (r1 & 7)) << 4));
@@ -533,12 +541,14 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
             uint32_t f[4];
-            ldmatrix_x4(f, ks + swz128(kw + (lane & 15), kk * 16 + (lane >> 4) * 8));
+            ldmatrix_x4(f, ks + swz128(L::kBox, kw + (lane & 15), kk * 16 + (lane >> 4) * 8));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_16816<MT>(sc[u][nt], f[0], f[1], f[2], f[3], qf[nt][kk][0], qf[nt][kk][1]);
           }
         }
       }
+
+      release();
 
       // scores in log2 units, cap, bias and mask
       float mx[NT][2];
@@ -546,13 +556,12 @@ __global__ void __launch_bounds__(kDecodeThreads)
       for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
       const bool edge = blk_key + BN > seg.w.rows.past + 1 || blk_key < seg.w.kv_len - a.window;
 #pragma unroll
-      for (int u = 0; u < SUB; ++u)
-#pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
+            constexpr int u = 0;
             const int e = i & 1;
-            const int key = blk_key + u * 64 + warp * 16 + perm(g + (i >> 1) * 8);
+            const int key = blk_key + kw + perm(g + (i >> 1) * 8);
             float x = sc[u][nt][i] * rscale[nt][e];
             if (a.softcap > 0.f) x = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(x));
             if (a.slopes) x = fmaf(slope[nt][e], static_cast<float>(key - pos[nt][e]), x);
@@ -589,9 +598,10 @@ __global__ void __launch_bounds__(kDecodeThreads)
       }
 
       // O^T += V^T P^T
-#pragma unroll
-      for (int u = 0; u < SUB; ++u) {
-        const int kw = u * 64 + warp * 16;
+      if (!arrived()) continue;
+      uint8_t* sv = smem + (at % E) * L::kEntry;
+      {
+        constexpr int u = 0;
         uint32_t pb[NT][kF32 ? 4 : 2 * QS];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -625,7 +635,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
         const int key_first = blk_key + kw;
         const bool stale = key_first + 16 > seg.w.kv_len || key_first < seg.w.key_lo;
         if constexpr (L::kFp4) {
-          const uint8_t* ss = sv + L::kCodes + L::kScales;
+          const uint8_t* ss = sv + L::kCodes;
           const int rw[4] = {kw + perm(2 * t), kw + perm(2 * t + 1), kw + perm(2 * t + 8), kw + perm(2 * t + 9)};
           uint32_t c[4][D / 64], sb[4];
 #pragma unroll
@@ -677,9 +687,9 @@ __global__ void __launch_bounds__(kDecodeThreads)
             for (int c = lane; c < 16 * (L::kRowBytes / 16); c += 32) {
               const int r = (c >> 3) & 15, box = c >> 7;
               if (key_first + r >= seg.w.kv_len || key_first + r < seg.w.key_lo)
-                *reinterpret_cast<uint4*>(sv + box * (64 * 128) + (kw + r) * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(sv + box * L::kBox + (kw + r) * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
-            fence_proxy_async_smem();  // before the stage is given back to the TMA
+            fence_proxy_async_smem();  // before the entry is given back to the TMA
             __syncwarp();
           }
           if constexpr (kF32) {
@@ -687,7 +697,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
             const int chunk = ((g & 1) << 2) | (g >> 1);
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
-              const uint8_t* box = sv + i * (64 * 128);
+              const uint8_t* box = sv + i * L::kBox;
               float part[NT][2][4], low[NT][2][4];
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
@@ -727,18 +737,17 @@ __global__ void __launch_bounds__(kDecodeThreads)
 #pragma unroll
           for (int i = 0; i < KK; ++i) {
             uint32_t f[4];
-            ldmatrix_x4_trans(f, vs + swz128(kw + (lane & 7) + (lane >> 4) * 8, i * 16 + ((lane >> 3) & 1) * 8));
+            ldmatrix_x4_trans(f, vs + swz128(L::kBox, kw + (lane & 7) + (lane >> 4) * 8, i * 16 + ((lane >> 3) & 1) * 8));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_16816<MT>(o[nt][i], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
           }
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
+      release();
     }
 
-    // ---- merge the four warps in order, then store the rows or the part
+    // ---- merge the warps in order, then store the rows or the part
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -750,7 +759,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
           wl[warp * R + nt * 8 + 2 * t + e] = l[nt][e];
         }
       }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory");
     constexpr int DH = L::DH;
 #pragma unroll
     for (int half = 0; half < D / DH; ++half) {
@@ -762,7 +771,7 @@ __global__ void __launch_bounds__(kDecodeThreads)
           const int r = nt * 8 + 2 * t + e;
           float top = -INFINITY;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) top = fmaxf(top, wm[w * R + r]);
+          for (int w = 0; w < W; ++w) top = fmaxf(top, wm[w * R + r]);
           f[e] = m[nt][e] == -INFINITY ? 0.f : exp2_approx(m[nt][e] - top);
         }
 #pragma unroll
@@ -777,15 +786,15 @@ __global__ void __launch_bounds__(kDecodeThreads)
               merge[(warp * R + nt * 8 + 2 * t + (k & 1)) * DH + (dim - half * DH)] = o[nt][i][k] * f[k & 1];
           }
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      for (int c = threadIdx.x; c < rows * (DH / 4); c += 128) {
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory");
+      for (int c = threadIdx.x; c < rows * (DH / 4); c += 32 * W) {
         const int r = c / (DH / 4), x = (c - r * (DH / 4)) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         float top = -INFINITY, den = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, wm[w * R + r]);
+        for (int w = 0; w < W; ++w) top = fmaxf(top, wm[w * R + r]);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
           const float4 v = *reinterpret_cast<const float4*>(&merge[(w * R + r) * DH + x]);
           sum.x += v.x;
           sum.y += v.y;
@@ -805,62 +814,112 @@ __global__ void __launch_bounds__(kDecodeThreads)
           if (dim == 0) d.part_ml[static_cast<int64_t>(seg.slot) * R + r] = make_float2(top, den);
         }
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-    }
-    if (d.split && threadIdx.x == 0 && seg.block == seg.w.block0) {
-      // the unit's first CTA says which slots hold its parts
-      int2 parts = make_int2(0, 0);
-      if (!seg.whole)
-        parts = make_int2(seg.slot, static_cast<int>(walk.cta_of(seg.unit_w + seg.w.blocks - 1) - blockIdx.x) + 1);
-      d.unit_parts[(static_cast<int64_t>(seg.b) * a.hkv + seg.kvh) * d.tiles_max + seg.rt] = parts;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory");
     }
   }
 }
 
-// Merges the parts of the units that were split, in order: slot 0 of the parts is
-// the unit's first, the others are the first slots of the CTAs after it.
-template <typename T, int D, int R>
+// Merges the parts of the units that were split, in the order of the list: the first
+// part's slot is its CTA's first or second, the others are the first slots of the
+// CTAs after it. grid = (units, D / 32); thread = (parts lane, row, 4 dims). Which
+// parts there are is worked out while the main kernel still runs: positions and starts
+// were final before that began.
+template <typename T, int D, int BN, int R>
 __global__ void __launch_bounds__(256) attn_paged_combine_kernel(const DecodeArgs d) {
-  DLI_PDL_ENTRY();
   const PagedAttnArgs& a = d.a;
   const int u = blockIdx.x, rt = u % d.tiles_max, kvh = u / d.tiles_max % a.hkv, b = u / d.tiles_max / a.hkv;
-  const SeqRows sr = seq_rows(a.seqs, b, false);
-  const int rows = min(sr.n * a.group - rt * R, R);
-  if (rows <= 0) return;
-  const int2 parts = d.unit_parts[u];
-  if (parts.y == 0) return;
-  const int cta = parts.x / 2;
-  for (int c = threadIdx.x; c < rows * (D / 4); c += 256) {
-    const int r = c / (D / 4), x = (c - r * (D / 4)) * 4;
-    float top = -INFINITY, den = 0.f;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < parts.y; ++p) {
-      const int64_t slot = p == 0 ? parts.x : 2 * (cta + p);
-      top = fmaxf(top, d.part_ml[slot * R + r].x);
+  const int lane = threadIdx.x & 31;
+  constexpr int ITEMS = R * 8, LANES = 256 / ITEMS;
+  __shared__ float4 so[LANES][ITEMS];
+  __shared__ float2 sml[LANES][ITEMS];
+
+  const SeqWork sw = seq_work<BN, R>(a, b, false);
+  const int rows = min(sw.rows.n * a.group - rt * R, R);
+  int total = 0, base = 0;
+  for (int c = 0; c < a.seqs.batch; c += 32) {
+    if (c + lane < a.seqs.batch) {
+      const SeqWork s = seq_work<BN, R>(a, c + lane, false);
+      const int work = a.hkv * s.tiles * s.blocks;
+      total += work;
+      if (c + lane < b) base += work;
     }
-#pragma unroll 4
-    for (int p = 0; p < parts.y; ++p) {
-      const int64_t slot = p == 0 ? parts.x : 2 * (cta + p);
-      const float2 ml = d.part_ml[slot * R + r];
-      const float4 v = *reinterpret_cast<const float4*>(d.part_o + (slot * R + r) * D + x);
-      const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
-      den += ml.y * f;
-      sum.x += v.x * f;
-      sum.y += v.y * f;
-      sum.z += v.z * f;
-      sum.w += v.w * f;
-    }
-    const int rr = rt * R + r, tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
-    const float inv = a.v_scale / den;
-    store4(static_cast<T*>(a.out) + ((sr.row0 + tok) * a.hq + h) * D + x, sum.x * inv, sum.y * inv, sum.z * inv,
-           sum.w * inv);
   }
+  total = __reduce_add_sync(0xffffffffu, total);
+  base = __reduce_add_sync(0xffffffffu, base);
+  const Shares shares(total, d.ctas, d.min_blocks);
+  const int begin = base + (kvh * sw.tiles + rt) * sw.blocks;
+  int first = 0, parts = 1;
+  if (rows > 0) {
+    first = shares.cta_of(begin);
+    parts = shares.cta_of(begin + sw.blocks - 1) - first + 1;
+  }
+  pdl_wait();
+  pdl_trigger();
+  if (rows <= 0 || parts == 1) return;  // uniform for the CTA
+
+  const int item = threadIdx.x % ITEMS, pl = threadIdx.x / ITEMS;
+  const int r = item >> 3, dim = blockIdx.y * 32 + (item & 7) * 4;
+  const int slot0 = begin == shares.begin(first) ? 2 * first : 2 * first + 1;
+  float top = -INFINITY, den = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (r < rows) {
+    for (int p0 = pl; p0 < parts; p0 += 4 * LANES) {
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int p = p0 + k * LANES;
+        ml[k] = make_float2(-INFINITY, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < parts) {
+          const int64_t slot = p == 0 ? slot0 : 2 * (first + p);
+          ml[k] = d.part_ml[slot * R + r];
+          v[k] = *reinterpret_cast<const float4*>(d.part_o + (slot * R + r) * D + dim);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (ml[k].x == -INFINITY) continue;  // a part in which the row sees no key
+        const float m = fmaxf(top, ml[k].x);
+        const float f = exp2_approx(top - m), f2 = exp2_approx(ml[k].x - m);  // top = -inf: 0
+        top = m;
+        den = den * f + ml[k].y * f2;
+        sum.x = sum.x * f + v[k].x * f2;
+        sum.y = sum.y * f + v[k].y * f2;
+        sum.z = sum.z * f + v[k].z * f2;
+        sum.w = sum.w * f + v[k].w * f2;
+      }
+    }
+  }
+  so[pl][item] = sum;
+  sml[pl][item] = make_float2(top, den);
+  __syncthreads();
+  if (pl > 0 || r >= rows) return;
+#pragma unroll
+  for (int k = 1; k < LANES; ++k) top = fmaxf(top, sml[k][item].x);
+  den = 0.f;
+  sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < LANES; ++k) {
+    const float2 ml = sml[k][item];
+    const float4 v = so[k][item];
+    const float f = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+    den += ml.y * f;
+    sum.x += v.x * f;
+    sum.y += v.y * f;
+    sum.z += v.z * f;
+    sum.w += v.w * f;
+  }
+  const int rr = rt * R + r, tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
+  const float inv = a.v_scale / den;
+  store4(static_cast<T*>(a.out) + ((sw.rows.row0 + tok) * a.hq + h) * D + dim, sum.x * inv, sum.y * inv, sum.z * inv,
+         sum.w * inv);
 }
 
 // ---- host ------------------------------------------------------------------------
 
 // CTAs that are resident at once, per kernel and device.
-int resident_ctas(const void* kernel, int smem) {
+int resident_ctas(const void* kernel, int threads, int smem) {
   static std::mutex mu;
   static std::map<std::pair<int, const void*>, int> cache;
   int dev = 0;
@@ -872,7 +931,7 @@ int resident_ctas(const void* kernel, int smem) {
   auto it = cache.find({dev, kernel});
   if (it != cache.end()) return it->second;
   int n = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kDecodeThreads, smem) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
@@ -901,13 +960,14 @@ DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t 
   p.nt = rows <= 8 || f32 ? 1 : 2;  // two row tiles of split operands do not fit the registers
   p.tiles_max = static_cast<int>(ceil_div(rows, 8 * p.nt));
   p.units = batch * hkv * p.tiles_max;
-  p.split = max_keys > kWholeKeys;
+  // the list's length has to fit an int (a longer one is never short of CTAs)
+  p.split = max_keys > kWholeKeys && p.units * (max_keys / 64 + 2) < INT_MAX;
   p.grid = p.split ? static_cast<int64_t>(sm_count()) * kMaxCtasPerSm : p.units;
   if (p.split) {
     const int64_t r = 8 * p.nt;
     p.part_o = static_cast<size_t>(2 * p.grid * r * head_dim) * 4;
     p.part_ml = static_cast<size_t>(2 * p.grid * r) * 8;
-    p.workspace = p.part_o + p.part_ml + static_cast<size_t>(p.units) * 8;
+    p.workspace = p.part_o + p.part_ml;
   }
   return p;
 }
@@ -930,17 +990,17 @@ dli_status launch_paged_decode(const PagedAttnArgs& a, const DecodePlan& plan, v
   d.a = a;
   d.tiles_max = plan.tiles_max;
   d.split = plan.split ? 1 : 0;
-  d.min_blocks = kMinKeys / L::BN;
+  d.min_blocks = std::max(1, kMinKeys / L::BN);
   int64_t grid = plan.grid;
   if (plan.split) {
     d.part_o = static_cast<float*>(workspace);
     d.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.part_o);
-    d.unit_parts = reinterpret_cast<int2*>(static_cast<uint8_t*>(workspace) + plan.part_o + plan.part_ml);
-    grid = std::min<int64_t>(grid, std::max(1, resident_ctas(reinterpret_cast<const void*>(kern), L::kBytes)));
+    grid = std::min<int64_t>(grid, std::max(1, resident_ctas(reinterpret_cast<const void*>(kern), L::kThreads, L::kBytes)));
+    d.ctas = static_cast<int>(grid);
   }
-  launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kDecodeThreads), L::kBytes, stream, d, tk, tv, tks, tvs);
+  launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(L::kThreads), L::kBytes, stream, d, tk, tv, tks, tvs);
   if (plan.split)
-    launch_pdl(attn_paged_combine_kernel<T, D, L::R>, dim3(static_cast<unsigned>(plan.units)), dim3(256), 0, stream, d);
+    launch_pdl(attn_paged_combine_kernel<T, D, L::BN, L::R>, dim3(static_cast<unsigned>(plan.units), D / 32), dim3(256), 0, stream, d);
   return check_launch("attention_paged", plan.split ? 2 : 1);
 }
 
