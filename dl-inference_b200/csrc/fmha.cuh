@@ -38,9 +38,9 @@ bool fmha_required();
 dli_status make_map_4d(CUtensorMap* map, const void* base, bool bf16, const uint64_t (&dims)[4],
                        const uint64_t (&strides)[3], const uint32_t (&box)[4]);
 
-// The same over bytes, with the 64- or 128-byte swizzle or none (0).
+// The same over bytes.
 dli_status make_map_4d_bytes(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                             const uint32_t (&box)[4], int swizzle);
+                             const uint32_t (&box)[4]);
 
 // Launches the kernel on `stream` (fmha_supported() must hold). Returns
 // DLI_ERR_UNSUPPORTED, launching nothing, when a tensor map cannot be encoded.

@@ -566,20 +566,17 @@ dli_status make_map_4d(CUtensorMap* map, const void* base, bool bf16, const uint
   return DLI_OK;
 }
 
-// The same over bytes, with the 64- or 128-byte swizzle or none (0).
+// The same over bytes.
 dli_status make_map_4d_bytes(CUtensorMap* map, const void* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3],
-                             const uint32_t (&box)[4], int swizzle) {
+                             const uint32_t (&box)[4]) {
   EncodeTiledFn fn = encode_tiled();
   if (fn == nullptr) return fail(DLI_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
   const cuuint64_t s[3] = {strides[0], strides[1], strides[2]};
   const cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
   const cuuint32_t es[4] = {1, 1, 1, 1};
-  const CUtensorMapSwizzle mode = swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                  : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                  : CU_TENSOR_MAP_SWIZZLE_NONE;
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), d, s, bx, es,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, mode, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(DLI_ERR_UNSUPPORTED, "attention: cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));

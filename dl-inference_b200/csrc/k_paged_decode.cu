@@ -20,8 +20,9 @@
 // zeros), K and V as entries of one ring; the consumer warps take 16 keys of the
 // block each. Every wait is bounded.
 //
-// 4-bit pages: codes arrive by TMA as bytes and become halves in registers, in
-// the order of the MMA fragments: E2M1 x E4M3 has 6 significant bits, so the
+// 4-bit pages: a (page, head) block is contiguous and arrives by one untiled bulk
+// copy (tiled boxes of 64- and 16-byte rows held the TMA at 3.8 TB/s); codes
+// become halves in registers, in the order of the MMA fragments: E2M1 x E4M3 has 6 significant bits, so the
 // products are exact, and the MMA runs in f16 for every model type. q is scaled
 // by a power of two per row for that, which is exact too; a float32 q, and its P,
 // enter as two halves each (22 bits).
@@ -34,7 +35,8 @@
 #include <climits>
 #include <map>
 #include <mutex>
-#include <tuple>
+#include <type_traits>
+#include <utility>
 
 #include "mma_sync.cuh"
 #include "paged_attn.cuh"
@@ -60,17 +62,16 @@ template <typename T, typename KV, int D, int NT>
 struct DecodeLayout {
   static constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
   static constexpr bool kF32 = std::is_same<KV, float>::value;
-  static constexpr int W = kFp4 || kF32 || (D == 64 && NT == 1) ? 8 : 4;
+  static constexpr int W = kF32 || (!kFp4 && D == 64 && NT == 1) ? 8 : 4;
+  static constexpr int SUB = kFp4 ? 2 : 1;  // 16-key groups of a warp per block
   static constexpr int kThreads = 32 * W + 32;
   static constexpr int R = 8 * NT;
-  static constexpr int BN = 16 * W;  // keys per block
+  static constexpr int BN = 16 * W * SUB;  // keys per block
   static constexpr int kCtas = kF32 || (kFp4 && (NT == 2 || std::is_same<T, float>::value)) ? 1 : 2;
   static constexpr int kRowBytes = kFp4 ? D / 2 : kF32 ? D * 4 : D * 2;
   static constexpr int kBox = BN * 128;          // bytes of one 128-byte-wide column of boxes
   static constexpr int kCodes = BN * kRowBytes;  // code or element bytes of a K (or V) block
-  static constexpr int kScales = kFp4 ? BN * 8 : 0;  // a TMA box of 64 bytes (D 64, pages of 16) takes 128
-  static constexpr int kEntry = kCodes + kScales;
-  static constexpr int kEntryTx = kCodes + (kFp4 ? BN * D / 16 : 0);
+  static constexpr int kEntry = kCodes + (kFp4 ? BN * D / 16 : 0);
   static constexpr int DH = 64;  // dims that the warps merge at a time
   static constexpr int kMerge = W * R * DH * 4;
   static constexpr int kMl = 2 * W * R * 4;
@@ -80,7 +81,7 @@ struct DecodeLayout {
   static constexpr int kMlOff = kMergeOff + kMerge;
   static constexpr int kBarOff = kMlOff + kMl;
   static constexpr int kBytes = kBarOff + 2 * kEntries * 8 + 1024;  // the ring's base is rounded up to 1 KiB
-  static_assert(kEntry % 1024 == 0, "entry alignment");
+  static_assert(kEntry % (kFp4 ? 16 : 1024) == 0, "entry alignment");
   static_assert(kEntries >= 3, "a ring that overlaps loads with work");
   static_assert(kBytes <= 232448, "shared memory");
 };
@@ -233,16 +234,259 @@ __device__ __forceinline__ int swz128(int box, int row, int col) {
   return (col >> 6) * box + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) << 4) + (col & 7) * 2;
 }
 
+// ---- the two products of 16 keys: S^T = K Q^T (sc is written) and O^T += V^T P^T
+// (sc holds p). sc[nt][i]: key row g (+ 8 for i >= 2), query row nt * 8 + 2t + (i & 1).
+
+template <typename T, int D, int NT>
+__device__ __forceinline__ void qk_16(float (&sc)[NT][4], uint32_t k, int box, int kw, int lane,
+                                      const uint32_t (&qf)[NT][D / 16][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    uint32_t f[4];
+    ldmatrix_x4(f, k + swz128(box, kw + (lane & 15), kk * 16 + (lane >> 4) * 8));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mma_16816<T>(sc[nt], f[0], f[1], f[2], f[3], qf[nt][kk][0], qf[nt][kk][1]);
+  }
+}
+template <typename T, int D, int NT>
+__device__ __forceinline__ void pv_16(float (&o)[NT][D / 16][4], const float (&p)[NT][4], uint32_t v, int box, int kw, int lane) {
+  uint32_t pb[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    pb[nt][0] = movmatrix_trans(pack16<T>(p[nt][0], p[nt][1]));
+    pb[nt][1] = movmatrix_trans(pack16<T>(p[nt][2], p[nt][3]));
+  }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    uint32_t f[4];
+    ldmatrix_x4_trans(f, v + swz128(box, kw + (lane & 7) + (lane >> 4) * 8, i * 16 + ((lane >> 3) & 1) * 8));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mma_16816<T>(o[nt][i], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
+  }
+}
+
+// float32: K rows perm(g), perm(g) + 8 by 16 bytes, 4 dims of each 16.
+template <int D, int NT>
+__device__ __forceinline__ void qk_f32(float (&sc)[NT][4], const uint8_t* sk, int box, int kw, int g, int t,
+                                       const uint32_t (&qf)[NT][D / 16][4]) {
+  const int r0 = kw + ((g >> 1) | ((g & 1) << 2)), r1 = r0 + 8;
+  float part[NT][4][4], low[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) low[nt][i] = part[nt][0][i] = part[nt][1][i] = part[nt][2][i] = part[nt][3][i] = 0.f;
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    const uint8_t* col = sk + (kk >> 1) * box;
+    const int ch = (kk & 1) * 4 + t;
+    const float4 k0 = *reinterpret_cast<const float4*>(col + r0 * 128 + ((ch ^ (r0 & 7)) << 4));
+    const float4 k1 = *reinterpret_cast<const float4*>(col + r1 * 128 + ((ch ^ (r1 & 7)) << 4));
+    uint32_t hi[2][4], lo[2][4];
+    split_tf32(k0.x, hi[0][0], lo[0][0]);
+    split_tf32(k1.x, hi[0][1], lo[0][1]);
+    split_tf32(k0.y, hi[0][2], lo[0][2]);
+    split_tf32(k1.y, hi[0][3], lo[0][3]);
+    split_tf32(k0.z, hi[1][0], lo[1][0]);
+    split_tf32(k1.z, hi[1][1], lo[1][1]);
+    split_tf32(k0.w, hi[1][2], lo[1][2]);
+    split_tf32(k1.w, hi[1][3], lo[1][3]);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float(&acc)[4] = part[nt][kk & 3];
+      mma_1688_f32(acc, low[nt], hi[0], lo[0], __uint_as_float(qf[nt][kk][0]), __uint_as_float(qf[nt][kk][1]));
+      mma_1688_f32(acc, low[nt], hi[1], lo[1], __uint_as_float(qf[nt][kk][2]), __uint_as_float(qf[nt][kk][3]));
+    }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      sc[nt][i] = low[nt][i] + ((part[nt][0][i] + part[nt][1][i]) + (part[nt][2][i] + part[nt][3][i]));
+}
+// V: the 4 dims of 16-byte chunk c(g) of each 32, of the keys perm(2t) = t and
+// perm(2t + 1) = t + 4 of each 8.
+__device__ __forceinline__ int f32_chunk(int g) { return ((g & 1) << 2) | (g >> 1); }
+template <int D, int NT>
+__device__ __forceinline__ void pv_f32(float (&o)[NT][D / 16][4], const float (&p)[NT][4], const uint8_t* sv, int box, int kw,
+                                       int g, int t) {
+  float pb[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    // P^T as the B operand: lane (g, t) gets rows g of the keys 2t, 2t + 1 (+ 8)
+    const int s0 = 8 * t + (g >> 1), s1 = s0 + 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float x0 = __shfl_sync(0xffffffffu, p[nt][2 * h], s0), y0 = __shfl_sync(0xffffffffu, p[nt][2 * h + 1], s0);
+      const float x1 = __shfl_sync(0xffffffffu, p[nt][2 * h], s1), y1 = __shfl_sync(0xffffffffu, p[nt][2 * h + 1], s1);
+      pb[nt][2 * h] = (g & 1) ? y0 : x0;
+      pb[nt][2 * h + 1] = (g & 1) ? y1 : x1;
+    }
+  }
+  const int chunk = f32_chunk(g);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const uint8_t* col = sv + i * box;
+    float part[NT][2][4], low[NT][2][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) part[nt][0][k] = part[nt][1][k] = low[nt][0][k] = low[nt][1][k] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int ra = kw + h * 8 + t, rb = ra + 4;
+      const float4 va = *reinterpret_cast<const float4*>(col + ra * 128 + ((chunk ^ (ra & 7)) << 4));
+      const float4 vb = *reinterpret_cast<const float4*>(col + rb * 128 + ((chunk ^ (rb & 7)) << 4));
+      uint32_t hi[2][4], lo[2][4];
+      split_tf32(va.x, hi[0][0], lo[0][0]);
+      split_tf32(va.y, hi[0][1], lo[0][1]);
+      split_tf32(vb.x, hi[0][2], lo[0][2]);
+      split_tf32(vb.y, hi[0][3], lo[0][3]);
+      split_tf32(va.z, hi[1][0], lo[1][0]);
+      split_tf32(va.w, hi[1][1], lo[1][1]);
+      split_tf32(vb.z, hi[1][2], lo[1][2]);
+      split_tf32(vb.w, hi[1][3], lo[1][3]);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_1688_f32(part[nt][0], low[nt][0], hi[0], lo[0], pb[nt][2 * h], pb[nt][2 * h + 1]);
+        mma_1688_f32(part[nt][1], low[nt][1], hi[1], lo[1], pb[nt][2 * h], pb[nt][2 * h + 1]);
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[nt][2 * i][k] += part[nt][0][k] + low[nt][0][k];
+        o[nt][2 * i + 1][k] += part[nt][1][k] + low[nt][1][k];
+      }
+  }
+}
+
+// 4-bit: code and scale are this thread's places in key row perm(g); dims t * D/4 ..
+// in the order of the code bytes.
+template <int D, int NT, int QS>
+__device__ __forceinline__ void qk_fp4(float (&sc)[NT][4], const uint8_t* code, const uint8_t* scale,
+                                       const uint32_t (&qf)[NT][D / 16][2 * QS]) {
+  uint32_t w0[D / 32], w1[D / 32], s0[D / 64], s1[D / 64];
+  if constexpr (D == 128) {
+    const uint4 c0 = *reinterpret_cast<const uint4*>(code), c1 = *reinterpret_cast<const uint4*>(code + 8 * 64);
+    w0[0] = c0.x, w0[1] = c0.y, w0[2] = c0.z, w0[3] = c0.w;
+    w1[0] = c1.x, w1[1] = c1.y, w1[2] = c1.z, w1[3] = c1.w;
+    const uint32_t e0 = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(scale));
+    const uint32_t e1 = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(scale + 8 * 8));
+    s0[0] = __byte_perm(e0, e0, 0x1010), s0[1] = __byte_perm(e0, e0, 0x3232);
+    s1[0] = __byte_perm(e1, e1, 0x1010), s1[1] = __byte_perm(e1, e1, 0x3232);
+  } else {
+    const uint2 c0 = *reinterpret_cast<const uint2*>(code), c1 = *reinterpret_cast<const uint2*>(code + 8 * 32);
+    w0[0] = c0.x, w0[1] = c0.y;
+    w1[0] = c1.x, w1[1] = c1.y;
+    const uint32_t e = e4m3x2_to_half2(static_cast<uint32_t>(scale[0]) | (static_cast<uint32_t>(scale[8 * 4]) << 8));
+    s0[0] = __byte_perm(e, e, 0x1010);
+    s1[0] = __byte_perm(e, e, 0x3232);
+  }
+  float part[NT][2][4];  // two chains
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) part[nt][0][k] = part[nt][1][k] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {  // a code word: two MMAs
+    const uint32_t x0 = s0[i / 2], x1 = s1[i / 2];
+    const uint32_t a00 = mul_half2(e2m1x2_to_half2<0>(w0[i]), x0), a01 = mul_half2(e2m1x2_to_half2<1>(w0[i]), x0);
+    const uint32_t a02 = mul_half2(e2m1x2_to_half2<2>(w0[i]), x0), a03 = mul_half2(e2m1x2_to_half2<3>(w0[i]), x0);
+    const uint32_t a10 = mul_half2(e2m1x2_to_half2<0>(w1[i]), x1), a11 = mul_half2(e2m1x2_to_half2<1>(w1[i]), x1);
+    const uint32_t a12 = mul_half2(e2m1x2_to_half2<2>(w1[i]), x1), a13 = mul_half2(e2m1x2_to_half2<3>(w1[i]), x1);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = QS - 1; k >= 0; --k) {
+        mma_16816<__half>(part[nt][0], a00, a10, a01, a11, qf[nt][2 * i][2 * k], qf[nt][2 * i][2 * k + 1]);
+        mma_16816<__half>(part[nt][1], a02, a12, a03, a13, qf[nt][2 * i + 1][2 * k], qf[nt][2 * i + 1][2 * k + 1]);
+      }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sc[nt][k] = part[nt][0][k] + part[nt][1][k];
+}
+// V: code and scale places in the rows of the keys 2t (0) and 2t + 1 (1), dims g * D/8
+// ..; bits of `gone`: keys 2t, 2t + 1, 2t + 8, 2t + 9 that count as zero.
+template <int D, int NT, int QS>
+__device__ __forceinline__ void pv_fp4(float (&o)[NT][D / 16][4], const float (&p)[NT][4], const uint8_t* code0,
+                                       const uint8_t* code1, const uint8_t* scale0, const uint8_t* scale1, uint32_t gone) {
+  uint32_t pb[NT][2 * QS];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    pb[nt][0] = movmatrix_trans(pack16<__half>(p[nt][0], p[nt][1]));
+    pb[nt][1] = movmatrix_trans(pack16<__half>(p[nt][2], p[nt][3]));
+    if constexpr (QS == 2) {
+      auto rest = [](float x) { return x - __half2float(__float2half_rn(x)); };
+      pb[nt][2] = movmatrix_trans(pack16<__half>(rest(p[nt][0]), rest(p[nt][1])));
+      pb[nt][3] = movmatrix_trans(pack16<__half>(rest(p[nt][2]), rest(p[nt][3])));
+    }
+  }
+  uint32_t c[4][D / 64], sb[4];
+  const uint8_t* code[4] = {code0, code1, code0 + 8 * (D / 2), code1 + 8 * (D / 2)};
+  const uint8_t* scale[4] = {scale0, scale1, scale0 + 8 * (D / 16), scale1 + 8 * (D / 16)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (D == 128) {
+      const uint2 v = *reinterpret_cast<const uint2*>(code[k]);
+      c[k][0] = v.x;
+      c[k][1] = v.y;
+    } else {
+      c[k][0] = *reinterpret_cast<const uint32_t*>(code[k]);
+    }
+    sb[k] = *scale[k];
+  }
+  if (gone) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (gone >> k & 1u) sb[k] = 0u;
+  }
+  const uint32_t s01 = e4m3x2_to_half2(sb[0] | (sb[1] << 8)), s23 = e4m3x2_to_half2(sb[2] | (sb[3] << 8));
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    // nibble pairs (key 2t, key 2t + 1) of the even and of the odd dims
+    const uint32_t ev0 = (c[0][i] & 0x0F0F0F0Fu) | ((c[1][i] << 4) & 0xF0F0F0F0u);
+    const uint32_t od0 = ((c[0][i] >> 4) & 0x0F0F0F0Fu) | (c[1][i] & 0xF0F0F0F0u);
+    const uint32_t ev1 = (c[2][i] & 0x0F0F0F0Fu) | ((c[3][i] << 4) & 0xF0F0F0F0u);
+    const uint32_t od1 = ((c[2][i] >> 4) & 0x0F0F0F0Fu) | (c[3][i] & 0xF0F0F0F0u);
+    auto tile = [&](auto byte) {
+      constexpr int B = decltype(byte)::value;
+      const uint32_t f0 = mul_half2(e2m1x2_to_half2<B>(ev0), s01), f1 = mul_half2(e2m1x2_to_half2<B>(od0), s01);
+      const uint32_t f2 = mul_half2(e2m1x2_to_half2<B>(ev1), s23), f3 = mul_half2(e2m1x2_to_half2<B>(od1), s23);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float(&acc)[4] = o[nt][4 * i + B];
+        if constexpr (QS == 2) {
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_16816<__half>(part, f0, f1, f2, f3, pb[nt][2], pb[nt][3]);
+          mma_16816<__half>(part, f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] += part[k];
+        } else {
+          mma_16816<__half>(acc, f0, f1, f2, f3, pb[nt][0], pb[nt][1]);
+        }
+      }
+    };
+    tile(std::integral_constant<int, 0>{});
+    tile(std::integral_constant<int, 1>{});
+    tile(std::integral_constant<int, 2>{});
+    tile(std::integral_constant<int, 3>{});
+  }
+}
+
 template <typename T, typename KV, int D, int NT>
 __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLayout<T, KV, D, NT>::kCtas)
     attn_paged_decode_kernel(const DecodeArgs d, const __grid_constant__ CUtensorMap tk,
-                             const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tks,
-                             const __grid_constant__ CUtensorMap tvs) {
+                             const __grid_constant__ CUtensorMap tv) {
   using L = DecodeLayout<T, KV, D, NT>;
   using MT = typename std::conditional<L::kFp4, __half, T>::type;  // MMA operand type of 16-bit MMAs
   constexpr bool kF32 = L::kF32;
   constexpr int QS = L::kFp4 && std::is_same<T, float>::value ? 2 : 1;  // halves that make up a q or p
-  constexpr int BN = L::BN, R = L::R, E = L::kEntries, W = L::W;
+  constexpr int BN = L::BN, R = L::R, E = L::kEntries, W = L::W, SUB = L::SUB;
   extern __shared__ uint8_t smem_base[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_base) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -266,9 +510,8 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
   pdl_trigger();
   Walker<BN, R> walk(d, lane);
   Segment seg;
-  // scale bytes of row r: r * D/16 + (r / 16) * scale_pad
-  const int scale_pad = L::kFp4 && D == 64 && a.seqs.page_shift == 4 ? 64 : 0;
-
+  // 4-bit pages: a (page, head) block is copied as it is, codes then scales
+  const int block_rows = 1 << a.seqs.page_shift, block_bytes = block_rows * D * 9 / 16;
   if (warp == W) {
     // ---- producer: page ids (32 at a time, the next 32 already asked for) and TMA boxes
     const int shift = a.seqs.page_shift, page_rows = 1 << shift;
@@ -311,14 +554,23 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
             break;
           }
           uint8_t* dst = smem + e * L::kEntry;
-          if (lane == 0) mbar_arrive_expect_tx(&full[e], L::kEntryTx);
-          __syncwarp();
-          if (lane < boxes) {
-            const CUtensorMap* map = which ? &tv : &tk;
-            if constexpr (L::kFp4) {
-              tma_load_4d(dst + box_at * (D / 2), map, 0, row, seg.kvh, page, &full[e]);
-              tma_load_4d(dst + L::kCodes + box_at * (D / 16) + lane * scale_pad, which ? &tvs : &tks, 0, 0, seg.kvh, page, &full[e]);
-            } else {
+          if constexpr (L::kFp4) {
+            const bool copy = lane < boxes && page != none;
+            uint8_t* block = dst + lane * block_bytes;
+            if (lane < boxes && page == none && first + lane <= last_page)  // a bad page
+              for (int i = 0; i < block_bytes; i += 16) *reinterpret_cast<uint4*>(block + i) = make_uint4(0u, 0u, 0u, 0u);
+            const int copies = __popc(__ballot_sync(0xffffffffu, copy));
+            if (lane == 0) mbar_arrive_expect_tx(&full[e], static_cast<uint32_t>(copies * block_bytes));
+            __syncwarp();
+            if (copy)
+              bulk_load(block, static_cast<const uint8_t*>(which ? a.v_pages : a.k_pages) +
+                                   (static_cast<int64_t>(page) * a.hkv + seg.kvh) * block_bytes,
+                        static_cast<uint32_t>(block_bytes), &full[e]);
+          } else {
+            if (lane == 0) mbar_arrive_expect_tx(&full[e], L::kEntry);
+            __syncwarp();
+            if (lane < boxes) {
+              const CUtensorMap* map = which ? &tv : &tk;
               constexpr int kBoxWidth = kF32 ? 128 : 64;  // in the map's units: bytes or 16-bit elements
 #pragma unroll
               for (int c = 0; c < L::kRowBytes / 128; ++c)
@@ -341,6 +593,7 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
   float* wl = wm + W * R;
   // MMA key row x of a 16-key group holds key perm(x): the fragment reads of 4-bit V
   // and of float32 K and V then fall into different banks
+  // (4-bit at D 128: two of the four keys still share banks)
   auto perm = [](int x) {
     if (L::kFp4 && D == 128) return x ^ ((x >> 1) & 1);
     return L::kFp4 || kF32 ? (x & 8) | ((x & 6) >> 1) | ((x & 1) << 2) : x;
@@ -349,7 +602,18 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
   const float base_scale = a.softcap > 0.f ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
   int at = 0;  // ring entries consumed
   bool alive = true;
-  const int kw = warp * 16;  // this warp's keys of every block
+  const int kw = warp * 16;  // this warp's keys of every block (and of each further 16 W)
+  // 4-bit pages: places of the warp's 16-key groups in an entry, and this thread's in a group
+  int code_off[SUB], scale_off[SUB];
+#pragma unroll
+  for (int u = 0; u < SUB; ++u) {
+    const int r = kw + u * 16 * W, at_block = (r >> a.seqs.page_shift) * block_bytes;
+    code_off[u] = at_block + (r & (block_rows - 1)) * (D / 2);
+    scale_off[u] = at_block + block_rows * (D / 2) + (r & (block_rows - 1)) * (D / 16);
+  }
+  const int kcode = perm(g) * (D / 2) + t * (D / 8), kscale = perm(g) * (D / 16) + t * (D / 64);
+  const int vcode0 = perm(2 * t) * (D / 2) + g * (D / 16), vcode1 = perm(2 * t + 1) * (D / 2) + g * (D / 16);
+  const int vscale0 = perm(2 * t) * (D / 16) + g * (D / 8) / 16, vscale1 = perm(2 * t + 1) * (D / 16) + g * (D / 8) / 16;
 
   while (walk.get(seg)) {
     const int rows_left = seg.w.rows.n * a.group - seg.rt * R;
@@ -426,9 +690,11 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
       }
     }
     float o[NT][KK][4];
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2], mul[NT][2];  // mul: what turns a masked score into log2 units
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      mul[nt][0] = a.softcap > 0.f || a.slopes ? 1.f : rscale[nt][0];
+      mul[nt][1] = a.softcap > 0.f || a.slopes ? 1.f : rscale[nt][1];
 #pragma unroll
       for (int i = 0; i < KK; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
       m[nt][0] = m[nt][1] = -INFINITY;
@@ -455,293 +721,117 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
       const uint8_t* sk = smem + (at % E) * L::kEntry;
       const int blk_key = (seg.block + j) * BN;
 
-      // S^T = K Q^T
-      float sc[1][NT][4];
-      {
-        constexpr int u = 0;
+      float sc[SUB][NT][4];  // S^T: key rows g, g + 8 of the group, query rows 2t, 2t + 1
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[u][nt][0] = sc[u][nt][1] = sc[u][nt][2] = sc[u][nt][3] = 0.f;
-        if constexpr (L::kFp4) {
-          const int r0 = kw + perm(g), r1 = kw + perm(g + 8);
-          const uint8_t* ss = sk + L::kCodes;
-          uint32_t w0[D / 32], w1[D / 32], s0[D / 64], s1[D / 64];
-          if constexpr (D == 128) {
-            const uint4 c0 = *reinterpret_cast<const uint4*>(sk + r0 * 64 + ((t ^ ((r0 >> 1) & 3)) << 4));
-            const uint4 c1 = *reinterpret_cast<const uint4*>(sk + r1 * 64 + ((t ^ ((r1 >> 1) & 3)) << 4));
-            w0[0] = c0.x, w0[1] = c0.y, w0[2] = c0.z, w0[3] = c0.w;
-            w1[0] = c1.x, w1[1] = c1.y, w1[2] = c1.z, w1[3] = c1.w;
-            const uint32_t e0 = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(ss + r0 * 8 + 2 * t));
-            const uint32_t e1 = e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(ss + r1 * 8 + 2 * t));
-            s0[0] = __byte_perm(e0, e0, 0x1010), s0[1] = __byte_perm(e0, e0, 0x3232);
-            s1[0] = __byte_perm(e1, e1, 0x1010), s1[1] = __byte_perm(e1, e1, 0x3232);
-          } else {
-            const uint2 c0 = *reinterpret_cast<const uint2*>(sk + r0 * 32 + t * 8);
-            const uint2 c1 = *reinterpret_cast<const uint2*>(sk + r1 * 32 + t * 8);
-            w0[0] = c0.x, w0[1] = c0.y;
-            w1[0] = c1.x, w1[1] = c1.y;
-            const uint32_t e =
-                e4m3x2_to_half2(static_cast<uint32_t>(ss[r0 * 4 + (r0 >> 4) * scale_pad + t]) |
-                                (static_cast<uint32_t>(ss[r1 * 4 + (r1 >> 4) * scale_pad + t]) << 8));
-            s0[0] = __byte_perm(e, e, 0x1010);
-            s1[0] = __byte_perm(e, e, 0x3232);
-          }
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {  // a code word: two MMAs
-            const uint32_t x0 = s0[i / 2], x1 = s1[i / 2];
-            const uint32_t a00 = mul_half2(e2m1x2_to_half2<0>(w0[i]), x0), a01 = mul_half2(e2m1x2_to_half2<1>(w0[i]), x0);
-            const uint32_t a02 = mul_half2(e2m1x2_to_half2<2>(w0[i]), x0), a03 = mul_half2(e2m1x2_to_half2<3>(w0[i]), x0);
-            const uint32_t a10 = mul_half2(e2m1x2_to_half2<0>(w1[i]), x1), a11 = mul_half2(e2m1x2_to_half2<1>(w1[i]), x1);
-            const uint32_t a12 = mul_half2(e2m1x2_to_half2<2>(w1[i]), x1), a13 = mul_half2(e2m1x2_to_half2<3>(w1[i]), x1);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_16816<MT>(sc[u][nt], a00, a10, a01, a11, qf[nt][2 * i][0], qf[nt][2 * i][1]);
-              mma_16816<MT>(sc[u][nt], a02, a12, a03, a13, qf[nt][2 * i + 1][0], qf[nt][2 * i + 1][1]);
-              if constexpr (QS == 2) {
-                mma_16816<MT>(sc[u][nt], a00, a10, a01, a11, qf[nt][2 * i][2], qf[nt][2 * i][3]);
-                mma_16816<MT>(sc[u][nt], a02, a12, a03, a13, qf[nt][2 * i + 1][2], qf[nt][2 * i + 1][3]);
-              }
-            }
-          }
-        } else if constexpr (kF32) {
-          const int r0 = kw + perm(g), r1 = kw + perm(g + 8);
-          float part[NT][4][4], low[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) low[nt][i] = part[nt][0][i] = part[nt][1][i] = part[nt][2][i] = part[nt][3][i] = 0.f;
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            const uint8_t* box = sk + (kk >> 1) * L::kBox;
-            const int ch = (kk & 1) * 4 + t;
-            const float4 k0 = *reinterpret_cast<const float4*>(box + r0 * 128 + ((ch ^ (r0 & 7)) << 4));
-            const float4 k1 = *reinterpret_cast<const float4*>(box + r1 * 128 + ((ch ^ (r1 & 7)) << 4));
-            uint32_t h[2][4], l2[2][4];
-            split_tf32(k0.x, h[0][0], l2[0][0]);
-            split_tf32(k1.x, h[0][1], l2[0][1]);
-            split_tf32(k0.y, h[0][2], l2[0][2]);
-            split_tf32(k1.y, h[0][3], l2[0][3]);
-            split_tf32(k0.z, h[1][0], l2[1][0]);
-            split_tf32(k1.z, h[1][1], l2[1][1]);
-            split_tf32(k0.w, h[1][2], l2[1][2]);
-            split_tf32(k1.w, h[1][3], l2[1][3]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float(&acc)[4] = part[nt][kk & 3];
-              mma_1688_f32(acc, low[nt], h[0], l2[0], __uint_as_float(qf[nt][kk][0]), __uint_as_float(qf[nt][kk][1]));
-              mma_1688_f32(acc, low[nt], h[1], l2[1], __uint_as_float(qf[nt][kk][2]), __uint_as_float(qf[nt][kk][3]));
-            }
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              sc[u][nt][i] = low[nt][i] + ((part[nt][0][i] + part[nt][1][i]) + (part[nt][2][i] + part[nt][3][i]));
-        } else {
-          const uint32_t ks = smem_u32(sk);
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            uint32_t f[4];
-            ldmatrix_x4(f, ks + swz128(L::kBox, kw + (lane & 15), kk * 16 + (lane >> 4) * 8));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816<MT>(sc[u][nt], f[0], f[1], f[2], f[3], qf[nt][kk][0], qf[nt][kk][1]);
-          }
-        }
+      for (int u = 0; u < SUB; ++u) {
+        if constexpr (L::kFp4) qk_fp4<D, NT, QS>(sc[u], sk + code_off[u] + kcode, sk + scale_off[u] + kscale, qf);
+        else if constexpr (kF32) qk_f32<D, NT>(sc[u], sk, L::kBox, kw + u * 16 * W, g, t, qf);
+        else qk_16<T, D, NT>(sc[u], smem_u32(sk), L::kBox, kw + u * 16 * W, lane, qf);
       }
-
       release();
 
-      // scores in log2 units, cap, bias and mask
-      float mx[NT][2];
+      // cap and bias (into log2 units), mask
+      if (a.softcap > 0.f || a.slopes) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
-      const bool edge = blk_key + BN > seg.w.rows.past + 1 || blk_key < seg.w.kv_len - a.window;
+        for (int u = 0; u < SUB; ++u)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            constexpr int u = 0;
-            const int e = i & 1;
-            const int key = blk_key + kw + perm(g + (i >> 1) * 8);
-            float x = sc[u][nt][i] * rscale[nt][e];
-            if (a.softcap > 0.f) x = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(x));
-            if (a.slopes) x = fmaf(slope[nt][e], static_cast<float>(key - pos[nt][e]), x);
-            if (edge && (key > pos[nt][e] || key <= pos[nt][e] - a.window)) x = -INFINITY;
-            sc[u][nt][i] = x;
-            mx[nt][e] = fmaxf(mx[nt][e], x);
-          }
+            for (int i = 0; i < 4; ++i) {
+              float x = sc[u][nt][i] * rscale[nt][i & 1];
+              if (a.softcap > 0.f) x = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(x));
+              const int key = blk_key + u * 16 * W + kw + perm(g + (i >> 1) * 8);
+              sc[u][nt][i] = fmaf(slope[nt][i & 1], static_cast<float>(key - pos[nt][i & 1]), x);
+            }
+      }
+      if (blk_key + BN > seg.w.rows.past + 1 || blk_key < seg.w.kv_len - a.window) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = blk_key + u * 16 * W + kw + perm(g + (i >> 1) * 8), at_pos = pos[nt][i & 1];
+              if (key > at_pos || key <= at_pos - a.window) sc[u][nt][i] = -INFINITY;
+            }
+      }
+      // running maximum; O and the sums are rescaled when it moves
+      float top[NT][2];
       bool moved = false;
-      float alpha[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
 #pragma unroll
-          for (int s = 4; s < 32; s <<= 1) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], s));
-          const float top = fmaxf(m[nt][e], mx[nt][e]);
-          alpha[nt][e] = m[nt][e] == top ? 1.f : exp2_approx(m[nt][e] - top);  // m = -inf: 0
-          moved |= m[nt][e] != top;
-          m[nt][e] = top;
+          for (int u = 1; u < SUB; ++u) x = fmaxf(x, fmaxf(sc[u][nt][e], sc[u][nt][e + 2]));
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
+          top[nt][e] = fmaxf(m[nt][e], x * mul[nt][e]);
+          moved |= top[nt][e] != m[nt][e];
         }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          l[nt][0] *= alpha[nt][0];
-          l[nt][1] *= alpha[nt][1];
+          float alpha[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            alpha[e] = m[nt][e] == top[nt][e] ? 1.f : exp2_approx(m[nt][e] - top[nt][e]);  // from -inf: 0
+            m[nt][e] = top[nt][e];
+            l[nt][e] *= alpha[e];
+          }
 #pragma unroll
           for (int i = 0; i < KK; ++i) {
-            o[nt][i][0] *= alpha[nt][0];
-            o[nt][i][1] *= alpha[nt][1];
-            o[nt][i][2] *= alpha[nt][0];
-            o[nt][i][3] *= alpha[nt][1];
+            o[nt][i][0] *= alpha[0];
+            o[nt][i][1] *= alpha[1];
+            o[nt][i][2] *= alpha[0];
+            o[nt][i][3] *= alpha[1];
           }
         }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // a row that has seen no key yet keeps m = -inf: its p are 0
+          const float neg = m[nt][e] == -INFINITY ? 0.f : -m[nt][e];
+#pragma unroll
+          for (int u = 0; u < SUB; ++u) {
+            sc[u][nt][e] = exp2_approx(fmaf(sc[u][nt][e], mul[nt][e], neg));
+            sc[u][nt][e + 2] = exp2_approx(fmaf(sc[u][nt][e + 2], mul[nt][e], neg));
+            l[nt][e] += sc[u][nt][e] + sc[u][nt][e + 2];  // this thread's keys; summed over the warp at the end
+          }
+        }
 
       // O^T += V^T P^T
       if (!arrived()) continue;
       uint8_t* sv = smem + (at % E) * L::kEntry;
-      {
-        constexpr int u = 0;
-        uint32_t pb[NT][kF32 ? 4 : 2 * QS];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          // a row that has seen no key yet keeps m = -inf: its p are 0
-          const float n0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], n1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-          const float p00 = exp2_approx(sc[u][nt][0] - n0), p01 = exp2_approx(sc[u][nt][1] - n1);
-          const float p10 = exp2_approx(sc[u][nt][2] - n0), p11 = exp2_approx(sc[u][nt][3] - n1);
-          l[nt][0] += p00 + p10;  // this thread's keys; summed over the warp at the end
-          l[nt][1] += p01 + p11;
-          if constexpr (kF32) {
-            // P^T as the B operand: lane (g, t) gets rows g of the keys 2t, 2t + 1 (+ 8)
-            const int s0 = 8 * t + (g >> 1), s1 = s0 + 4;
-            const float x0 = __shfl_sync(0xffffffffu, p00, s0), y0 = __shfl_sync(0xffffffffu, p01, s0);
-            const float x1 = __shfl_sync(0xffffffffu, p00, s1), y1 = __shfl_sync(0xffffffffu, p01, s1);
-            const float x2 = __shfl_sync(0xffffffffu, p10, s0), y2 = __shfl_sync(0xffffffffu, p11, s0);
-            const float x3 = __shfl_sync(0xffffffffu, p10, s1), y3 = __shfl_sync(0xffffffffu, p11, s1);
-            pb[nt][0] = __float_as_uint((g & 1) ? y0 : x0);
-            pb[nt][1] = __float_as_uint((g & 1) ? y1 : x1);
-            pb[nt][2] = __float_as_uint((g & 1) ? y2 : x2);
-            pb[nt][3] = __float_as_uint((g & 1) ? y3 : x3);
-          } else {
-            pb[nt][0] = movmatrix_trans(pack16<MT>(p00, p01));
-            pb[nt][1] = movmatrix_trans(pack16<MT>(p10, p11));
-            if constexpr (QS == 2) {
-              auto rest = [](float p) { return p - __half2float(__float2half_rn(p)); };
-              pb[nt][2] = movmatrix_trans(pack16<MT>(rest(p00), rest(p01)));
-              pb[nt][3] = movmatrix_trans(pack16<MT>(rest(p10), rest(p11)));
-            }
-          }
-        }
-        const int key_first = blk_key + kw;
+      for (int u = 0; u < SUB; ++u) {
+        const int key_first = blk_key + u * 16 * W + kw;
+        // rows that are not of the sequence may hold anything: a zero weight must meet a zero
         const bool stale = key_first + 16 > seg.w.kv_len || key_first < seg.w.key_lo;
+        auto foreign = [&](int r) { return key_first + r >= seg.w.kv_len || key_first + r < seg.w.key_lo; };
         if constexpr (L::kFp4) {
-          const uint8_t* ss = sv + L::kCodes;
-          const int rw[4] = {kw + perm(2 * t), kw + perm(2 * t + 1), kw + perm(2 * t + 8), kw + perm(2 * t + 9)};
-          uint32_t c[4][D / 64], sb[4];
+          uint32_t gone = 0u;  // of the keys 2t, 2t + 1, 2t + 8, 2t + 9
+          if (stale) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (D == 128) {
-              const uint2 v = *reinterpret_cast<const uint2*>(sv + rw[k] * 64 + (((g >> 1) ^ ((rw[k] >> 1) & 3)) << 4) + (g & 1) * 8);
-              c[k][0] = v.x;
-              c[k][1] = v.y;
-              sb[k] = ss[rw[k] * 8 + g];
-            } else {
-              c[k][0] = *reinterpret_cast<const uint32_t*>(sv + rw[k] * 32 + g * 4);
-              sb[k] = ss[rw[k] * 4 + (rw[k] >> 4) * scale_pad + (g >> 1)];
-            }
-            // a row that is not of the sequence may hold a NaN scale
-            if (stale && (blk_key + rw[k] >= seg.w.kv_len || blk_key + rw[k] < seg.w.key_lo)) sb[k] = 0u;
+            for (int k = 0; k < 4; ++k) gone |= static_cast<uint32_t>(foreign(perm(2 * t + (k & 1) + (k >> 1) * 8))) << k;
           }
-          const uint32_t s01 = e4m3x2_to_half2(sb[0] | (sb[1] << 8)), s23 = e4m3x2_to_half2(sb[2] | (sb[3] << 8));
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i) {
-            // nibble pairs (key 2t, key 2t+1) of the even and of the odd dims
-            const uint32_t ev0 = (c[0][i] & 0x0F0F0F0Fu) | ((c[1][i] << 4) & 0xF0F0F0F0u);
-            const uint32_t od0 = ((c[0][i] >> 4) & 0x0F0F0F0Fu) | (c[1][i] & 0xF0F0F0F0u);
-            const uint32_t ev1 = (c[2][i] & 0x0F0F0F0Fu) | ((c[3][i] << 4) & 0xF0F0F0F0u);
-            const uint32_t od1 = ((c[2][i] >> 4) & 0x0F0F0F0Fu) | (c[3][i] & 0xF0F0F0F0u);
-#define DLI_FP4_V(B)                                                                                                 \
-  {                                                                                                                  \
-    const uint32_t f0 = mul_half2(e2m1x2_to_half2<B>(ev0), s01), f1 = mul_half2(e2m1x2_to_half2<B>(od0), s01);      \
-    const uint32_t f2 = mul_half2(e2m1x2_to_half2<B>(ev1), s23), f3 = mul_half2(e2m1x2_to_half2<B>(od1), s23);      \
-    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) {                                                              \
-      if constexpr (QS == 2) {                                                                                       \
-        float part[4] = {0.f, 0.f, 0.f, 0.f};                                                                        \
-        mma_16816<MT>(part, f0, f1, f2, f3, pb[nt][2 * QS - 2], pb[nt][2 * QS - 1]);                                 \
-        mma_16816<MT>(part, f0, f1, f2, f3, pb[nt][0], pb[nt][1]);                                                   \
-        _Pragma("unroll") for (int k = 0; k < 4; ++k) o[nt][4 * i + B][k] += part[k];                                \
-      } else {                                                                                                       \
-        mma_16816<MT>(o[nt][4 * i + B], f0, f1, f2, f3, pb[nt][0], pb[nt][1]);                                       \
-      }                                                                                                              \
-    }                                                                                                                \
-  }
-            DLI_FP4_V(0)
-            DLI_FP4_V(1)
-            DLI_FP4_V(2)
-            DLI_FP4_V(3)
-#undef DLI_FP4_V
-          }
+          pv_fp4<D, NT, QS>(o, sc[u], sv + code_off[u] + vcode0, sv + code_off[u] + vcode1, sv + scale_off[u] + vscale0,
+                            sv + scale_off[u] + vscale1, gone);
         } else {
           if (stale) {
-            // V rows that are not of the sequence may hold anything: a zero weight must meet a zero
             for (int c = lane; c < 16 * (L::kRowBytes / 16); c += 32) {
               const int r = (c >> 3) & 15, box = c >> 7;
-              if (key_first + r >= seg.w.kv_len || key_first + r < seg.w.key_lo)
-                *reinterpret_cast<uint4*>(sv + box * L::kBox + (kw + r) * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+              if (foreign(r))
+                *reinterpret_cast<uint4*>(sv + box * L::kBox + (kw + u * 16 * W + r) * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
             fence_proxy_async_smem();  // before the entry is given back to the TMA
             __syncwarp();
           }
-          if constexpr (kF32) {
-            // lane (g, t): 4 dims 4 * chunk of each 32, of the keys 2t and 2t + 1 of each 8
-            const int chunk = ((g & 1) << 2) | (g >> 1);
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-              const uint8_t* box = sv + i * L::kBox;
-              float part[NT][2][4], low[NT][2][4];
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) part[nt][0][k] = part[nt][1][k] = low[nt][0][k] = low[nt][1][k] = 0.f;
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int ra = kw + h * 8 + t, rb = ra + 4;
-                const float4 va = *reinterpret_cast<const float4*>(box + ra * 128 + ((chunk ^ (ra & 7)) << 4));
-                const float4 vb = *reinterpret_cast<const float4*>(box + rb * 128 + ((chunk ^ (rb & 7)) << 4));
-                uint32_t hi[2][4], lo[2][4];
-                split_tf32(va.x, hi[0][0], lo[0][0]);
-                split_tf32(va.y, hi[0][1], lo[0][1]);
-                split_tf32(vb.x, hi[0][2], lo[0][2]);
-                split_tf32(vb.y, hi[0][3], lo[0][3]);
-                split_tf32(va.z, hi[1][0], lo[1][0]);
-                split_tf32(va.w, hi[1][1], lo[1][1]);
-                split_tf32(vb.z, hi[1][2], lo[1][2]);
-                split_tf32(vb.w, hi[1][3], lo[1][3]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  const float b0 = __uint_as_float(pb[nt][2 * h]), b1 = __uint_as_float(pb[nt][2 * h + 1]);
-                  mma_1688_f32(part[nt][0], low[nt][0], hi[0], lo[0], b0, b1);
-                  mma_1688_f32(part[nt][1], low[nt][1], hi[1], lo[1], b0, b1);
-                }
-              }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  o[nt][2 * i][k] += part[nt][0][k] + low[nt][0][k];
-                  o[nt][2 * i + 1][k] += part[nt][1][k] + low[nt][1][k];
-                }
-            }
-          } else {
-          const uint32_t vs = smem_u32(sv);
-#pragma unroll
-          for (int i = 0; i < KK; ++i) {
-            uint32_t f[4];
-            ldmatrix_x4_trans(f, vs + swz128(L::kBox, kw + (lane & 7) + (lane >> 4) * 8, i * 16 + ((lane >> 3) & 1) * 8));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_16816<MT>(o[nt][i], f[0], f[1], f[2], f[3], pb[nt][0], pb[nt][1]);
-          }
-          }
+          if constexpr (kF32) pv_f32<D, NT>(o, sc[u], sv, L::kBox, kw + u * 16 * W, g, t);
+          else pv_16<T, D, NT>(o, sc[u], smem_u32(sv), L::kBox, kw + u * 16 * W, lane);
         }
       }
       release();
@@ -780,7 +870,7 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
           for (int k = 0; k < 4; ++k) {
             // 16-bit: dims i * 16 + g (+ 8); 4-bit: g * D/8 + 2 i (+ 1); float32: see the reads of V
             const int dim = L::kFp4 ? g * (D / 8) + 2 * i + (k >> 1)
-                            : kF32  ? 32 * (i >> 1) + 4 * (((g & 1) << 2) | (g >> 1)) + 2 * (i & 1) + (k >> 1)
+                            : kF32  ? 32 * (i >> 1) + 4 * f32_chunk(g) + 2 * (i & 1) + (k >> 1)
                                     : i * 16 + g + (k >> 1) * 8;
             if (D == DH || dim / DH == half)
               merge[(warp * R + nt * 8 + 2 * t + (k & 1)) * DH + (dim - half * DH)] = o[nt][i][k] * f[k & 1];
@@ -975,13 +1065,12 @@ DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t 
 template <typename T, typename KV, int D, int NT>
 dli_status launch_paged_decode(const PagedAttnArgs& a, const DecodePlan& plan, void* workspace, cudaStream_t stream) {
   using L = DecodeLayout<T, KV, D, NT>;
-  CUtensorMap tk, tv, tks, tvs;
+  CUtensorMap tk{}, tv{};  // not used for 4-bit pages
   const int64_t page_rows = 1ll << a.seqs.page_shift;
-  const dli_dtype kv_dtype = L::kFp4                                   ? DLI_DTYPE_FP4
-                             : L::kF32                                 ? DLI_DTYPE_F32
+  const dli_dtype kv_dtype = L::kF32                                 ? DLI_DTYPE_F32
                              : std::is_same<T, __nv_bfloat16>::value ? DLI_DTYPE_BF16
                                                                        : DLI_DTYPE_F16;
-  dli_status st = make_page_maps(a, kv_dtype, D, static_cast<int>(std::min<int64_t>(page_rows, L::BN)), &tk, &tv, &tks, &tvs);
+  dli_status st = L::kFp4 ? DLI_OK : make_page_maps(a, kv_dtype, D, static_cast<int>(std::min<int64_t>(page_rows, L::BN)), &tk, &tv);
   if (st != DLI_OK) return st;
   auto kern = attn_paged_decode_kernel<T, KV, D, NT>;
   st = ensure_smem(reinterpret_cast<const void*>(kern), L::kBytes, "attention_paged");
@@ -998,7 +1087,7 @@ dli_status launch_paged_decode(const PagedAttnArgs& a, const DecodePlan& plan, v
     grid = std::min<int64_t>(grid, std::max(1, resident_ctas(reinterpret_cast<const void*>(kern), L::kThreads, L::kBytes)));
     d.ctas = static_cast<int>(grid);
   }
-  launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(L::kThreads), L::kBytes, stream, d, tk, tv, tks, tvs);
+  launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(L::kThreads), L::kBytes, stream, d, tk, tv);
   if (plan.split)
     launch_pdl(attn_paged_combine_kernel<T, D, L::BN, L::R>, dim3(static_cast<unsigned>(plan.units), D / 32), dim3(256), 0, stream, d);
   return check_launch("attention_paged", plan.split ? 2 : 1);
@@ -1019,38 +1108,26 @@ int64_t max_keys_of(const PagedAttnArgs& a) {
 
 }  // namespace
 
-// 4-D maps over the pages: [num_pages, Hkv, page rows, D] 16-bit elements or bytes,
-// and the scale bytes of 4-bit pages as 16-byte chunks.
-dli_status make_page_maps(const PagedAttnArgs& a, dli_dtype kv_dtype, int d, int box_rows, CUtensorMap* tk, CUtensorMap* tv,
-                          CUtensorMap* tks, CUtensorMap* tvs) {
+// 4-D maps over the pages: [num_pages, Hkv, page rows, D] 16-bit elements, or bytes of
+// float32 elements.
+dli_status make_page_maps(const PagedAttnArgs& a, dli_dtype dtype, int d, int box_rows, CUtensorMap* tk, CUtensorMap* tv) {
   const uint64_t page_rows = 1ull << a.seqs.page_shift, hkv = static_cast<uint64_t>(a.hkv);
   const uint64_t pages = static_cast<uint64_t>(a.seqs.num_pages), ud = static_cast<uint64_t>(d);
   const uint32_t rows = static_cast<uint32_t>(box_rows);
   const void* base[2] = {a.k_pages, a.v_pages};
   CUtensorMap* map[2] = {tk, tv};
-  CUtensorMap* scale[2] = {tks, tvs};
+  const uint64_t es = dtype_bytes(dtype);
+  const uint64_t strides[3] = {ud * es, page_rows * ud * es, hkv * page_rows * ud * es};
   for (int i = 0; i < 2; ++i) {
-    dli_status st = DLI_OK;
-    if (kv_dtype == DLI_DTYPE_FP4) {
-      const uint64_t block = static_cast<uint64_t>(fp4_block_bytes(static_cast<int64_t>(page_rows), d));
-      const uint64_t dims[4] = {ud / 2, page_rows, hkv, pages}, sdims[4] = {16, page_rows * ud / 256, hkv, pages};
-      const uint64_t strides[3] = {ud / 2, block, hkv * block}, sstrides[3] = {16, block, hkv * block};
-      const uint32_t box[4] = {static_cast<uint32_t>(d / 2), rows, 1u, 1u}, sbox[4] = {16u, rows * d / 256, 1u, 1u};
-      st = make_map_4d_bytes(map[i], base[i], dims, strides, box, d == 128 ? 64 : 0);
-      if (st == DLI_OK)
-        st = make_map_4d_bytes(scale[i], static_cast<const uint8_t*>(base[i]) + page_rows * ud / 2, sdims, sstrides, sbox, 0);
-    } else if (kv_dtype == DLI_DTYPE_F32) {
+    dli_status st;
+    if (dtype == DLI_DTYPE_F32) {
       const uint64_t dims[4] = {ud * 4, page_rows, hkv, pages};
-      const uint64_t strides[3] = {ud * 4, page_rows * ud * 4, hkv * page_rows * ud * 4};
       const uint32_t box[4] = {128u, rows, 1u, 1u};
-      st = make_map_4d_bytes(map[i], base[i], dims, strides, box, 128);
-      *scale[i] = *map[i];
+      st = make_map_4d_bytes(map[i], base[i], dims, strides, box);
     } else {
       const uint64_t dims[4] = {ud, page_rows, hkv, pages};
-      const uint64_t strides[3] = {ud * 2, page_rows * ud * 2, hkv * page_rows * ud * 2};
       const uint32_t box[4] = {64u, rows, 1u, 1u};
-      st = make_map_4d(map[i], base[i], kv_dtype == DLI_DTYPE_BF16, dims, strides, box);
-      *scale[i] = *map[i];
+      st = make_map_4d(map[i], base[i], dtype == DLI_DTYPE_BF16, dims, strides, box);
     }
     if (st != DLI_OK) return st;
   }

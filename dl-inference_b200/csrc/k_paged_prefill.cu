@@ -706,9 +706,9 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
   using L = PrefillLayout<D>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
-  CUtensorMap tq{}, tk{}, tv{}, tks, tvs;  // not used for 4-bit pages
+  CUtensorMap tq{}, tk{}, tv{};  // not used for 4-bit pages
   const int page_rows = 1 << a.seqs.page_shift;
-  dli_status st = kFp4 ? DLI_OK : make_page_maps(a, kBf16 ? DLI_DTYPE_BF16 : DLI_DTYPE_F16, D, std::min(page_rows, BN), &tk, &tv, &tks, &tvs);
+  dli_status st = kFp4 ? DLI_OK : make_page_maps(a, kBf16 ? DLI_DTYPE_BF16 : DLI_DTYPE_F16, D, std::min(page_rows, BN), &tk, &tv);
   if (st != DLI_OK) return st;
   const uint64_t qd[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.hq), static_cast<uint64_t>(a.seqs.tokens), 1ull};
   const uint64_t row_bytes = static_cast<uint64_t>(a.hq) * D * 2;

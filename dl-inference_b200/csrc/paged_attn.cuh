@@ -6,11 +6,9 @@
 
 namespace dli_sm100 {
 
-// Tensor maps over the K and V pages with boxes of box_rows rows x 128 bytes of one
-// (page, head); for 4-bit pages tk/tv cover the code bytes (whole rows) and tks/tvs
-// the scale bytes.
-dli_status make_page_maps(const PagedAttnArgs& a, dli_dtype kv_dtype, int d, int box_rows, CUtensorMap* tk, CUtensorMap* tv,
-                          CUtensorMap* tks, CUtensorMap* tvs);
+// Tensor maps over the K and V pages of the model's type with boxes of box_rows rows x
+// 128 bytes of one (page, head).
+dli_status make_page_maps(const PagedAttnArgs& a, dli_dtype dtype, int d, int box_rows, CUtensorMap* tk, CUtensorMap* tv);
 
 // Few query rows per KV head, and every float32 call (k_paged_decode.cu): head_dim 64
 // or 128, 16-byte aligned tensors.
