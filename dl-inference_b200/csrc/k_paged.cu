@@ -6,7 +6,9 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
+#include "mma_sync.cuh"
 #include "paged_attn.cuh"
 
 namespace dli_sm100 {
@@ -23,53 +25,72 @@ __device__ __forceinline__ float round_to_odd(double x) {
 
 // E4M3 code nearest to most / 6 (ties to the even code, at most 448). `most` is
 // rounded to odd, and six times the midpoint of two neighbouring codes has at
-// most 7 bits, so the comparisons decide as the exact value would.
+// most 7 bits, so the comparison decides as the exact value would.
 __device__ __forceinline__ unsigned e4m3_scale(float most) {
-  unsigned c = __nv_cvt_float_to_fp8(most * (1.f / 6.f), __NV_SATFINITE, __NV_E4M3);
+  const float t = most * (1.f / 6.f);
+  const unsigned c = __nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
   const float v = e4m3_value(c);
-  if (c < 126u) {
-    const float up = 3.f * (v + e4m3_value(c + 1u));
-    if (most > up || (most == up && (c & 1u))) return c + 1u;
-  }
-  if (c > 0u) {
-    const float down = 3.f * (v + e4m3_value(c - 1u));
-    if (most < down || (most == down && (c & 1u))) return c - 1u;
-  }
+  const unsigned up = t > v ? 1u : 0u;  // which neighbour could be nearer
+  if (up ? c >= 126u : c == 0u) return c;
+  const float mid = 3.f * (v + e4m3_value(up ? c + 1u : c - 1u));
+  const bool odd_tie = most == mid && (c & 1u);
+  if (up ? most > mid || odd_tie : most < mid || odd_tie) return up ? c + 1u : c - 1u;
   return c;
 }
 
-// 16 values (rounded to odd where they are not exact) -> scale byte and 8 code
-// bytes. A value's code is the number of rounding borders below it: 0.25, 0.75,
-// ... times the scale, products of 3-bit numbers, hence exact; a border itself
-// goes to the even code.
-__device__ __forceinline__ void fp4_block(const float (&x)[16], unsigned& scale, uint2& codes) {
-  float most = 0.f;
-  bool nan = false;
+// The code word of 8 values (rounded to odd where they are not exact) for scale value
+// s > 0, from its definition: a value's code is the number of rounding borders at or
+// below it: 0.25, 0.75, ... times the scale, products of 3-bit numbers, hence exact; a
+// border itself goes to the even code, so those below an even code count from the next
+// float on.
+__device__ __forceinline__ unsigned fp4_codes_by_borders(const float (&x)[8], float s) {
+  auto after = [](float v) { return __uint_as_float(__float_as_uint(v) + 1u); };
+  const float b0 = after(0.25f * s), b1 = 0.75f * s, b2 = after(1.25f * s), b3 = 1.75f * s, b4 = after(2.5f * s),
+              b5 = 3.5f * s, b6 = after(5.f * s);
+  unsigned w = 0u;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    most = fmaxf(most, fabsf(x[i]));
-    nan |= x[i] != x[i];
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(x[i]);
+    const bool hi = a >= b3, mid = a >= (hi ? b5 : b1);
+    const bool low = a >= (hi ? (mid ? b6 : b4) : (mid ? b2 : b0));
+    const unsigned c = (hi ? 4u : 0u) | (mid ? 2u : 0u) | (low ? 1u : 0u) | (x[i] < 0.f ? 8u : 0u);
+    w |= c << (4 * i);
   }
-  scale = nan ? 0x7Fu : e4m3_scale(most);
-  const float s = nan ? 0.f : e4m3_value(scale);
-  unsigned w[2] = {0u, 0u};
-  if (s > 0.f) {
-    const float b0 = 0.25f * s, b1 = 0.75f * s, b2 = 1.25f * s, b3 = 1.75f * s, b4 = 2.5f * s, b5 = 3.5f * s,
-                b6 = 5.f * s;
+  return w;
+}
+// The same by division and the conversion instruction: q = x / s correctly rounded
+// (one Newton step from the rounded reciprocal), so a quotient that is a border comes
+// out as it, and the conversion rounds ties to even. Only a q that is a border while
+// x / s is not could go wrong; such a word is left to the comparisons.
+__device__ __forceinline__ unsigned fp4_codes(const float (&x)[8], float s) {
+  const float inv = __frcp_rn(s), most = 7.f * s;  // 6 s is the largest value: further out only saturates
+  float q[8];
+  bool doubt = false;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float a = fabsf(x[i]);
-      unsigned c = static_cast<unsigned>(a > b0) + static_cast<unsigned>(a >= b1) + static_cast<unsigned>(a > b2) +
-                   static_cast<unsigned>(a >= b3) + static_cast<unsigned>(a > b4) + static_cast<unsigned>(a >= b5) +
-                   static_cast<unsigned>(a > b6);
-      if (x[i] < 0.f) c |= 8u;
-      w[i / 8] |= c << (4 * (i % 8));
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float v = fminf(fmaxf(x[i], -most), most);
+    const float q0 = v * inv;
+    q[i] = fmaf(fmaf(-q0, s, v), inv, q0);
+    doubt |= (__float_as_uint(q[i]) & 0x000FFFFFu) == 0u && fmaf(-q[i], s, v) != 0.f;
   }
-  codes = make_uint2(w[0], w[1]);
+  if (doubt) return fp4_codes_by_borders(x, s);
+  unsigned w = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    unsigned byte;  // + 0: a code for -0 has no sign
+    asm("{.reg .b8 b; cvt.rn.satfinite.e2m1x2.f32 b, %1, %2; cvt.u32.u8 %0, b;}" : "=r"(byte) : "f"(q[i + 1] + 0.f), "f"(q[i] + 0.f));
+    w |= byte << (4 * i);
+  }
+  return w;
 }
 
 // ---- append ------------------------------------------------------------------------
+// The heads [head0, head1) of a token on per_pass x (D / V) threads, `tokens` tokens to
+// a CTA.
+struct HeadSplit {
+  int head0, head1, per_pass, passes, tokens;
+};
+
 struct AppendArgs {
   PagedSeqs seqs;
   const void* qkv;
@@ -81,167 +102,277 @@ struct AppendArgs {
   int hq, hkv, head_dim, pairs;
   int64_t table_rows;
   float k_scale, v_scale;
-  int heads_per_pass, passes;
+  HeadSplit all, q, kv;
+  int vec_tables;  // cos/sin rows can be read by 16 bytes
 };
 
-// A thread owns elements [vi * V, vi * V + V) of a head row and walks heads
-// hl, hl + heads_per_pass, ... of its token: the token's cos/sin values are read
-// once for all of them. grid = (token walkers, sequences, parts of the head
-// passes). Bound by memory: it reads qkv once and writes q, k and v once.
-template <typename T, typename KV, int V>
-__global__ void __launch_bounds__(256) qkv_rotary_paged_kernel(const AppendArgs a) {
-  DLI_PDL_ENTRY();
+// A thread owns elements [vi * V, vi * V + V) of a head row and NP heads of a token,
+// hl, hl + heads_per_pass, ..., which it reads at once: a token's cos/sin values and
+// page are read once for all of them. A CTA holds as many tokens as it has room for.
+// Bound by memory: it reads qkv once and writes q, k and v once.
+// V elements of T as they lie in memory: 16-byte vectors where they fill any.
+template <typename T, int V>
+struct Row {
+  static constexpr int kVecs = V * static_cast<int>(sizeof(T)) / 16;
+  union {
+    uint4 raw[kVecs > 0 ? kVecs : 1];
+    uint32_t w[V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1];
+    T e[V];
+  };
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kVecs > 0) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) raw[i] = *reinterpret_cast<const uint4*>(p + i * Vec16<T>::N);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kVecs > 0) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) *reinterpret_cast<uint4*>(p + i * Vec16<T>::N) = raw[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) p[i] = e[i];
+    }
+  }
+  __device__ __forceinline__ float2 pair(int j) const {
+    if constexpr (std::is_same<T, float>::value) return make_float2(e[2 * j], e[2 * j + 1]);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      return make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+  }
+  __device__ __forceinline__ void set_pair(int j, float x, float y) {
+    if constexpr (std::is_same<T, float>::value) {
+      e[2 * j] = x;
+      e[2 * j + 1] = y;
+    } else {
+      w[j] = pack16<T>(x, y);
+    }
+  }
+};
+
+template <typename T, typename KV, int V, int NP>
+__device__ __forceinline__ void append_rows(const AppendArgs& a, const HeadSplit& hs, int walker, int walkers, int part,
+                                            int parts) {
   constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
-  constexpr int kVec = V * static_cast<int>(sizeof(T)) / 16;  // 16-byte vectors per item, 0: one pair
+  constexpr int H = V / 2;  // pairs of a thread
   const int b = blockIdx.y;
   const int d = a.head_dim, ipr = d / V, heads = a.hq + 2 * a.hkv;
-  const int vi = threadIdx.x % ipr, hl = threadIdx.x / ipr;
-  if (hl >= a.heads_per_pass) return;
+  const int per_token = hs.per_pass * ipr;
+  const int tl = threadIdx.x / per_token, lane = threadIdx.x - tl * per_token;
+  if (tl >= hs.tokens) return;
+  const int hl = lane / ipr, vi = lane - hl * ipr;
   const SeqRows sr = seq_rows(a.seqs, b, true);
   const int page_rows = 1 << a.seqs.page_shift;
-  const int part = static_cast<int>(gridDim.z);
-  for (int t = blockIdx.x; t < sr.n; t += gridDim.x) {
+  const int first_pair = vi * H;
+  const int turned = max(0, min(H, a.pairs - first_pair));  // pairs of this thread that rotate
+  const bool full = 2 * a.pairs == d;
+  const int32_t* ids = a.seqs.page_table + b * a.seqs.max_pages;
+  const int head_step = hs.per_pass * d;
+  const int page_bytes = a.hkv * page_rows * d * 9 / 16;  // of 4-bit pages
+  for (int t = walker * hs.tokens + tl; t < sr.n; t += walkers * hs.tokens) {
     const int p = sr.past + t;
     const int64_t row = sr.row0 + t;
-    float c[V / 2], s[V / 2];
-    const int first_pair = vi * (V / 2);
-    const bool in_table = p < a.table_rows;
-    if (!in_table && first_pair < a.pairs) set_device_error(a.seqs.err, kDevErrRotaryPosition);
+    for (int pass = part * NP; pass < hs.passes; pass += parts * NP) {
+      // everything the rows need is asked for before any of it is looked at
+      const int h0 = hs.head0 + hl + pass * hs.per_pass;
+      const T* src = static_cast<const T*>(a.qkv) + row * (heads * d) + h0 * d + vi * V;
+      T* q_row = static_cast<T*>(a.q_out) + row * (a.hq * d) + vi * V;
+      Row<T, V> x[NP];
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) {
-      c[j] = s[j] = 0.f;
-      if (in_table && first_pair + j < a.pairs) {
-        c[j] = a.cos_t[static_cast<int64_t>(p) * a.pairs + first_pair + j];
-        s[j] = a.sin_t[static_cast<int64_t>(p) * a.pairs + first_pair + j];
-      }
-    }
-    const int page = page_of(a.seqs, b, p);
-    for (int pass = blockIdx.z; pass < a.passes; pass += part) {
-      const int h = hl + pass * a.heads_per_pass;
-      if (h >= heads) break;
-      float x[V];
-      const T* src = static_cast<const T*>(a.qkv) + (row * heads + h) * d + vi * V;
-      if constexpr (kVec > 0) {
+      for (int k = 0; k < NP; ++k)
+        if (h0 + k * hs.per_pass < hs.head1) x[k].load(src + k * head_step);
+      float c[H], s[H];
+      const bool turn = turned > 0 && p < a.table_rows && h0 < a.hq + a.hkv;
+      if (turn) {
+        const float* ct = a.cos_t + static_cast<int64_t>(p) * a.pairs + first_pair;
+        const float* st = a.sin_t + static_cast<int64_t>(p) * a.pairs + first_pair;
+        if (H >= 4 && a.vec_tables) {
 #pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-          const Vec16<T> in = load16(src + v * Vec16<T>::N);
-#pragma unroll
-          for (int j = 0; j < Vec16<T>::N; ++j) x[v * Vec16<T>::N + j] = to_f32(in.e[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = to_f32(src[j]);
-      }
-      T* dst = nullptr;
-      if (h < a.hq) {
-        dst = static_cast<T*>(a.q_out) + (row * a.hq + h) * d + vi * V;
-      } else {
-        if (page < 0) continue;
-        const bool is_k = h < a.hq + a.hkv;
-        const int kvh = is_k ? h - a.hq : h - a.hq - a.hkv;
-        const int64_t block = static_cast<int64_t>(page) * a.hkv + kvh;
-        const int r = p & (page_rows - 1);
-        void* pages = is_k ? a.k_pages : a.v_pages;
-        if constexpr (kFp4) {
-          const float cache_scale = is_k ? a.k_scale : a.v_scale;
-          if (is_k || cache_scale != 1.f) {
-            // products of a 24-bit and an at most 24-bit number are exact in 53 bits
-#pragma unroll
-            for (int j = 0; j < V / 2; ++j) {
-              double u = x[2 * j], w = x[2 * j + 1];
-              if (is_k && in_table && first_pair + j < a.pairs) {
-                const double cd = c[j], sd = s[j];
-                const double u0 = u * cd - w * sd;
-                w = u * sd + w * cd;
-                u = u0;
-              }
-              if (cache_scale != 1.f) {
-                u /= static_cast<double>(cache_scale);
-                w /= static_cast<double>(cache_scale);
-              }
-              x[2 * j] = round_to_odd(u);
-              x[2 * j + 1] = round_to_odd(w);
+          for (int j = 0; j + 4 <= H; j += 4) {
+            if (full || j < turned) {
+              const float4 cv = *reinterpret_cast<const float4*>(ct + j), sv = *reinterpret_cast<const float4*>(st + j);
+              c[j] = cv.x, c[j + 1] = cv.y, c[j + 2] = cv.z, c[j + 3] = cv.w;
+              s[j] = sv.x, s[j + 1] = sv.y, s[j + 2] = sv.z, s[j + 3] = sv.w;
             }
           }
-          unsigned scale;
-          uint2 codes;
-          fp4_block(x, scale, codes);
-          uint8_t* base = static_cast<uint8_t*>(pages) + block * fp4_block_bytes(page_rows, d);
-          *reinterpret_cast<uint2*>(base + r * (d / 2) + vi * 8) = codes;
-          base[page_rows * (d / 2) + r * (d / 16) + vi] = static_cast<uint8_t>(scale);
-          continue;
-        }
-        dst = static_cast<T*>(pages) + (block * page_rows + r) * d + vi * V;
-        if (!is_k) {  // v is copied
-          if constexpr (kVec > 0) {
+        } else {
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) store16(dst + v * Vec16<T>::N, load16(src + v * Vec16<T>::N));
-          } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) dst[j] = src[j];
+          for (int j = 0; j < H; ++j) {
+            if (j < turned) {
+              c[j] = ct[j];
+              s[j] = st[j];
+            }
           }
-          continue;
         }
+      } else if (turned > 0 && h0 < a.hq + a.hkv) {
+        set_device_error(a.seqs.err, kDevErrRotaryPosition);
       }
+      const int page = ids[p >> a.seqs.page_shift];
+      const bool good = page >= 0 && page < a.seqs.num_pages;
+      if (!good) set_device_error(a.seqs.err, kDevErrPageIndex);
+      const int r = p & (page_rows - 1);
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) {
-        const float u = x[2 * j], w = x[2 * j + 1];
-        if (in_table && first_pair + j < a.pairs) {
-          x[2 * j] = u * c[j] - w * s[j];
-          x[2 * j + 1] = u * s[j] + w * c[j];
+      for (int k = 0; k < NP; ++k) {
+        const int h = h0 + k * hs.per_pass;
+        if (h >= hs.head1) break;
+        const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.hkv;
+        if (!is_q && !good) break;
+        const int kvh = is_k ? h - a.hq : h - a.hq - a.hkv;
+        if constexpr (kFp4) {
+          if (!is_q) {
+            static_assert(V == 8, "two threads share a block of 16");
+            float f[V];
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+              const float2 v = x[k].pair(j);
+              f[2 * j] = v.x;
+              f[2 * j + 1] = v.y;
+            }
+            const float cache_scale = is_k ? a.k_scale : a.v_scale;
+            if (is_k || cache_scale != 1.f) {
+              // products of a 24-bit and an at most 24-bit number are exact in 53 bits
+#pragma unroll
+              for (int j = 0; j < H; ++j) {
+                double u = f[2 * j], w = f[2 * j + 1];
+                if (is_k && turn && (full || j < turned)) {
+                  const double cd = c[j], sd = s[j];
+                  const double u0 = u * cd - w * sd;
+                  w = u * sd + w * cd;
+                  u = u0;
+                }
+                if (cache_scale != 1.f) {
+                  u /= static_cast<double>(cache_scale);
+                  w /= static_cast<double>(cache_scale);
+                }
+                f[2 * j] = round_to_odd(u);
+                f[2 * j + 1] = round_to_odd(w);
+              }
+            }
+            // the largest magnitude of the block, whose other half is the lane next door
+            // (same token and head, so it is here too); as bits, a NaN is larger than any
+            unsigned most = 0u;
+#pragma unroll
+            for (int j = 0; j < V; ++j) most = max(most, __float_as_uint(f[j]) & 0x7FFFFFFFu);
+            most = max(most, __shfl_xor_sync(3u << (threadIdx.x & 30u), most, 1));
+            const bool nan = most > 0x7F800000u;
+            const unsigned scale = nan ? 0x7Fu : e4m3_scale(__uint_as_float(most));
+            const float sv = nan ? 0.f : e4m3_value(scale);
+            uint8_t* base = static_cast<uint8_t*>(is_k ? a.k_pages : a.v_pages) + static_cast<int64_t>(page) * page_bytes +
+                            kvh * (page_rows * d * 9 / 16);
+            *reinterpret_cast<unsigned*>(base + r * (d / 2) + vi * 4) = sv > 0.f ? fp4_codes(f, sv) : 0u;
+            if ((vi & 1) == 0) base[page_rows * (d / 2) + r * (d / 16) + vi / 2] = static_cast<uint8_t>(scale);
+            continue;
+          }
         }
-      }
-      if constexpr (kVec > 0) {
+        if ((is_q || is_k) && turn) {
 #pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-          Vec16<T> o;
-#pragma unroll
-          for (int j = 0; j < Vec16<T>::N; ++j) o.e[j] = from_f32<T>(x[v * Vec16<T>::N + j]);
-          store16(dst + v * Vec16<T>::N, o);
+          for (int j = 0; j < H; ++j) {
+            if (full || j < turned) {
+              const float2 v = x[k].pair(j);
+              x[k].set_pair(j, v.x * c[j] - v.y * s[j], v.x * s[j] + v.y * c[j]);
+            }
+          }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) dst[j] = from_f32<T>(x[j]);
+        if (is_q) {
+          x[k].store(q_row + h * d);
+        } else {
+          T* page_at = static_cast<T*>(is_k ? a.k_pages : a.v_pages) + static_cast<int64_t>(page) * (a.hkv * page_rows * d);
+          x[k].store(page_at + (kvh * page_rows + r) * d + vi * V);
+        }
       }
     }
   }
 }
 
+// grid = (token walkers, sequences, parts of the head passes).
+template <typename T, typename KV, int V, int NP>
+__global__ void __launch_bounds__(256, NP == 1 ? 2 : 4) qkv_rotary_paged_kernel(const AppendArgs a) {
+  DLI_PDL_ENTRY();
+  append_rows<T, KV, V, NP>(a, a.all, blockIdx.x, gridDim.x, blockIdx.z, gridDim.z);
+}
+
+// Many tokens into 4-bit pages: every other CTA streams q, three heads a thread, while
+// its neighbours quantise k and v, whose arithmetic (ALU half busy) then hides under the
+// streaming. grid = (2 x token walkers, sequences).
+template <typename T>
+__global__ void __launch_bounds__(256, 4) qkv_rotary_paged_fp4_kernel(const AppendArgs a) {
+  DLI_PDL_ENTRY();
+  const int walker = blockIdx.x >> 1, walkers = gridDim.x >> 1;
+  if (blockIdx.x & 1) append_rows<T, Fp4, 8, 1>(a, a.kv, walker, walkers, 0, 1);
+  else append_rows<T, T, 8, 3>(a, a.q, walker, walkers, 0, 1);
+}
+
 template <typename T, typename KV, int V>
 void launch_append(AppendArgs a, cudaStream_t stream) {
-  const int ipr = a.head_dim / V, heads = a.hq + 2 * a.hkv;
-  a.passes = static_cast<int>(ceil_div(static_cast<int64_t>(heads) * ipr, 256));
-  a.heads_per_pass = static_cast<int>(ceil_div(heads, a.passes));
-  const int threads = std::min(256, static_cast<int>(ceil_div(a.heads_per_pass * ipr, 32)) * 32);
-  // few tokens: one head pass per CTA, the shortest chain; many: all passes in one
+  constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
   const int64_t slots = static_cast<int64_t>(sm_count()) * 8;
-  const int64_t tokens = static_cast<int64_t>(a.seqs.batch) * a.seqs.max_new;
-  const unsigned parts = tokens * a.passes <= slots ? static_cast<unsigned>(a.passes) : 1u;
-  const int64_t walkers = std::min<int64_t>(a.seqs.max_new, ceil_div(4 * slots, a.seqs.batch));
-  launch_pdl(qkv_rotary_paged_kernel<T, KV, V>,
-             dim3(static_cast<unsigned>(walkers), static_cast<unsigned>(a.seqs.batch), parts),
-             dim3(static_cast<unsigned>(threads)), 0, stream, a);
+  const int64_t tokens = std::min<int64_t>(a.seqs.tokens, static_cast<int64_t>(a.seqs.batch) * a.seqs.max_new);
+  const unsigned batch = static_cast<unsigned>(a.seqs.batch);
+  const int ipr = a.head_dim / V;
+  auto split = [&](int head0, int head1, int at_least) {
+    HeadSplit s{};
+    const int heads = head1 - head0;
+    s.head0 = head0;
+    s.head1 = head1;
+    s.passes = static_cast<int>(std::max<int64_t>(ceil_div(static_cast<int64_t>(heads) * ipr, 256), std::min(at_least, heads)));
+    s.per_pass = static_cast<int>(ceil_div(heads, s.passes));
+    s.passes = static_cast<int>(ceil_div(heads, s.per_pass));
+    s.tokens = std::max(1, 256 / (s.per_pass * ipr));
+    return s;
+  };
+  auto threads = [&](const HeadSplit& s) { return static_cast<unsigned>(ceil_div(s.per_pass * ipr * s.tokens, 32) * 32); };
+  // eight tokens or more for each place in a CTA, while that leaves enough CTAs
+  auto walkers = [&](const HeadSplit& s) {
+    const int64_t steps = ceil_div(a.seqs.max_new, s.tokens);
+    return static_cast<unsigned>(std::min<int64_t>(steps, std::max<int64_t>(ceil_div(steps, 8), ceil_div(2 * slots, a.seqs.batch))));
+  };
+  const int heads = a.hq + 2 * a.hkv;
+  a.all = split(0, heads, 3);
+  if (tokens * a.all.passes <= slots) {
+    // few tokens: one head of each thread per CTA, the shortest chain
+    a.all.tokens = 1;
+    launch_pdl(qkv_rotary_paged_kernel<T, KV, V, 1>,
+               dim3(static_cast<unsigned>(a.seqs.max_new), batch, static_cast<unsigned>(a.all.passes)),
+               dim3(threads(a.all)), 0, stream, a);
+  } else if constexpr (kFp4) {
+    a.q = split(0, a.hq, 3);
+    a.kv = split(a.hq, heads, 1);
+    launch_pdl(qkv_rotary_paged_fp4_kernel<T>, dim3(2u * std::max(walkers(a.q), walkers(a.kv)), batch),
+               dim3(std::max(threads(a.q), threads(a.kv))), 0, stream, a);
+  } else {
+    launch_pdl(qkv_rotary_paged_kernel<T, KV, V, 3>, dim3(walkers(a.all), batch), dim3(threads(a.all)), 0, stream, a);
+  }
 }
 
 // ---- gather ------------------------------------------------------------------------
 struct GatherArgs {
   PagedSeqs seqs;  // positions: first rows (or null), starts: lengths (or null)
-  const void* pages[2];
-  void* out[2];
-  float scale[2];
+  const void* k_pages;
+  const void* v_pages;
+  void* k_out;
+  void* v_out;
+  float k_scale, v_scale;
   int hkv, head_dim;
   int64_t count;
 };
 
-// One thread per 8 elements (one in the general form) of an output row; grid =
-// (row walkers, sequences x heads, K and V). Bound by memory.
+// A thread owns elements [vi * V, vi * V + V) of a row and walks rows; grid = (row
+// walkers, sequences x heads, K and V). Bound by memory.
 template <typename T, typename KV, int V>
 __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
   DLI_PDL_ENTRY();
   constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
+  constexpr int U = 2;  // rows in flight
   const int b = blockIdx.y / a.hkv, h = blockIdx.y - b * a.hkv;
-  const int which = blockIdx.z;
+  const void* pages = blockIdx.z ? a.v_pages : a.k_pages;
+  const float scale = blockIdx.z ? a.v_scale : a.k_scale;
   const int d = a.head_dim, ipr = d / V, page_rows = 1 << a.seqs.page_shift;
+  const int per_cta = 256 / ipr;  // rows
+  const int vi = threadIdx.x % ipr, rl = threadIdx.x / ipr;
+  if (rl >= per_cta) return;
   const int64_t rows_max = a.seqs.max_pages << a.seqs.page_shift;
   const int64_t first = a.seqs.positions ? a.seqs.positions[b] : 0;
   int64_t end = a.seqs.starts ? a.seqs.starts[b] : rows_max;
@@ -249,40 +380,32 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
     if (threadIdx.x == 0) set_device_error(a.seqs.err, kDevErrKvCapacity);
     end = min(end, rows_max);
   }
-  T* out = static_cast<T*>(a.out[which]) + static_cast<int64_t>(blockIdx.y) * a.count * d;
-  const int64_t items = a.count * ipr;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < items; i += gridDim.x * 256ll) {
-    const int64_t r = i / ipr;
-    const int c = static_cast<int>(i - r * ipr) * V;
-    const int64_t p = first + r;
-    T v[V];
+  T* out = static_cast<T*>(blockIdx.z ? a.v_out : a.k_out) + static_cast<int64_t>(blockIdx.y) * a.count * d + vi * V;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * per_cta;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per_cta + rl; r0 < a.count; r0 += U * stride) {
+    Row<T, V> x[U];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = from_f32<T>(0.f);
-    const int page = (p >= 0 && p < end) ? page_of(a.seqs, b, static_cast<int>(p)) : -1;
-    if (page >= 0) {
+    for (int k = 0; k < U; ++k) {
+      const int64_t p = first + r0 + k * stride;
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[k].e[j] = from_f32<T>(0.f);
+      const int page = r0 + k * stride < a.count && p >= 0 && p < end ? page_of(a.seqs, b, static_cast<int>(p)) : -1;
+      if (page < 0) continue;
       const int64_t block = static_cast<int64_t>(page) * a.hkv + h;
       const int pr = static_cast<int>(p) & (page_rows - 1);
       if constexpr (kFp4) {
-        const uint8_t* base = static_cast<const uint8_t*>(a.pages[which]) + block * fp4_block_bytes(page_rows, d);
-        const float s = e4m3_value(base[page_rows * (d / 2) + pr * (d / 16) + c / 16]);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + pr * (d / 2) + c / 2);
+        const uint8_t* base = static_cast<const uint8_t*>(pages) + block * fp4_block_bytes(page_rows, d);
+        const uint2 w = *reinterpret_cast<const uint2*>(base + pr * (d / 2) + vi * 8);
+        const float s = e4m3_value(base[page_rows * (d / 2) + pr * (d / 16) + vi]) * 16384.f;  // exact
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = from_f32<T>(e2m1_value((w >> (4 * j)) & 15u) * s * a.scale[which]);
+        for (int j = 0; j < V; ++j) x[k].e[j] = from_f32<T>(e2m1_small(((j < 8 ? w.x : w.y) >> (4 * (j & 7))) & 15u) * s * scale);
       } else {
-        const T* src = static_cast<const T*>(a.pages[which]) + (block * page_rows + pr) * d + c;
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = src[j];
+        x[k].load(static_cast<const T*>(pages) + (block * page_rows + pr) * d + vi * V);
       }
     }
-    T* dst = out + r * d + c;
-    if constexpr (V * sizeof(T) >= 16) {
 #pragma unroll
-      for (int q = 0; q < static_cast<int>(V * sizeof(T) / 16); ++q)
-        *reinterpret_cast<uint4*>(dst + q * Vec16<T>::N) = *reinterpret_cast<uint4*>(&v[q * Vec16<T>::N]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) dst[j] = v[j];
-    }
+    for (int k = 0; k < U; ++k)
+      if (r0 + k * stride < a.count) x[k].store(out + (r0 + k * stride) * d);
   }
 }
 
@@ -407,7 +530,7 @@ dli_status check_pages(const std::string& what, int64_t batch, int64_t kv_heads,
     if (!aligned(k_pages, 16) || !aligned(v_pages, 16))
       return fail(DLI_ERR_INVALID_ARGUMENT, what + ": 4-bit pages must be 16-byte aligned");
   }
-  if (batch > 65535) return fail(DLI_ERR_UNSUPPORTED, what + ": more than 65535 sequences");
+  if (batch > 65535 || kv_heads > 65535) return fail(DLI_ERR_UNSUPPORTED, what + ": more than 65535 sequences or heads");
   if (num_pages > INT_MAX || max_pages > (1ll << 30) / page_size)
     return fail(DLI_ERR_UNSUPPORTED, what + ": more than 2^30 rows per sequence or 2^31 pages");
   if (batch > 0 && (k_pages == nullptr || v_pages == nullptr || page_table == nullptr) && num_pages > 0 && max_pages > 0)
@@ -419,6 +542,7 @@ dli_status check_rows(const std::string& what, int64_t tokens, int64_t batch, in
                       const void* positions, const void* starts) {
   if (tokens < 0 || max_new < 0 || q_heads <= 0) return fail(DLI_ERR_INVALID_ARGUMENT, what + ": bad sizes");
   if (positions == nullptr) return fail(DLI_ERR_INVALID_ARGUMENT, what + ": positions required");
+  if (q_heads > 65535) return fail(DLI_ERR_UNSUPPORTED, what + ": more than 65535 heads");
   if (max_new > (1 << 30)) return fail(DLI_ERR_UNSUPPORTED, what + ": sequence too long");
   if (starts == nullptr && tokens < batch * max_new)
     return fail(DLI_ERR_INVALID_ARGUMENT, what + ": fewer rows than batch * max_new");
@@ -489,14 +613,14 @@ extern "C" dli_status dli_sm100_qkv_rotary_paged(const void* qkv, const float* c
   a.k_scale = k_scale;
   a.v_scale = v_scale;
   const bool al = aligned(qkv, 16) && aligned(q_out, 16) && aligned(k_pages, 16) && aligned(v_pages, 16);
-  if (kv_dtype == DLI_DTYPE_FP4 && (!al || head_dim > 4096))
-    return fail(DLI_ERR_INVALID_ARGUMENT, "qkv_rotary_paged: 4-bit pages need 16-byte aligned tensors and head_dim <= 4096");
-  if (kv_dtype != DLI_DTYPE_FP4 && head_dim > 512)
-    return fail(DLI_ERR_UNSUPPORTED, "qkv_rotary_paged: head_dim > 512");
+  if (kv_dtype == DLI_DTYPE_FP4 && !al)
+    return fail(DLI_ERR_INVALID_ARGUMENT, "qkv_rotary_paged: 4-bit pages need 16-byte aligned tensors");
+  if (head_dim > 256) return fail(DLI_ERR_UNSUPPORTED, "qkv_rotary_paged: head_dim > 256");
+  a.vec_tables = pairs % 4 == 0 && aligned(cos_table, 16) && aligned(sin_table, 16);
   st = dispatch_float(dtype, what, [&](auto tag) {
     using T = decltype(tag);
     constexpr int V = Vec16<T>::N;
-    if (kv_dtype == DLI_DTYPE_FP4) launch_append<T, Fp4, 16>(a, as_stream(stream));
+    if (kv_dtype == DLI_DTYPE_FP4) launch_append<T, Fp4, 8>(a, as_stream(stream));
     else if (al && head_dim % V == 0) launch_append<T, T, V>(a, as_stream(stream));
     else launch_append<T, T, 2>(a, as_stream(stream));
   });
@@ -518,28 +642,33 @@ extern "C" dli_status dli_sm100_paged_gather(const void* k_pages, const void* v_
   if (batch == 0 || count == 0) return ok();
   GatherArgs a{};
   a.seqs = make_seqs(first, lengths, page_table, 0, batch, 0, page_size, num_pages, max_pages);
-  a.pages[0] = k_pages;
-  a.pages[1] = v_pages;
-  a.out[0] = k_out;
-  a.out[1] = v_out;
-  a.scale[0] = k_scale;
-  a.scale[1] = v_scale;
+  a.k_pages = k_pages;
+  a.v_pages = v_pages;
+  a.k_out = k_out;
+  a.v_out = v_out;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
   a.hkv = static_cast<int>(kv_heads);
   a.head_dim = static_cast<int>(head_dim);
   a.count = count;
   const bool al = aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(k_out, 16) && aligned(v_out, 16);
   if (kv_dtype == DLI_DTYPE_FP4 && !al)
     return fail(DLI_ERR_INVALID_ARGUMENT, "paged_gather: 4-bit pages need 16-byte aligned tensors");
+  if (head_dim > 256) return fail(DLI_ERR_UNSUPPORTED, "paged_gather: head_dim > 256");
   st = dispatch_float(dtype, what, [&](auto tag) {
     using T = decltype(tag);
-    const bool vec = al && head_dim % 8 == 0;
-    const int64_t items = count * (vec ? head_dim / 8 : head_dim);
-    const int64_t walkers = std::min<int64_t>(ceil_div(items, 256),
-                                              std::max<int64_t>(1, ceil_div(32ll * sm_count(), batch * kv_heads)));
-    const dim3 grid(static_cast<unsigned>(walkers), static_cast<unsigned>(batch * kv_heads), 2u);
-    if (kv_dtype == DLI_DTYPE_FP4) launch_pdl(paged_gather_kernel<T, Fp4, 8>, grid, dim3(256), 0, as_stream(stream), a);
-    else if (vec) launch_pdl(paged_gather_kernel<T, T, 8>, grid, dim3(256), 0, as_stream(stream), a);
-    else launch_pdl(paged_gather_kernel<T, T, 1>, grid, dim3(256), 0, as_stream(stream), a);
+    auto grid = [&](int64_t elements) {  // of a thread
+      const int64_t per_cta = 256 / (head_dim / elements);
+      const int64_t walkers = std::min<int64_t>(ceil_div(count, per_cta),
+                                                std::max<int64_t>(1, ceil_div(32ll * sm_count(), batch * kv_heads)));
+      return dim3(static_cast<unsigned>(walkers), static_cast<unsigned>(batch * kv_heads), 2u);
+    };
+    if (kv_dtype == DLI_DTYPE_FP4)
+      launch_pdl(paged_gather_kernel<T, Fp4, 16>, grid(16), dim3(256), 0, as_stream(stream), a);
+    else if (al && head_dim % Vec16<T>::N == 0)
+      launch_pdl(paged_gather_kernel<T, T, Vec16<T>::N>, grid(Vec16<T>::N), dim3(256), 0, as_stream(stream), a);
+    else
+      launch_pdl(paged_gather_kernel<T, T, 1>, grid(1), dim3(256), 0, as_stream(stream), a);
   });
   if (st != DLI_OK) return st;
   return check_launch(what);

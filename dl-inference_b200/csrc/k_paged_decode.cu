@@ -67,7 +67,7 @@ struct DecodeLayout {
   static constexpr int kThreads = 32 * W + 32;
   static constexpr int R = 8 * NT;
   static constexpr int BN = 16 * W * SUB;  // keys per block
-  static constexpr int kCtas = kF32 || (kFp4 && (NT == 2 || std::is_same<T, float>::value)) ? 1 : 2;
+  static constexpr int kCtas = kF32 || (kFp4 && (NT == 2 || std::is_same<T, float>::value)) ? 1 : kFp4 ? 3 : 2;
   static constexpr int kRowBytes = kFp4 ? D / 2 : kF32 ? D * 4 : D * 2;
   static constexpr int kBox = BN * 128;          // bytes of one 128-byte-wide column of boxes
   static constexpr int kCodes = BN * kRowBytes;  // code or element bytes of a K (or V) block
@@ -75,7 +75,7 @@ struct DecodeLayout {
   static constexpr int DH = 64;  // dims that the warps merge at a time
   static constexpr int kMerge = W * R * DH * 4;
   static constexpr int kMl = 2 * W * R * 4;
-  static constexpr int kRoom = (kCtas == 2 ? 113 : 227) * 1024 - kMerge - kMl - 1024 - 256;
+  static constexpr int kRoom = (kCtas == 3 ? 75 : kCtas == 2 ? 113 : 227) * 1024 - kMerge - kMl - 1024 - 256;
   static constexpr int kEntries = (kRoom / kEntry) < 16 ? (kRoom / kEntry) : 16;
   static constexpr int kMergeOff = kEntries * kEntry;
   static constexpr int kMlOff = kMergeOff + kMerge;
@@ -1041,7 +1041,7 @@ struct DecodePlan {
 // exceed kWholeKeys runs one CTA per unit.
 constexpr int kWholeKeys = 512;
 constexpr int kMinKeys = 256;
-constexpr int kMaxCtasPerSm = 2;
+constexpr int kMaxCtasPerSm = 3;
 
 DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys,
                              bool f32) {

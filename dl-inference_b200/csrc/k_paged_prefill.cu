@@ -185,6 +185,9 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   if (share >= shares) return;
   const int block_first = x.block0 + static_cast<int>(static_cast<int64_t>(share) * x.blocks / shares);
   const int nblocks = x.block0 + static_cast<int>(static_cast<int64_t>(share + 1) * x.blocks / shares) - block_first;
+  // the last keys first: with a distance bias the maximum is then met early, and O is
+  // not rescaled block after block
+  auto key_of = [&](int j) { return (block_first + nblocks - 1 - j) * BN; };  // first key of step j
 
   if (threadIdx.x == 0) {
     constexpr int kWriters = kFp4 ? 4 : 1;  // warps that fill Q, K and V, or TMA
@@ -232,8 +235,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         tma_load_4d(smem + c * L::kBox, &tq, c * 64, kvh * a.group, static_cast<int>(x.rows.row0) + x.t0, 0, q_full);
     }
     auto page_for = [&](int j) {  // of lane's box of block j
-      const int i = (((block_first + j) * BN) >> shift) + lane;
       int page = none;
+      const int i = j < nblocks ? (key_of(j) >> shift) + lane : 0;
       if (lane < boxes && j < nblocks && i <= last_page) {
         page = ids[i];
         if (page < 0 || page >= none) {
@@ -255,7 +258,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       if (lane == 0) mbar_arrive_expect_tx(full, L::kKVBytes);
       __syncwarp();
       if (lane < boxes) {
-        const int row = ((block_first + j) * BN) & (page_rows - 1);
+        const int row = key_of(j) & (page_rows - 1);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
           tma_load_4d(dst + c * (BN * 128) + lane * box_rows * 128, is_k ? &tk : &tv, c * 64, row, kvh, page, full);
@@ -347,8 +350,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     const int64_t block_bytes = fp4_block_bytes(page_rows, D);
     const uint8_t* pages[2] = {static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages)};
     auto page_for = [&](int j) {
-      const int key = (block_first + j) * BN + key_row;
-      if (j >= nblocks || key >= x.kv_len || key < x.key_lo) return -1;
+      const int key = j < nblocks ? key_of(j) + key_row : -1;
+      if (key < 0 || key >= x.kv_len || key < x.key_lo) return -1;
       const int page = ids[key >> shift];
       if (page < 0 || page >= a.seqs.num_pages) {
         set_device_error(a.seqs.err, kDevErrPageIndex);
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       for (int i = 0; i < WORDS; ++i) w[i] = 0u;
       sc = 0u;  // rows that are not of the tile's keys: zeros
       if (page < 0) return;
-      const int r = ((block_first + j) * BN + key_row) & (page_rows - 1);
+      const int r = (key_of(j) + key_row) & (page_rows - 1);
       const uint8_t* base = pages[which] + (static_cast<int64_t>(page) * a.hkv + kvh) * block_bytes;
 #pragma unroll
       for (int i = 0; i < WORDS; i += 4) {
@@ -477,7 +480,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_empty[sb]);
 
-      const int key0 = (block_first + j) * BN;
+      const int key0 = key_of(j);
       if (cap) {
 #pragma unroll
         for (int i = 0; i < BN; ++i) s[i] = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(s[i] * in_scale));

@@ -69,12 +69,12 @@ __device__ __forceinline__ float e4m3_value(unsigned byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
 }
 
-// E2M1 nibble -> float: 3 magnitude bits placed as the low exponent bits and top
-// mantissa bit of a half are 2^-14 of the value (subnormals included).
-__device__ __forceinline__ float e2m1_value(unsigned nibble) {
-  const unsigned short h = static_cast<unsigned short>(((nibble & 8u) << 12) | ((nibble & 7u) << 9));
-  return __half2float(__ushort_as_half(h)) * 16384.f;
+// 2^-14 of an E2M1 nibble's value: its 3 magnitude bits as the low exponent bits and
+// the top mantissa bit of a half (subnormals included).
+__device__ __forceinline__ float e2m1_small(unsigned nibble) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(((nibble & 8u) << 12) | ((nibble & 7u) << 9))));
 }
+__device__ __forceinline__ float e2m1_value(unsigned nibble) { return e2m1_small(nibble) * 16384.f; }
 
 // Element `c` of row `r` of a (page, head) block of 4-bit pages.
 __device__ __forceinline__ float fp4_element(const uint8_t* block, int page_rows, int d, int r, int c) {

@@ -276,8 +276,8 @@ dli_status dli_sm100_attention_kvcache_noalloc(const void* q, const void* cache_
  * page_table[b, p / page_size]. page_size is 16, 32, 64 or 128. Sequences may
  * share pages that no call appends to.
  *
- * k_pages / v_pages: [num_pages, kv_heads, page_size, head_dim] of kv_dtype ==
- * dtype, or with kv_dtype = DLI_DTYPE_FP4 (head_dim a multiple of 16)
+ * head_dim is at most 256 in every call. k_pages / v_pages: [num_pages, kv_heads,
+ * page_size, head_dim] of kv_dtype == dtype, or with kv_dtype = DLI_DTYPE_FP4 (head_dim a multiple of 16)
  * [num_pages, kv_heads, page_size * head_dim * 9 / 16] bytes: per (page, head)
  * the page_size rows of head_dim / 2 code bytes (E2M1, element 2i in the low
  * half of byte i), then page_size rows of head_dim / 16 scale bytes (E4M3). A
@@ -316,7 +316,7 @@ dli_status dli_sm100_qkv_rotary_paged(const void* qkv, const float* cos_table, c
  * window > 0 only i - window < j. Score of (i, j) in head h: x = scale * q . k;
  * softcap > 0: x = softcap * tanh(x / softcap); slopes (float [Hq], NULL = none):
  * x += slopes[h] * (j - i). scale <= 0 selects 1/sqrt(D). Hq must be a multiple
- * of Hkv; head_dim <= 256. The workspace is scratch: nothing in it has to be
+ * of Hkv. The workspace is scratch: nothing in it has to be
  * initialised or kept, but calls that may overlap on the GPU need their own. */
 size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads,
                                                 int64_t kv_heads, int64_t head_dim, int64_t page_size,
