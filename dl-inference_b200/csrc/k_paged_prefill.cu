@@ -7,25 +7,31 @@
 // so a K/V block is fetched once for the whole group and a tile's rows differ by
 // few tokens: few blocks are partly masked.
 //
-// One CTA = one tile, or one of `splits` shares of its key blocks when the tiles
-// alone do not fill the GPU; 192 threads, two CTAs per SM:
-//   warp 0     loads the Q tile once (a box of group x tokens of q by TMA), walks
-//              the page table and loads 64-key K and V blocks (a box per page;
-//              boxes past the sequence or of a bad page read as zeros) into rings
-//              of 3 and 2 stages;
+// The grid is the list of tiles (longest first within groups of (sequence, KV head)
+// pairs whose K/V stay in L2), or of the tiles' `splits` shares of key blocks when the
+// tiles alone do not fill the GPU. A CTA that works claims the next one of the list from
+// the hardware scheduler (cluster launch control) while it computes, so two CTAs per SM
+// stay for the whole call, one tile's end overlaps the next one's start, and a ragged
+// batch is balanced as it runs (which CTA computes a tile changes nothing in it).
+// 192 threads:
+//   warp 0     loads each Q tile (a box of group x tokens of q by TMA), walks the page
+//              table and loads 64-key K and V blocks (a box per page; boxes past the
+//              sequence or of a bad page read as zeros) into rings of 3 and 2 stages,
+//              running ahead into the next tile;
 //   warp 1     allocates tensor memory and issues the MMAs, S_j = Q K_j^T and
 //              O += P_j V_j, in the order S_0, S_1, P_0 V_0, S_2, ...;
 //   warps 2-5  softmax, one thread per row: S from tensor memory, cap, bias and
 //              mask, running maximum (moved only when it grows by more than 2^8,
 //              so O is seldom rescaled) and sum in fp32, P as 16 bits over S's own
-//              columns; at the end O / sum through shared memory to the rows, or
-//              the share's (max, sum, O) to the workspace.
+//              columns; at the end O / sum to the rows, or the share's (max, sum, O)
+//              to the workspace, while the next tile's first S is computed.
 // 4-bit pages: no producer warp; four converter warps read codes and scales a
 // block ahead into registers and write the K and V stages as halves (E2M1 x E4M3
 // has 6 significant bits: exact), and the MMAs run in f16 for every model type. The
 // softmax warps then write the Q tile, each row scaled by a power of two (exact), and
 // undo the scale on the scores.
-// Every wait is bounded; one that runs out sets the device error word.
+// Every wait is bounded; one that runs out sets the device error word and winds the
+// CTA down.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -62,9 +68,11 @@ struct PrefillLayout {
   static constexpr int kKOff = kQBytes;
   static constexpr int kVOff = kKOff + KST * kKVBytes;
   static constexpr int kBarOff = kVOff + VST * kKVBytes;
-  // q_full, k_full/empty, v_full/empty, s_full[2], s_empty[2], p_full, o_done, mma_done
-  static constexpr int kBars = 1 + 2 * KST + 2 * VST + 4 + 3;
-  static constexpr int kBytes = kBarOff + kBars * 8 + 16;  // two CTAs fit without alignment slack
+  static constexpr int kClaims = 2 * 16;  // answers of the scheduler, then the barriers:
+  // q_full, q_empty, k_full/empty, v_full/empty, s_full[2], s_empty[2], p_full, o_done,
+  // o_full, o_empty, mma_done, claim_full[2], claim_empty[2]
+  static constexpr int kBars = 2 + 2 * KST + 2 * VST + 4 + 5 + 4;
+  static constexpr int kBytes = kBarOff + kClaims + kBars * 8 + 16;  // two CTAs fit without alignment slack
   static constexpr uint32_t kTmemCols = 256;
   static constexpr uint32_t kOCol = 2 * BN;
   static_assert(kBytes <= 115712, "two CTAs per SM");
@@ -74,7 +82,10 @@ struct PrefillLayout {
 struct PrefillArgs {
   PagedAttnArgs a;
   int tile_tokens;  // 128 / group
+  int tiles;        // of a sequence of max_new tokens
   int splits;
+  int pairs_group;  // (sequence, KV head) pairs whose tiles are interleaved
+  int wide_out;     // out is 32-byte aligned
   float* part_o;    // [units * splits][128][D]
   float2* part_ml;  // [units * splits][128]
   unsigned q_bytes; // of the Q box
@@ -85,23 +96,89 @@ __device__ __forceinline__ int shares_of(int blocks, int splits) { return max(1,
 
 struct Tile {
   SeqRows rows;
-  int t0, tokens;       // of the tile
-  int kv_len, key_lo;   // keys any of its rows sees: [key_lo, kv_len)
-  int block0, blocks;
+  int b, kvh, tile, share, shares;
+  int t0, tokens;      // of the tile
+  int kv_len, key_lo;  // keys any of its rows sees: [key_lo, kv_len)
+  int block_first, nblocks;
+  // the last keys first: with a distance bias the maximum is then met early, and O is
+  // not rescaled block after block
+  __device__ __forceinline__ int key_of(int j) const { return (block_first + nblocks - 1 - j) * BN; }
 };
 
-__device__ __forceinline__ Tile tile_of(const PrefillArgs& p, int b, int tile, bool report) {
-  Tile x;
-  x.rows = seq_rows(p.a.seqs, b, report);
-  x.t0 = tile * p.tile_tokens;
-  x.tokens = max(0, min(p.tile_tokens, x.rows.n - x.t0));
+// Tile (or share) `at` of the list; false when there is nothing to do in it. Order:
+// groups of pairs, within a group the longest tiles first, their shares, the pairs.
+__device__ __forceinline__ bool tile_at(const PrefillArgs& p, int at, Tile& x, bool report) {
+  const int pairs = p.a.hkv * p.a.seqs.batch;
+  const int per_pair = p.tiles * p.splits;
+  const int group = at / per_pair / p.pairs_group;  // at < pairs * per_pair
+  const int first = group * p.pairs_group, size = min(p.pairs_group, pairs - first);
+  const int in_group = at - first * per_pair;
+  const int rank = in_group / size, pair = first + in_group - rank * size;
+  x.b = pair / p.a.hkv;
+  x.kvh = pair - x.b * p.a.hkv;
+  x.tile = p.tiles - 1 - rank / p.splits;
+  x.share = rank % p.splits;
+  x.rows = seq_rows(p.a.seqs, x.b, report && x.tile == 0);
+  x.t0 = x.tile * p.tile_tokens;
+  x.tokens = min(p.tile_tokens, x.rows.n - x.t0);
+  if (x.tokens <= 0) return false;
   const int pos0 = x.rows.past + x.t0;
   x.kv_len = pos0 + x.tokens;
   x.key_lo = p.a.window <= pos0 ? pos0 - p.a.window + 1 : 0;
-  x.block0 = x.key_lo / BN;
-  x.blocks = (x.kv_len + BN - 1) / BN - x.block0;
-  return x;
+  const int block0 = x.key_lo / BN, blocks = (x.kv_len + BN - 1) / BN - block0;
+  x.shares = shares_of(blocks, p.splits);
+  if (x.share >= x.shares) return false;
+  x.block_first = block0 + static_cast<int>(static_cast<int64_t>(x.share) * blocks / x.shares);
+  x.nblocks = block0 + static_cast<int>(static_cast<int64_t>(x.share + 1) * blocks / x.shares) - x.block_first;
+  return true;
 }
+
+// A warp's (or, for the MMA thread, a thread's) way through the tiles of its CTA: the
+// CTA's own first, then what it claims. The MMA thread asks for the next one as soon as
+// a tile begins; every warp reads the answers. Two answers alternate; a slot is asked
+// for again once all `readers` have left it.
+struct TileWalk {
+  const PrefillArgs& p;
+  uint8_t* answers;
+  uint64_t* full;
+  uint64_t* empty;
+  bool asks, single;  // single: one thread walks, not a warp
+  int n = 0;          // answers read
+  bool open = false;  // (asks) an answer is outstanding
+
+  __device__ __forceinline__ void ask() {
+    if (!asks) return;
+    if (!mbar_wait(&empty[n & 1], ((n >> 1) & 1) ^ 1)) return;  // the wait below then runs out
+    mbar_arrive_expect_tx(&full[n & 1], 16);
+    claim_next_cta(answers + 16 * (n & 1), &full[n & 1]);
+    open = true;
+  }
+  // The CTA index of the next tile, -1 at the end, -2 when a wait ran out.
+  __device__ __forceinline__ int claim(volatile int* abort_flag) {
+    bool got = mbar_wait(&full[n & 1], (n >> 1) & 1) && *abort_flag == 0;
+    if (!single) got = __all_sync(0xffffffffu, got);
+    if (!got) return -2;
+    const int at = claimed_cta(answers + 16 * (n & 1));
+    open = false;
+    fence_proxy_async_smem();  // read before the slot is written again
+    if (!single) __syncwarp();
+    if (single || (threadIdx.x & 31) == 0) mbar_arrive(&empty[n & 1]);
+    ++n;
+    return at;
+  }
+  // Advances to the next tile with work. `at`: -1 before the first call.
+  __device__ __forceinline__ bool next(Tile& x, int& at, bool report, volatile int* abort_flag, bool& ok) {
+    while (true) {
+      at = at == -1 ? static_cast<int>(blockIdx.x) : claim(abort_flag);
+      if (at < 0) {
+        ok = ok && at == -1;
+        return false;
+      }
+      ask();
+      if (tile_at(p, at, x, report)) return true;
+    }
+  }
+};
 
 __device__ __forceinline__ float max3f(float a, float b, float c) {
   float d;
@@ -157,8 +234,9 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     if (threadIdx.x == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
     return;  // uniform for the CTA, nothing was started
   }
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
-  uint64_t* k_full = q_full + 1;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff + L::kClaims);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_empty + 1;
   uint64_t* k_empty = k_full + KST;
   uint64_t* v_full = k_empty + KST;
   uint64_t* v_empty = v_full + VST;
@@ -166,32 +244,19 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_empty + 2;
   uint64_t* o_done = p_full + 1;
-  uint64_t* mma_done = o_done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* o_full = o_done + 1;
+  uint64_t* o_empty = o_full + 1;
+  uint64_t* mma_done = o_empty + 1;
+  uint64_t* claim_full = mma_done + 1;
+  uint64_t* claim_empty = claim_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(claim_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per_split = gridDim.x / p.splits;
-  const int tile = per_split - 1 - static_cast<int>(blockIdx.x) / p.splits;  // the longest first
-  const int share = static_cast<int>(blockIdx.x) % p.splits;
-  const int kvh = blockIdx.y, b = blockIdx.z;
-
-  // starts and positions may come from the kernel before
-  pdl_wait();
-  pdl_trigger();
-  const Tile x = tile_of(p, b, tile, threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0);
-  if (x.tokens <= 0) return;  // uniform for the CTA, nothing was started
-  const int shares = shares_of(x.blocks, p.splits);
-  if (share >= shares) return;
-  const int block_first = x.block0 + static_cast<int>(static_cast<int64_t>(share) * x.blocks / shares);
-  const int nblocks = x.block0 + static_cast<int>(static_cast<int64_t>(share + 1) * x.blocks / shares) - block_first;
-  // the last keys first: with a distance bias the maximum is then met early, and O is
-  // not rescaled block after block
-  auto key_of = [&](int j) { return (block_first + nblocks - 1 - j) * BN; };  // first key of step j
-
   if (threadIdx.x == 0) {
     constexpr int kWriters = kFp4 ? 4 : 1;  // warps that fill Q, K and V, or TMA
     mbar_init(q_full, kWriters);
+    mbar_init(q_empty, 1);
     for (int s = 0; s < KST; ++s) {
       mbar_init(&k_full[s], kWriters);
       mbar_init(&k_empty[s], 1);
@@ -206,7 +271,13 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     }
     mbar_init(p_full, 4);
     mbar_init(o_done, 1);
+    mbar_init(o_full, 1);
+    mbar_init(o_empty, 4);
     mbar_init(mma_done, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&claim_full[s], 1);
+      mbar_init(&claim_empty[s], kFp4 ? 9 : 6);  // the warps that walk
+    }
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -218,125 +289,152 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int rows = x.tokens * a.group;  // of the 128
-  const int pos0 = x.rows.past + x.t0;
+  pdl_wait();
+  pdl_trigger();
+  TileWalk walk{p, smem + L::kBarOff, claim_full, claim_empty, warp == W::kMma, warp == W::kMma};
+  Tile x;
+  int at = -1;
+  bool ok = true;
+  int g0 = 0;    // key blocks of the tiles before this one: stages and phases run on
+  int tile_n = 0;  // tiles before this one
 
   if (!kFp4 && warp == 0) {
-    // ---- Q tile, then K and V blocks in the order the MMAs use them: K0, K1, V0, K2, V1, ...
+    // ---- Q tiles, and K and V blocks in the order the MMAs use them: K0, K1, V0, K2, V1, ...
     const int shift = a.seqs.page_shift, page_rows = 1 << shift;
     const int box_rows = min(page_rows, BN), boxes = BN / box_rows;
-    const int32_t* ids = a.seqs.page_table + b * a.seqs.max_pages;
-    const int last_page = (x.kv_len - 1) >> shift;
     const int none = static_cast<int>(a.seqs.num_pages);  // outside the map: reads as zeros
-    if (lane == 0) {
-      mbar_arrive_expect_tx(q_full, p.q_bytes);
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-        tma_load_4d(smem + c * L::kBox, &tq, c * 64, kvh * a.group, static_cast<int>(x.rows.row0) + x.t0, 0, q_full);
-    }
-    auto page_for = [&](int j) {  // of lane's box of block j
-      int page = none;
-      const int i = j < nblocks ? (key_of(j) >> shift) + lane : 0;
-      if (lane < boxes && j < nblocks && i <= last_page) {
-        page = ids[i];
-        if (page < 0 || page >= none) {
-          set_device_error(a.seqs.err, kDevErrPageIndex);
-          page = none;
+    int k_issued = 0, v_issued = 0, q_issued = 0;
+    while (ok && walk.next(x, at, lane == 0, abort_flag, ok)) {
+      const int32_t* ids = a.seqs.page_table + x.b * a.seqs.max_pages;
+      const int last_page = (x.kv_len - 1) >> shift;
+      auto page_for = [&](int j) {  // of lane's box of step j
+        int page = none;
+        const int i = j < x.nblocks ? (x.key_of(j) >> shift) + lane : 0;
+        if (lane < boxes && j < x.nblocks && i <= last_page) {
+          page = ids[i];
+          if (page < 0 || page >= none) {
+            set_device_error(a.seqs.err, kDevErrPageIndex);
+            page = none;
+          }
         }
-      }
-      return page;
-    };
-    int k_issued = 0, v_issued = 0;
-    bool ok = true;
-    auto load = [&](int j, int page, bool is_k) {
-      const int st = is_k ? j % KST : j % VST, round = is_k ? j / KST : j / VST;
-      uint64_t* empty = is_k ? &k_empty[st] : &v_empty[st];
-      uint64_t* full = is_k ? &k_full[st] : &v_full[st];
-      const bool free_stage = mbar_wait(empty, (round & 1) ^ 1) && *abort_flag == 0;
-      if (!__all_sync(0xffffffffu, free_stage)) return false;
-      uint8_t* dst = smem + (is_k ? L::kKOff : L::kVOff) + st * L::kKVBytes;
-      if (lane == 0) mbar_arrive_expect_tx(full, L::kKVBytes);
-      __syncwarp();
-      if (lane < boxes) {
-        const int row = key_of(j) & (page_rows - 1);
+        return page;
+      };
+      auto load = [&](int j, int page, bool is_k) {
+        const int g = g0 + j;
+        const int st = is_k ? g % KST : g % VST, round = is_k ? g / KST : g / VST;
+        uint64_t* empty = is_k ? &k_empty[st] : &v_empty[st];
+        uint64_t* full = is_k ? &k_full[st] : &v_full[st];
+        const bool free_stage = mbar_wait(empty, (round & 1) ^ 1) && *abort_flag == 0;
+        if (!__all_sync(0xffffffffu, free_stage)) return false;
+        uint8_t* dst = smem + (is_k ? L::kKOff : L::kVOff) + st * L::kKVBytes;
+        if (lane == 0) mbar_arrive_expect_tx(full, L::kKVBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          const int row = x.key_of(j) & (page_rows - 1);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(dst + c * (BN * 128) + lane * box_rows * 128, is_k ? &tk : &tv, c * 64, row, x.kvh, page, full);
+        }
+        __syncwarp();
+        (is_k ? k_issued : v_issued) = g + 1;
+        return true;
+      };
+      // the ids of the steps ahead are asked for before they are needed
+      int page0 = page_for(0), page1 = page_for(1), page2 = page_for(2);
+      // K of the first step does not wait for the Q tile's buffer
+      ok = load(0, page0, true);
+      if (!ok) break;
+      const bool q_free = mbar_wait(q_empty, (tile_n & 1) ^ 1) && *abort_flag == 0;
+      ok = __all_sync(0xffffffffu, q_free);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, p.q_bytes);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(dst + c * (BN * 128) + lane * box_rows * 128, is_k ? &tk : &tv, c * 64, row, kvh, page, full);
+          tma_load_4d(smem + c * L::kBox, &tq, c * 64, x.kvh * a.group, static_cast<int>(x.rows.row0) + x.t0, 0, q_full);
       }
       __syncwarp();
-      (is_k ? k_issued : v_issued) = j + 1;
-      return true;
-    };
-    // the ids of the blocks ahead are asked for before they are needed
-    int page0 = page_for(0), page1 = page_for(1), page2 = page_for(2);
-    ok = load(0, page0, true);
-    for (int j = 0; j < nblocks && ok; ++j) {
-      const int page3 = page_for(j + 3);
-      if (j + 1 < nblocks) ok = load(j + 1, page1, true);
-      if (ok) ok = load(j, page0, false);
-      page0 = page1;
-      page1 = page2;
-      page2 = page3;
+      q_issued = tile_n + 1;
+      for (int j = 0; j < x.nblocks && ok; ++j) {
+        const int page3 = page_for(j + 3);
+        if (j + 1 < x.nblocks) ok = load(j + 1, page1, true);
+        if (ok) ok = load(j, page0, false);
+        page0 = page1;
+        page1 = page2;
+        page2 = page3;
+      }
+      g0 += x.nblocks;
+      ++tile_n;
     }
     if (!ok && lane == 0) {
       set_device_error(a.seqs.err, kDevErrAttentionTimeout);
       *abort_flag = 1;
     }
     // no copy may still be writing shared memory when the CTA exits
-    mbar_wait(q_full, 0);
-    for (int j = max(0, k_issued - KST); j < k_issued; ++j) mbar_wait(&k_full[j % KST], (j / KST) & 1);
-    for (int j = max(0, v_issued - VST); j < v_issued; ++j) mbar_wait(&v_full[j % VST], (j / VST) & 1);
+    if (q_issued > 0) mbar_wait(q_full, (q_issued - 1) & 1);
+    for (int g = max(0, k_issued - KST); g < k_issued; ++g) mbar_wait(&k_full[g % KST], (g / KST) & 1);
+    for (int g = max(0, v_issued - VST); g < v_issued; ++g) mbar_wait(&v_full[g % VST], (g / VST) & 1);
   } else if (warp == W::kMma) {
     if (lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, BM, BN);
       constexpr uint32_t idesc_o = umma_idesc_f16_bmn(kBf16, BM, D);
       const uint32_t q_addr = smem_u32(smem);
-      auto qk = [&](int j) -> bool {
-        const int s = j % KST, sb = j & 1;
-        if (!mbar_wait(&k_full[s], (j / KST) & 1)) return false;
-        if (!mbar_wait(&s_empty[sb], ((j >> 1) & 1) ^ 1) || *abort_flag) return false;
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + L::kKOff + s * L::kKVBytes);
+      while (ok && walk.next(x, at, false, abort_flag, ok)) {
+        auto qk = [&](int j) -> bool {
+          const int g = g0 + j, s = g % KST, sb = g & 1;
+          if (!mbar_wait(&k_full[s], (g / KST) & 1)) return false;
+          if (!mbar_wait(&s_empty[sb], ((g >> 1) & 1) ^ 1) || *abort_flag) return false;
+          tc_fence_after();
+          const uint32_t k_addr = smem_u32(smem + L::kKOff + s * L::kKVBytes);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t ad = umma_desc_sw128(q_addr + (kk / 4) * L::kBox) + 2 * (kk % 4);
-          const uint64_t bd = umma_desc_sw128(k_addr + (kk / 4) * (BN * 128)) + 2 * (kk % 4);
-          umma_f16(tmem + static_cast<uint32_t>(sb * BN), ad, bd, idesc_s, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&k_empty[s]);
-        umma_commit(&s_full[sb]);
-        return true;
-      };
-      auto pv = [&](int j) -> bool {
-        const int s = j % VST;
-        if (!mbar_wait(p_full, j & 1)) return false;
-        if (!mbar_wait(&v_full[s], (j / VST) & 1) || *abort_flag) return false;
-        tc_fence_after();
-        const uint32_t v_addr = smem_u32(smem + L::kVOff + s * L::kKVBytes);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t ad = umma_desc_sw128(q_addr + (kk / 4) * L::kBox) + 2 * (kk % 4);
+            const uint64_t bd = umma_desc_sw128(k_addr + (kk / 4) * (BN * 128)) + 2 * (kk % 4);
+            umma_f16(tmem + static_cast<uint32_t>(sb * BN), ad, bd, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&k_empty[s]);
+          umma_commit(&s_full[sb]);
+          if (j == x.nblocks - 1) umma_commit(q_empty);
+          return true;
+        };
+        auto pv = [&](int j) -> bool {
+          const int g = g0 + j, s = g % VST;
+          if (!mbar_wait(p_full, g & 1)) return false;
+          if (!mbar_wait(&v_full[s], (g / VST) & 1) || *abort_flag) return false;
+          // O of the tile before has been read
+          if (j == 0 && tile_n > 0 && !mbar_wait(o_empty, (tile_n - 1) & 1)) return false;
+          tc_fence_after();
+          const uint32_t v_addr = smem_u32(smem + L::kVOff + s * L::kKVBytes);
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
-          // P_j over S_j's columns: S_{j+2}, issued later, cannot overwrite it before it is read
-          const uint64_t bd = umma_desc_mn_sw128(v_addr + kk * 16 * 128, BN * 128, 1024);
-          umma_f16_ts(tmem + L::kOCol, tmem + static_cast<uint32_t>((j & 1) * BN + kk * 8), bd, idesc_o,
-                      (j > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            // P_j over S_j's columns: S_{j+2}, issued later, cannot overwrite it before it is read
+            const uint64_t bd = umma_desc_mn_sw128(v_addr + kk * 16 * 128, BN * 128, 1024);
+            umma_f16_ts(tmem + L::kOCol, tmem + static_cast<uint32_t>((g & 1) * BN + kk * 8), bd, idesc_o,
+                        (j > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&v_empty[s]);
+          umma_commit(o_done);
+          if (j == x.nblocks - 1) umma_commit(o_full);
+          return true;
+        };
+        ok = mbar_wait(q_full, tile_n & 1);
+        if (ok) ok = qk(0);
+        for (int j = 0; j < x.nblocks && ok; ++j) {
+          if (j + 1 < x.nblocks) ok = qk(j + 1);
+          if (ok) ok = pv(j);
         }
-        umma_commit(&v_empty[s]);
-        umma_commit(o_done);
-        return true;
-      };
-      bool ok = mbar_wait(q_full, 0);
-      if (ok) ok = qk(0);
-      for (int j = 0; j < nblocks && ok; ++j) {
-        if (j + 1 < nblocks) ok = qk(j + 1);
-        if (ok) ok = pv(j);
+        g0 += x.nblocks;
+        ++tile_n;
       }
       if (!ok) {
         set_device_error(a.seqs.err, kDevErrAttentionTimeout);
         *abort_flag = 1;
       }
-      // every issued MMA has finished before the CTA releases tensor memory
+      // every issued MMA has finished before the CTA releases tensor memory, and no
+      // answer is still to be written
       umma_commit(mma_done);
       mbar_wait(mma_done, 0);
+      if (walk.open) mbar_wait(&claim_full[walk.n & 1], (walk.n >> 1) & 1);
     }
   } else if (kFp4 && warp >= W::kConvert) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::kConvertRegs));
@@ -346,34 +444,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     constexpr int WORDS = D / 16;  // code words of half a row
     constexpr int SB = D / 32;     // scale bytes
     const int shift = a.seqs.page_shift, page_rows = 1 << shift;
-    const int32_t* ids = a.seqs.page_table + b * a.seqs.max_pages;
     const int64_t block_bytes = fp4_block_bytes(page_rows, D);
     const uint8_t* pages[2] = {static_cast<const uint8_t*>(a.k_pages), static_cast<const uint8_t*>(a.v_pages)};
-    auto page_for = [&](int j) {
-      const int key = j < nblocks ? key_of(j) + key_row : -1;
-      if (key < 0 || key >= x.kv_len || key < x.key_lo) return -1;
-      const int page = ids[key >> shift];
-      if (page < 0 || page >= a.seqs.num_pages) {
-        set_device_error(a.seqs.err, kDevErrPageIndex);
-        return -1;
-      }
-      return page;
-    };
-    auto fetch = [&](int j, int page, int which, uint32_t (&w)[WORDS], uint32_t& sc) {
-#pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[i] = 0u;
-      sc = 0u;  // rows that are not of the tile's keys: zeros
-      if (page < 0) return;
-      const int r = (key_of(j) + key_row) & (page_rows - 1);
-      const uint8_t* base = pages[which] + (static_cast<int64_t>(page) * a.hkv + kvh) * block_bytes;
-#pragma unroll
-      for (int i = 0; i < WORDS; i += 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(base + r * (D / 2) + half * (D / 4) + i * 4);
-        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-      }
-      const uint8_t* s = base + page_rows * (D / 2) + r * (D / 16) + half * SB;
-      sc = SB == 4 ? *reinterpret_cast<const uint32_t*>(s) : static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(s));
-    };
     // the half row as swizzled 16-byte chunks of halves, then the warp's arrival
     auto put = [&](uint8_t* stage, const uint32_t (&w)[WORDS], uint32_t sc, uint64_t* full) {
       uint8_t* row = stage + (D == 128 ? half * (BN * 128) : 0) + key_row * 128;
@@ -389,30 +461,59 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     };
-    uint32_t kw[WORDS], vw[WORDS], ks, vs;
-    int page0 = page_for(0), page1 = page_for(1);
-    fetch(0, page0, 0, kw, ks);
-    fetch(0, page0, 1, vw, vs);
-    bool ok = true;
-    // V of block j is converted after K of block j + 1: the order of the MMAs
-    for (int j = 0; j <= nblocks && ok; ++j) {
-      const int page2 = page_for(j + 2);
-      if (j < nblocks) {
-        const int st = j % KST;
-        ok = warp_wait(&k_empty[st], ((j / KST) & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        put(smem + L::kKOff + st * L::kKVBytes, kw, ks, &k_full[st]);
-        fetch(j + 1, page1, 0, kw, ks);
+    while (ok && walk.next(x, at, lane == 0, abort_flag, ok)) {
+      const int32_t* ids = a.seqs.page_table + x.b * a.seqs.max_pages;
+      auto page_for = [&](int j) {
+        const int key = j < x.nblocks ? x.key_of(j) + key_row : -1;
+        if (key < 0 || key >= x.kv_len || key < x.key_lo) return -1;
+        const int page = ids[key >> shift];
+        if (page < 0 || page >= a.seqs.num_pages) {
+          set_device_error(a.seqs.err, kDevErrPageIndex);
+          return -1;
+        }
+        return page;
+      };
+      auto fetch = [&](int j, int page, int which, uint32_t (&w)[WORDS], uint32_t& sc) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+        sc = 0u;  // rows that are not of the tile's keys: zeros
+        if (page < 0) return;
+        const int r = (x.key_of(j) + key_row) & (page_rows - 1);
+        const uint8_t* base = pages[which] + (static_cast<int64_t>(page) * a.hkv + x.kvh) * block_bytes;
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(base + r * (D / 2) + half * (D / 4) + i * 4);
+          w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+        }
+        const uint8_t* s = base + page_rows * (D / 2) + r * (D / 16) + half * SB;
+        sc = SB == 4 ? *reinterpret_cast<const uint32_t*>(s) : static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(s));
+      };
+      uint32_t kw[WORDS], vw[WORDS], ks, vs;
+      int page0 = page_for(0), page1 = page_for(1);
+      fetch(0, page0, 0, kw, ks);
+      fetch(0, page0, 1, vw, vs);
+      // V of step j is converted after K of step j + 1: the order of the MMAs
+      for (int j = 0; j <= x.nblocks; ++j) {
+        const int page2 = page_for(j + 2);
+        if (j < x.nblocks) {
+          const int g = g0 + j, st = g % KST;
+          ok = warp_wait(&k_empty[st], ((g / KST) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          put(smem + L::kKOff + st * L::kKVBytes, kw, ks, &k_full[st]);
+          fetch(j + 1, page1, 0, kw, ks);
+        }
+        if (j > 0) {
+          const int g = g0 + j - 1, st = g % VST;
+          ok = warp_wait(&v_empty[st], ((g / VST) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          put(smem + L::kVOff + st * L::kKVBytes, vw, vs, &v_full[st]);
+          fetch(j, page0, 1, vw, vs);
+        }
+        page0 = page1;
+        page1 = page2;
       }
-      if (j > 0) {
-        const int st = (j - 1) % VST;
-        ok = warp_wait(&v_empty[st], (((j - 1) / VST) & 1) ^ 1, abort_flag);
-        if (!ok) break;
-        put(smem + L::kVOff + st * L::kKVBytes, vw, vs, &v_full[st]);
-        fetch(j, page0, 1, vw, vs);
-      }
-      page0 = page1;
-      page1 = page2;
+      g0 += x.nblocks;
+      ++tile_n;
     }
     if (!ok && lane == 0) {
       set_device_error(a.seqs.err, kDevErrAttentionTimeout);
@@ -423,216 +524,210 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;  // tensor-memory lane = row of the tile
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
-    const int pos = row < rows ? pos0 + tok : -1;  // rows past the tile compute what nobody reads
-    const int lo = max(-1, pos - a.window);        // sees the keys in (lo, pos]
-    const float slope = a.slopes && row < rows ? a.slopes[head] * kLog2e : 0.f;
+    const int tok = row / a.group, in_group = row - tok * a.group;
     const bool cap = a.softcap > 0.f, bias = a.slopes != nullptr;
     const float cap_out = a.softcap * kLog2e;
-    float in_scale = cap ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
-    if constexpr (kFp4) {
-      // this thread's row of the Q tile, scaled by 2^-e with 2^e <= max|q| < 2^(e+1)
-      const T* q = static_cast<const T*>(a.q) + ((x.rows.row0 + x.t0 + tok) * a.hq + head) * D;
-      float big = 0.f;
-      if (row < rows) {
+    while (ok && walk.next(x, at, false, abort_flag, ok)) {
+      const int rows = x.tokens * a.group;  // of the 128
+      const int pos0 = x.rows.past + x.t0;
+      const int head = x.kvh * a.group + in_group;
+      const int pos = row < rows ? pos0 + tok : -1;  // rows past the tile compute what nobody reads
+      const int lo = max(-1, pos - a.window);        // sees the keys in (lo, pos]
+      const float slope = bias && row < rows ? a.slopes[head] * kLog2e : 0.f;
+      float in_scale = cap ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
+      if constexpr (kFp4) {
+        // this thread's row of the Q tile (every S of the tile before has been read, so
+        // its Q has too), scaled by 2^-e with 2^e <= max|q| < 2^(e+1)
+        const T* q = static_cast<const T*>(a.q) + ((x.rows.row0 + x.t0 + tok) * a.hq + head) * D;
+        float big = 0.f;
+        if (row < rows) {
+#pragma unroll 4
+          for (int c = 0; c < D; c += 8) {
+            const Vec16<T> in = load16(q + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(to_f32(in.e[i])));
+          }
+        }
+        const int e = max(-120, min(120, static_cast<int>((__float_as_uint(big) >> 23) & 255u) - 127));
+        const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
+        in_scale *= __uint_as_float(static_cast<unsigned>(127 + e) << 23);
 #pragma unroll 4
         for (int c = 0; c < D; c += 8) {
-          const Vec16<T> in = load16(q + c);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(to_f32(in.e[i])));
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (row < rows) {
+            const Vec16<T> in = load16(q + c);
+            v.x = pack16<MT>(to_f32(in.e[0]) * down, to_f32(in.e[1]) * down);
+            v.y = pack16<MT>(to_f32(in.e[2]) * down, to_f32(in.e[3]) * down);
+            v.z = pack16<MT>(to_f32(in.e[4]) * down, to_f32(in.e[5]) * down);
+            v.w = pack16<MT>(to_f32(in.e[6]) * down, to_f32(in.e[7]) * down);
+          }
+          *reinterpret_cast<uint4*>(smem + (c >> 6) * L::kBox + row * 128 + ((((c >> 3) & 7) ^ (row & 7)) << 4)) = v;
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
       }
-      const int e = max(-120, min(120, static_cast<int>((__float_as_uint(big) >> 23) & 255u) - 127));
-      const float down = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
-      in_scale *= __uint_as_float(static_cast<unsigned>(127 + e) << 23);
-#pragma unroll 4
-      for (int c = 0; c < D; c += 8) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) {
-          const Vec16<T> in = load16(q + c);
-          v.x = pack16<MT>(to_f32(in.e[0]) * down, to_f32(in.e[1]) * down);
-          v.y = pack16<MT>(to_f32(in.e[2]) * down, to_f32(in.e[3]) * down);
-          v.z = pack16<MT>(to_f32(in.e[4]) * down, to_f32(in.e[5]) * down);
-          v.w = pack16<MT>(to_f32(in.e[6]) * down, to_f32(in.e[7]) * down);
-        }
-        *reinterpret_cast<uint4*>(smem + (c >> 6) * L::kBox + row * 128 + ((((c >> 3) & 7) ^ (row & 7)) << 4)) = v;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    }
-    const float mul = cap || bias ? 1.f : in_scale;  // what the scores still want when the maximum is taken
-    float m_used = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < nblocks; ++j) {
-      const int sb = j & 1;
-      if (!warp_wait(&s_full[sb], (j >> 1) & 1, abort_flag)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float s[BN];
-#pragma unroll
-      for (int c = 0; c < BN / 32; ++c)
-        tmem_ld_32x32b_x32(lane_base + static_cast<uint32_t>(sb * BN + c * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[sb]);
-
-      const int key0 = key_of(j);
-      if (cap) {
-#pragma unroll
-        for (int i = 0; i < BN; ++i) s[i] = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(s[i] * in_scale));
-      }
-      if (bias) {
-        const float first = cap ? 1.f : in_scale, at = slope * static_cast<float>(key0 - pos);
-#pragma unroll
-        for (int i = 0; i < BN; i += 2) {
-          const float2 far = fma2(make_float2(slope, slope), make_float2(i, i + 1), make_float2(at, at));
-          const float2 y = fma2(make_float2(s[i], s[i + 1]), make_float2(first, first), far);
-          s[i] = y.x;
-          s[i + 1] = y.y;
-        }
-      }
-      if (key0 + BN - 1 > pos0 || key0 <= pos0 + x.tokens - 1 - a.window) {
-        const int end = pos - key0, begin = lo - key0;
-#pragma unroll
-        for (int i = 0; i < BN; ++i)
-          if (i > end || i <= begin) s[i] = -INFINITY;
-      }
-      float mc[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mc[k] = max3f(s[2 * k], s[2 * k + 1], -INFINITY);
-#pragma unroll
-      for (int i = 16; i < BN; i += 16)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mc[k] = max3f(mc[k], s[i + 2 * k], s[i + 2 * k + 1]);
-      const float m_blk = max3f(max3f(mc[0], mc[1], mc[2]), max3f(mc[3], mc[4], mc[5]), fmaxf(mc[6], mc[7])) * mul;
-      float alpha = 1.f;
-      bool rescale_row = false;
-      if (m_blk > m_used + kRescale) {  // from -inf: any visible key
-        if (m_used != -INFINITY) {
-          alpha = exp2_approx(m_used - m_blk);
-          rescale_row = row < rows;
-        }
-        l *= alpha;
-        m_used = m_blk;
-      }
-      if (__any_sync(0xffffffffu, rescale_row)) {
-        // O holds P_0 V_0 + ... + P_{j-1} V_{j-1}: wait for the last of them. S_j's
-        // commit covered P V_{j-2}, so o_done is at most one phase behind.
-        if (!warp_wait(o_done, (j - 1) & 1, abort_flag)) {
+      const float mul = cap || bias ? 1.f : in_scale;  // what the scores still want when the maximum is taken
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < x.nblocks; ++j) {
+        const int g = g0 + j, sb = g & 1;
+        if (!warp_wait(&s_full[sb], (g >> 1) & 1, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        float s[BN];
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c)
+          tmem_ld_32x32b_x32(lane_base + static_cast<uint32_t>(sb * BN + c * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[sb]);
+
+        const int key0 = x.key_of(j);
+        if (cap) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i) s[i] = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(s[i] * in_scale));
+        }
+        if (bias) {
+          const float first = cap ? 1.f : in_scale, far0 = slope * static_cast<float>(key0 - pos);
+#pragma unroll
+          for (int i = 0; i < BN; i += 2) {
+            const float2 far = fma2(make_float2(slope, slope), make_float2(i, i + 1), make_float2(far0, far0));
+            const float2 y = fma2(make_float2(s[i], s[i + 1]), make_float2(first, first), far);
+            s[i] = y.x;
+            s[i + 1] = y.y;
+          }
+        }
+        if (key0 + BN - 1 > pos0 || key0 <= pos0 + x.tokens - 1 - a.window) {
+          const int end = pos - key0, begin = lo - key0;
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            if (i > end || i <= begin) s[i] = -INFINITY;
+        }
+        float mc[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mc[k] = max3f(s[2 * k], s[2 * k + 1], -INFINITY);
+#pragma unroll
+        for (int i = 16; i < BN; i += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mc[k] = max3f(mc[k], s[i + 2 * k], s[i + 2 * k + 1]);
+        const float m_blk = max3f(max3f(mc[0], mc[1], mc[2]), max3f(mc[3], mc[4], mc[5]), fmaxf(mc[6], mc[7])) * mul;
+        float alpha = 1.f;
+        bool rescale_row = false;
+        if (m_blk > m_used + kRescale) {  // from -inf: any visible key
+          if (m_used != -INFINITY) {
+            alpha = exp2_approx(m_used - m_blk);
+            rescale_row = row < rows;
+          }
+          l *= alpha;
+          m_used = m_blk;
+        }
+        if (__any_sync(0xffffffffu, rescale_row)) {
+          // O holds P_0 V_0 + ... + P_{j-1} V_{j-1}: wait for the last of them. S_j's
+          // commit covered P V_{j-2}, so o_done is at most one phase behind.
+          if (!warp_wait(o_done, (g - 1) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(lane_base + L::kOCol + c, r);
-          tmem_ld_wait();
+          for (int c = 0; c < D; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(lane_base + L::kOCol + c, r);
+            tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-          tmem_st_32x32b_x32(lane_base + L::kOCol + c, r);
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+            tmem_st_32x32b_x32(lane_base + L::kOCol + c, r);
+          }
+          tmem_st_wait();
         }
+        const float neg = m_used == -INFINITY ? 0.f : -m_used;
+        uint32_t pk[BN / 2];
+        float2 rs[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < BN; i += 2) {
+          float2 e = fma2(make_float2(s[i], s[i + 1]), make_float2(mul, mul), make_float2(neg, neg));
+          e.x = exp2_approx(e.x);
+          e.y = exp2_approx(e.y);
+          rs[(i / 2) & 3] = add2(rs[(i / 2) & 3], e);
+          pk[i / 2] = pack16<MT>(e.x, e.y);
+        }
+        const float2 sum = add2(add2(rs[0], rs[1]), add2(rs[2], rs[3]));
+        l += sum.x + sum.y;
+        // V rows that no row of the tile sees may hold anything: a zero weight must meet
+        // a zero (converters write zeros there)
+        const int z_end = x.kv_len - key0, z_begin = x.key_lo - key0;
+        const bool stale = !kFp4 && (z_end < BN || z_begin > 0);
+        if (stale) {
+          if (!warp_wait(&v_full[g % VST], (g / VST) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint8_t* vt = smem + L::kVOff + (g % VST) * L::kKVBytes;
+          for (int c = row; c < BN * (D / 8); c += BM) {
+            const int box = c / (BN * 8), rem = c - box * (BN * 8);
+            if (rem / 8 >= z_end || rem / 8 < z_begin)
+              *reinterpret_cast<uint4*>(vt + box * BN * 128 + rem * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        tmem_st_32x32b_x32(lane_base + static_cast<uint32_t>(sb * BN), pk);
         tmem_st_wait();
+        if (stale) fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
       }
-      const float neg = m_used == -INFINITY ? 0.f : -m_used;
-      uint32_t pk[BN / 2];
-      float2 rs[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+      // the tile's last P V (o_done may be two phases behind here, o_full completes once a tile)
+      if (!ok || !warp_wait(o_full, tile_n & 1, abort_flag)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const bool whole = x.shares == 1;
+      const float inv = l > 0.f ? a.v_scale / l : 0.f;
+      T* dst = static_cast<T*>(a.out) + ((x.rows.row0 + x.t0 + tok) * a.hq + head) * D;
+      // the share's O, unnormalised, its maximum and sum
+      const int64_t part = ((static_cast<int64_t>(x.b) * a.hkv + x.kvh) * p.tiles + x.tile) * p.splits + x.share;
+      float* part_dst = p.part_o + (part * BM + row) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(lane_base + L::kOCol + c, r);
+        tmem_ld_wait();
+        if (c + 32 == D) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(o_empty);  // the next tile may write O
+        }
+        if (row >= rows) continue;
+        if (whole) {
+          uint32_t v[16];
 #pragma unroll
-      for (int i = 0; i < BN; i += 2) {
-        float2 e = fma2(make_float2(s[i], s[i + 1]), make_float2(mul, mul), make_float2(neg, neg));
-        e.x = exp2_approx(e.x);
-        e.y = exp2_approx(e.y);
-        rs[(i / 2) & 3] = add2(rs[(i / 2) & 3], e);
-        pk[i / 2] = pack16<MT>(e.x, e.y);
-      }
-      const float2 sum = add2(add2(rs[0], rs[1]), add2(rs[2], rs[3]));
-      l += sum.x + sum.y;
-      // V rows that no row of the tile sees may hold anything: a zero weight must meet a zero
-      const int z_end = x.kv_len - key0, z_begin = x.key_lo - key0;
-      const bool stale = !kFp4 && (z_end < BN || z_begin > 0);  // the converters write zeros there
-      if (stale) {
-        if (!warp_wait(&v_full[j % VST], (j / VST) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        uint8_t* vt = smem + L::kVOff + (j % VST) * L::kKVBytes;
-        for (int c = row; c < BN * (D / 8); c += BM) {
-          const int box = c / (BN * 8), rem = c - box * (BN * 8);
-          if (rem / 8 >= z_end || rem / 8 < z_begin)
-            *reinterpret_cast<uint4*>(vt + box * BN * 128 + rem * 16) = make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < 16; ++i) v[i] = pack16<T>(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
+          if (p.wide_out) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+              asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c + 2 * i), "r"(v[i]), "r"(v[i + 1]),
+                           "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+                           : "memory");
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(dst + c + 2 * i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part_dst + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
         }
       }
-      tmem_st_32x32b_x32(lane_base + static_cast<uint32_t>(sb * BN), pk);
-      tmem_st_wait();
-      if (stale) fence_proxy_async_smem();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (!whole && row < rows) p.part_ml[part * BM + row] = make_float2(m_used, l);
+      g0 += x.nblocks;
+      ++tile_n;
     }
     if (!ok && lane == 0) {
       set_device_error(a.seqs.err, kDevErrAttentionTimeout);
       *abort_flag = 1;
-    }
-    // every MMA has finished before O is read (o_done may be two phases behind here)
-    bool have_o = ok;
-    if (have_o && !warp_wait(mma_done, 0, abort_flag)) {
-      if (lane == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
-      have_o = false;
-    }
-    tc_fence_after();
-    if (shares > 1) {
-      // the share's O, unnormalised, its maximum and sum
-      const int64_t unit = (static_cast<int64_t>(b) * a.hkv + kvh) * per_split + tile;
-      const int64_t at = (unit * p.splits + share) * BM + row;
-#pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(lane_base + L::kOCol + c, r);
-        tmem_ld_wait();
-        if (row < rows && have_o) {
-          float* dst = p.part_o + at * D + c;
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(dst + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
-        }
-      }
-      if (row < rows) p.part_ml[at] = make_float2(have_o ? m_used : -INFINITY, l);
-    } else {
-      // O / l over the Q tile (the last Q K^T has completed), then whole head rows
-      // of 16-byte chunks to the output
-      const float inv = l > 0.f ? a.v_scale / l : 0.f;
-      uint8_t* orow = smem + row * 128;
-      const int r7 = row & 7;
-#pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(lane_base + L::kOCol + c, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          uint32_t v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] = have_o ? pack16<T>(__uint_as_float(r[q4 * 8 + 2 * i]) * inv, __uint_as_float(r[q4 * 8 + 2 * i + 1]) * inv) : 0u;
-          const int ch = ((c & 63) >> 3) + q4;
-          *reinterpret_cast<uint4*>(orow + (c >> 6) * L::kBox + ((ch ^ r7) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-        }
-      }
-      __syncwarp();
-      // each warp stores its own 32 rows
-      T* out = static_cast<T*>(a.out) + (x.rows.row0 + x.t0) * a.hq * D;
-      constexpr int CPR = D / 8;
-      const int r_end = min(32, rows - quarter * 32);
-      for (int c = lane; c < r_end * CPR; c += 32) {
-        const int r = quarter * 32 + c / CPR, ch = c % CPR;
-        const int rt = r / a.group, rh = kvh * a.group + r - rt * a.group;
-        const uint4 v = *reinterpret_cast<const uint4*>(smem + (ch >> 3) * L::kBox + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-        *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(rt) * a.hq + rh) * D + ch * 8) = v;
-      }
     }
   }
   tc_fence_before();
@@ -644,48 +739,61 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   }
 }
 
-// Merges the shares of a tile in order.
+// Merges the shares of a tile in order. grid = (tiles x (128 x D / 1024), KV heads,
+// sequences); thread = 4 elements of a row. Which shares there are is worked out while
+// the main kernel still runs: positions and starts were final before that began.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_paged_prefill_combine_kernel(const PrefillArgs p) {
-  DLI_PDL_ENTRY();
+  constexpr int CHUNKS = BM * D / 1024;
   const PagedAttnArgs& a = p.a;
-  const int tile = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const Tile x = tile_of(p, b, tile, false);
-  if (x.tokens <= 0) return;
-  const int shares = shares_of(x.blocks, p.splits);
-  if (shares == 1) return;
-  const int64_t unit = (static_cast<int64_t>(b) * a.hkv + kvh) * gridDim.x + tile;
-  const int rows = x.tokens * a.group;
-  for (int c = threadIdx.x; c < rows * (D / 4); c += 256) {
-    const int r = c / (D / 4), d = (c - r * (D / 4)) * 4;
-    const int64_t at = unit * p.splits * BM + r;
-    float top = -INFINITY, den = 0.f;
-    for (int s = 0; s < shares; ++s) top = fmaxf(top, p.part_ml[at + s * BM].x);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < shares; ++s) {
-      const float2 ml = p.part_ml[at + s * BM];
-      if (ml.x == -INFINITY) continue;
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + s * BM) * D + d);
-      const float f = exp2_approx(ml.x - top);
-      den += ml.y * f;
-      sum.x += v.x * f;
-      sum.y += v.y * f;
-      sum.z += v.z * f;
-      sum.w += v.w * f;
+  const int tile = blockIdx.x / CHUNKS, chunk = blockIdx.x % CHUNKS, kvh = blockIdx.y, b = blockIdx.z;
+  const SeqRows sr = seq_rows(a.seqs, b, false);
+  const int t0 = tile * p.tile_tokens, tokens = min(p.tile_tokens, sr.n - t0);
+  const int pos0 = sr.past + t0, key_lo = a.window <= pos0 ? pos0 - a.window + 1 : 0;
+  const int shares = shares_of((pos0 + tokens + BN - 1) / BN - key_lo / BN, p.splits);
+  const int c = chunk * 256 + threadIdx.x;
+  const int r = c / (D / 4), d = (c - r * (D / 4)) * 4;
+  pdl_wait();
+  pdl_trigger();
+  if (tokens <= 0 || shares == 1 || r >= tokens * a.group) return;
+  const int64_t at = ((static_cast<int64_t>(b) * a.hkv + kvh) * p.tiles + tile) * p.splits * BM + r;
+  float top = -INFINITY, den = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < shares; s0 += 4) {
+    float2 ml[4];
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + k < shares) {
+        ml[k] = p.part_ml[at + (s0 + k) * BM];
+        v[k] = *reinterpret_cast<const float4*>(p.part_o + (at + (s0 + k) * BM) * D + d);
+      }
     }
-    const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
-    const float inv = a.v_scale / den;
-    uint2 v;
-    v.x = pack16<T>(sum.x * inv, sum.y * inv);
-    v.y = pack16<T>(sum.z * inv, sum.w * inv);
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((x.rows.row0 + x.t0 + tok) * a.hq + head) * D + d) = v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (ml[k].x == -INFINITY) continue;  // a share in which the row sees no key
+      const float m = fmaxf(top, ml[k].x);
+      const float f = exp2_approx(top - m), f2 = exp2_approx(ml[k].x - m);  // top = -inf: 0
+      top = m;
+      den = den * f + ml[k].y * f2;
+      sum.x = sum.x * f + v[k].x * f2;
+      sum.y = sum.y * f + v[k].y * f2;
+      sum.z = sum.z * f + v[k].z * f2;
+      sum.w = sum.w * f + v[k].w * f2;
+    }
   }
+  const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
+  const float inv = a.v_scale / den;
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((sr.row0 + t0 + tok) * a.hq + head) * D + d) =
+      make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
 }
 
 // ---- host ------------------------------------------------------------------------
 struct PrefillPlan {
-  int64_t tiles, units;
-  int tile_tokens, splits;
+  int64_t tiles, pairs, units;
+  int tile_tokens, splits, pairs_group;
   size_t part_o, workspace;
 };
 
@@ -693,7 +801,10 @@ PrefillPlan plan_prefill(int64_t batch, int64_t hkv, int64_t group, int64_t max_
   PrefillPlan p{};
   p.tile_tokens = static_cast<int>(BM / group);
   p.tiles = ceil_div(max_new, p.tile_tokens);
-  p.units = p.tiles * hkv * batch;
+  p.pairs = hkv * batch;
+  p.units = p.tiles * p.pairs;
+  // pairs of a group: their K and V (2 x 2 bytes an element) within about a quarter of L2
+  p.pairs_group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.pairs, (32ll << 20) / (4 * head_dim * std::max<int64_t>(1, max_keys)))));
   // as many shares of the keys as keep every CTA resident at once, at least 256 keys each
   const int64_t slots = 2ll * sm_count();
   p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({slots / std::max<int64_t>(1, p.units), max_keys / (4 * BN), 64})));
@@ -723,6 +834,9 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
   p.a = a;
   p.tile_tokens = plan.tile_tokens;
   p.splits = plan.splits;
+  p.tiles = static_cast<int>(plan.tiles);
+  p.pairs_group = plan.splits > 1 ? static_cast<int>(std::min<int64_t>(plan.pairs, INT_MAX)) : plan.pairs_group;
+  p.wide_out = aligned(a.out, 32);
   p.q_bytes = static_cast<unsigned>(plan.tile_tokens * a.group * D * 2);
   if (plan.splits > 1) {
     p.part_o = static_cast<float*>(workspace);
@@ -739,12 +853,11 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
     }();
     if (regs < Roles<true>::kLaunchRegs) return fail(DLI_ERR_UNSUPPORTED, "attention_paged: built with too few registers a thread");
   }
-  const dim3 grid(static_cast<unsigned>(plan.tiles * plan.splits), static_cast<unsigned>(a.hkv),
-                  static_cast<unsigned>(a.seqs.batch));
-  launch_pdl(kern, grid, dim3(Roles<kFp4>::kThreads), L::kBytes, stream, p, tq, tk, tv);
+  launch_pdl(kern, dim3(static_cast<unsigned>(plan.units * plan.splits)), dim3(Roles<kFp4>::kThreads), L::kBytes, stream, p, tq, tk, tv);
   if (plan.splits > 1)
     launch_pdl(attn_paged_prefill_combine_kernel<T, D>,
-               dim3(static_cast<unsigned>(plan.tiles), static_cast<unsigned>(a.hkv), static_cast<unsigned>(a.seqs.batch)),
+               dim3(static_cast<unsigned>(plan.tiles * (BM * D / 1024)), static_cast<unsigned>(a.hkv),
+                    static_cast<unsigned>(a.seqs.batch)),
                dim3(256), 0, stream, p);
   return check_launch("attention_paged", plan.splits > 1 ? 2 : 1);
 }
@@ -756,6 +869,8 @@ int64_t keys_of(const PagedAttnArgs& a) {
 }  // namespace
 
 bool paged_prefill_serves(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype) {
+  // the grid's x dimension, and int arithmetic on it
+  if (a.group > BM || ceil_div(a.seqs.max_new, BM / a.group) * a.hkv * static_cast<int64_t>(a.seqs.batch) > (1ll << 30)) return false;
   if ((dtype != DLI_DTYPE_BF16 && dtype != DLI_DTYPE_F16) || (kv_dtype != dtype && kv_dtype != DLI_DTYPE_FP4)) return false;
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (a.group > BM || a.hkv > 65535 || a.seqs.num_pages < 1 || a.seqs.tokens > INT_MAX) return false;

@@ -114,6 +114,32 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// ---- cluster launch control ----------------------------------------------------------
+// Asks the hardware scheduler for the next CTA of this grid that has not started: if
+// there is one it is withdrawn, and the caller does its work. The 16-byte answer
+// arrives in shared memory on `bar`. Not to be asked again after a refusal.
+__device__ __forceinline__ void claim_next_cta(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// blockIdx.x of the CTA an answer stands for, or -1 when none was left.
+__device__ __forceinline__ int claimed_cta(const void* answer) {
+  int won, x;
+  asm volatile(
+      "{\n\t.reg .pred won;\n\t.reg .b128 a;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "mov.b32 %1, 0;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 won, a;\n\t"
+      "selp.b32 %0, 1, 0, won;\n\t"
+      "@won clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+      : "=r"(won), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return won ? x : -1;
+}
+
 // ---- tcgen05 ----------------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
