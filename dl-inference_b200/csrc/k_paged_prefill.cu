@@ -69,9 +69,9 @@ struct PrefillLayout {
   static constexpr int kVOff = kKOff + KST * kKVBytes;
   static constexpr int kBarOff = kVOff + VST * kKVBytes;
   static constexpr int kClaims = 2 * 16;  // answers of the scheduler, then the barriers:
-  // q_full, q_empty, k_full/empty, v_full/empty, s_full[2], s_empty[2], p_full, o_done,
+  // q_full, q_empty, k_full/empty, v_full/empty, s_full[2], p_full[2], o_done,
   // o_full, o_empty, mma_done, claim_full[2], claim_empty[2]
-  static constexpr int kBars = 2 + 2 * KST + 2 * VST + 4 + 5 + 4;
+  static constexpr int kBars = 2 + 2 * KST + 2 * VST + 4 + 4 + 4;
   static constexpr int kBytes = kBarOff + kClaims + kBars * 8 + 16;  // two CTAs fit without alignment slack
   static constexpr uint32_t kTmemCols = 256;
   static constexpr uint32_t kOCol = 2 * BN;
@@ -241,9 +241,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   uint64_t* v_full = k_empty + KST;
   uint64_t* v_empty = v_full + VST;
   uint64_t* s_full = v_empty + VST;
-  uint64_t* s_empty = s_full + 2;
-  uint64_t* p_full = s_empty + 2;
-  uint64_t* o_done = p_full + 1;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_done = p_full + 2;
   uint64_t* o_full = o_done + 1;
   uint64_t* o_empty = o_full + 1;
   uint64_t* mma_done = o_empty + 1;
@@ -267,9 +266,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_empty[s], 4);
+      mbar_init(&p_full[s], 4);
     }
-    mbar_init(p_full, 4);
     mbar_init(o_done, 1);
     mbar_init(o_full, 1);
     mbar_init(o_empty, 4);
@@ -383,7 +381,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         auto qk = [&](int j) -> bool {
           const int g = g0 + j, s = g % KST, sb = g & 1;
           if (!mbar_wait(&k_full[s], (g / KST) & 1)) return false;
-          if (!mbar_wait(&s_empty[sb], ((g >> 1) & 1) ^ 1) || *abort_flag) return false;
+          // S_g's buffer held S and P_{g-2}, whose P V is issued: no wait for the readers
+          if (*abort_flag) return false;
           tc_fence_after();
           const uint32_t k_addr = smem_u32(smem + L::kKOff + s * L::kKVBytes);
 #pragma unroll
@@ -399,7 +398,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         };
         auto pv = [&](int j) -> bool {
           const int g = g0 + j, s = g % VST;
-          if (!mbar_wait(p_full, g & 1)) return false;
+          if (!mbar_wait(&p_full[g & 1], (g >> 1) & 1)) return false;
           if (!mbar_wait(&v_full[s], (g / VST) & 1) || *abort_flag) return false;
           // O of the tile before has been read
           if (j == 0 && tile_n > 0 && !mbar_wait(o_empty, (tile_n - 1) & 1)) return false;
@@ -581,9 +580,6 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         for (int c = 0; c < BN / 32; ++c)
           tmem_ld_32x32b_x32(lane_base + static_cast<uint32_t>(sb * BN + c * 32), *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
         tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[sb]);
 
         const int key0 = x.key_of(j);
         if (cap) {
@@ -677,7 +673,9 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         if (stale) fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        // one barrier per S buffer: a warp may be a block ahead of another, and its arrival
+        // must not stand in for the other's
+        if (lane == 0) mbar_arrive(&p_full[sb]);
       }
       // the tile's last P V (o_done may be two phases behind here, o_full completes once a tile)
       if (!ok || !warp_wait(o_full, tile_n & 1, abort_flag)) {
