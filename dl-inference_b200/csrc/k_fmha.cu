@@ -33,7 +33,9 @@
 // Synchronisation (all mbarriers, every wait bounded; a timeout sets the device
 // error word and winds the CTA down): q_full; k_full/k_empty and v_full/v_empty
 // per ring stage; s_full (MMA commit) and s_empty (4 softmax warps) per S
-// buffer; p_full (4 softmax warps) per P; o_done (MMA commit after each P V):
+// buffer; p_full (4 softmax warps) per S buffer, since with P in tensor memory a warp
+// may be a block ahead of another, and its arrival must not stand in for the other's;
+// o_done (MMA commit after each P V):
 // the softmax warps wait for it before they rescale O (and, with P in shared
 // memory, before they rewrite the single P tile). A P in tensor memory needs
 // no such wait: P_j sits in S_j's buffer, and S_{j+2}, the next write there,
@@ -83,8 +85,8 @@ struct FmhaLayout {
   static constexpr int kPOff = kVOff + VST * kKVBytes;
   static constexpr int kBarOff = kPOff + kPBytes;
   // q_full, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
-  // s_empty[2], p_full, o_done, mma_done
-  static constexpr int kBars = 1 + 2 * KST + 2 * VST + 4 + 3;
+  // s_empty[2], p_full[2], o_done, mma_done
+  static constexpr int kBars = 1 + 2 * KST + 2 * VST + 4 + 4;
   // One CTA per SM rounds its base up to 1 KiB inside the allocation; two CTAs
   // per SM have no room for that slack and rely on the dynamic shared memory
   // base being 1 KiB aligned, which the kernel checks (an error, never a
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(kFmhaThreads, FmhaLayout<D, BNK, PT>::kCtasPer
   uint64_t* s_full = v_empty + VST;
   uint64_t* s_empty = s_full + 2;
   uint64_t* p_full = s_empty + 2;
-  uint64_t* o_done = p_full + 1;
+  uint64_t* o_done = p_full + 2;
   uint64_t* mma_done = o_done + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -184,8 +186,8 @@ __global__ void __launch_bounds__(kFmhaThreads, FmhaLayout<D, BNK, PT>::kCtasPer
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&s_empty[s], 4);
+      mbar_init(&p_full[s], 4);
     }
-    mbar_init(p_full, 4);
     mbar_init(o_done, 1);
     mbar_init(mma_done, 1);
     *abort_flag = 0;
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(kFmhaThreads, FmhaLayout<D, BNK, PT>::kCtasPer
       };
       auto pv = [&](int j) -> bool {
         const int s = j % VST;
-        if (!mbar_wait(p_full, j & 1)) return false;
+        if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1)) return false;
         if (!mbar_wait(&v_full[s], (j / VST) & 1) || *abort_flag) return false;
         tc_fence_after();
         const uint32_t v_addr = smem_u32(smem + L::kVOff + s * L::kKVBytes);
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(kFmhaThreads, FmhaLayout<D, BNK, PT>::kCtasPer
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (lane == 0) mbar_arrive(&p_full[sb]);
     }
     if (!ok && lane == 0) {
       set_device_error(p.err, kDevErrAttentionTimeout);
