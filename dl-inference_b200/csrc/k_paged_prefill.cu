@@ -7,12 +7,16 @@
 // so a K/V block is fetched once for the whole group and a tile's rows differ by
 // few tokens: few blocks are partly masked.
 //
-// The grid is the list of tiles (longest first within groups of (sequence, KV head)
-// pairs whose K/V stay in L2), or of the tiles' `splits` shares of key blocks when the
-// tiles alone do not fill the GPU. A CTA that works claims the next one of the list from
-// the hardware scheduler (cluster launch control) while it computes, so two CTAs per SM
-// stay for the whole call, one tile's end overlaps the next one's start, and a ragged
-// batch is balanced as it runs (which CTA computes a tile changes nothing in it).
+// Many tiles: the grid is their list (longest first within groups of (sequence, KV
+// head) pairs whose K/V stay in L2). A CTA that works claims the next one of the list
+// from the hardware scheduler (cluster launch control) while it computes, so two CTAs
+// per SM stay for the whole call, one tile's end overlaps the next one's start, and a
+// ragged batch is balanced as it runs (which CTA computes a tile changes nothing in it).
+// Few tiles: with room for several CTAs per tile, each tile's keys are split evenly;
+// else the tiles are one list, a tile counting as its sequence's mean number of key
+// blocks and short tiles taking turns with long ones, of which every CTA takes an equal
+// share. Tiles that are cut store their parts' (max, sum, O) in the workspace, and a
+// second kernel merges them in order.
 // 192 threads:
 //   warp 0     loads each Q tile (a box of group x tokens of q by TMA), walks the page
 //              table and loads 64-key K and V blocks (a box per page; boxes past the
@@ -23,7 +27,7 @@
 //   warps 2-5  softmax, one thread per row: S from tensor memory, cap, bias and
 //              mask, running maximum (moved only when it grows by more than 2^8,
 //              so O is seldom rescaled) and sum in fp32, P as 16 bits over S's own
-//              columns; at the end O / sum to the rows, or the share's (max, sum, O)
+//              columns; at the end O / sum to the rows, or the part's (max, sum, O)
 //              to the workspace, while the next tile's first S is computed.
 // 4-bit pages: no producer warp; four converter warps read codes and scales a
 // block ahead into registers and write the K and V stages as halves (E2M1 x E4M3
@@ -43,21 +47,22 @@
 namespace dli_sm100 {
 namespace {
 
-// warps: producer, MMA, 4 softmax; for 4-bit pages 4 softmax, 4 converters, MMA.
-// The softmax warps hold a row of S: with converters in the CTA they take 32
-// registers a thread from those (launched with 96: 128 x 128 + 128 x 64 + 32 x 96).
+// warps: producer, MMA, 4 softmax; for 4-bit pages 4 softmax, 4 converters, MMA,
+// scheduler. The softmax warps hold a row of S: with converters in the CTA they take 32
+// registers a thread from those (launched with 96: 128 x 128 + 128 x 64 + 64 x 96).
 template <bool FP4>
 struct Roles {
-  static constexpr int kThreads = FP4 ? 288 : 192;
+  static constexpr int kThreads = FP4 ? 320 : 192;
   static constexpr int kMma = FP4 ? 8 : 1;
   static constexpr int kSoftmax = FP4 ? 0 : 2;
-  static constexpr int kConvert = 4;  // FP4 only
+  static constexpr int kConvert = 4, kSchedule = 9;  // FP4 only
   static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 128, kConvertRegs = 64;
-  static_assert(128 * kSoftmaxRegs + 128 * kConvertRegs + 32 * kLaunchRegs <= 288 * kLaunchRegs, "register split");
+  static_assert(128 * kSoftmaxRegs + 128 * kConvertRegs + 64 * kLaunchRegs <= 320 * kLaunchRegs, "register split");
 };
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2: P <= 2^8 before O is rescaled
 constexpr int BM = 128, BN = 64;
+constexpr int kMinBlocks = 4;  // shared: no CTA takes fewer key blocks (but the last)
 
 template <int D>
 struct PrefillLayout {
@@ -68,11 +73,11 @@ struct PrefillLayout {
   static constexpr int kKOff = kQBytes;
   static constexpr int kVOff = kKOff + KST * kKVBytes;
   static constexpr int kBarOff = kVOff + VST * kKVBytes;
-  static constexpr int kClaims = 2 * 16;  // answers of the scheduler, then the barriers:
+  static constexpr int kTiles = 16 + 2 * 48;  // the hardware scheduler's answer, two tiles; then the barriers:
   // q_full, q_empty, k_full/empty, v_full/empty, s_full[2], p_full[2], o_done,
-  // o_full, o_empty, mma_done, claim_full[2], claim_empty[2]
-  static constexpr int kBars = 2 + 2 * KST + 2 * VST + 4 + 4 + 4;
-  static constexpr int kBytes = kBarOff + kClaims + kBars * 8 + 16;  // two CTAs fit without alignment slack
+  // o_full, o_empty, mma_done, claimed, near_end, tile_full[2], tile_empty[2]
+  static constexpr int kBars = 2 + 2 * KST + 2 * VST + 4 + 4 + 6;
+  static constexpr int kBytes = kBarOff + kTiles + kBars * 8 + 16;  // two CTAs fit without alignment slack
   static constexpr uint32_t kTmemCols = 256;
   static constexpr uint32_t kOCol = 2 * BN;
   static_assert(kBytes <= 115712, "two CTAs per SM");
@@ -83,100 +88,239 @@ struct PrefillArgs {
   PagedAttnArgs a;
   int tile_tokens;  // 128 / group
   int tiles;        // of a sequence of max_new tokens
-  int splits;
+  int ctas;         // of the main kernel, when shared or split
+  int split;        // few tiles, several CTAs each: parts of a tile's keys (else 1)
+  int shared;       // few tiles: equal shares of their list
   int pairs_group;  // (sequence, KV head) pairs whose tiles are interleaved
   int wide_out;     // out is 32-byte aligned
-  float* part_o;    // [units * splits][128][D]
-  float2* part_ml;  // [units * splits][128]
+  float* part_o;    // [slots][D / 4][128][4]
+  float2* part_ml;  // [slots][128]
   unsigned q_bytes; // of the Q box
 };
 
-// The shares of a tile's key blocks: at least 4 blocks each.
-__device__ __forceinline__ int shares_of(int blocks, int splits) { return max(1, min(splits, blocks / 4)); }
-
-struct Tile {
-  SeqRows rows;
-  int b, kvh, tile, share, shares;
-  int t0, tokens;      // of the tile
-  int kv_len, key_lo;  // keys any of its rows sees: [key_lo, kv_len)
-  int block_first, nblocks;
+// A tile, or the part of one at hand; 48 bytes, as it lies in shared memory.
+struct alignas(16) Tile {
+  int b, kvh, row0, past;
+  int t0, tokens;            // of the tile
+  int kv_len, key_lo;        // keys any of its rows sees: [key_lo, kv_len)
+  int block_first, nblocks;  // of the part; no blocks: the end
+  int slot;                  // of the part in the workspace, -1: the whole tile
+  int unused;
   // the last keys first: with a distance bias the maximum is then met early, and O is
   // not rescaled block after block
   __device__ __forceinline__ int key_of(int j) const { return (block_first + nblocks - 1 - j) * BN; }
 };
+static_assert(sizeof(Tile) == 48, "three 16-byte words");
 
-// Tile (or share) `at` of the list; false when there is nothing to do in it. Order:
-// groups of pairs, within a group the longest tiles first, their shares, the pairs.
-__device__ __forceinline__ bool tile_at(const PrefillArgs& p, int at, Tile& x, bool report) {
-  const int pairs = p.a.hkv * p.a.seqs.batch;
-  const int per_pair = p.tiles * p.splits;
-  const int group = at / per_pair / p.pairs_group;  // at < pairs * per_pair
-  const int first = group * p.pairs_group, size = min(p.pairs_group, pairs - first);
-  const int in_group = at - first * per_pair;
-  const int rank = in_group / size, pair = first + in_group - rank * size;
-  x.b = pair / p.a.hkv;
-  x.kvh = pair - x.b * p.a.hkv;
-  x.tile = p.tiles - 1 - rank / p.splits;
-  x.share = rank % p.splits;
-  x.rows = seq_rows(p.a.seqs, x.b, report && x.tile == 0);
-  x.t0 = x.tile * p.tile_tokens;
-  x.tokens = min(p.tile_tokens, x.rows.n - x.t0);
+// Sets x to all of tile `tile` of sequence b; false when it has no tokens.
+__device__ __forceinline__ bool tile_set(const PrefillArgs& p, const SeqRows& rows, int b, int kvh, int tile, Tile& x) {
+  x.b = b;
+  x.kvh = kvh;
+  x.row0 = static_cast<int>(rows.row0);
+  x.past = rows.past;
+  x.t0 = tile * p.tile_tokens;
+  x.tokens = min(p.tile_tokens, rows.n - x.t0);
   if (x.tokens <= 0) return false;
-  const int pos0 = x.rows.past + x.t0;
+  const int pos0 = x.past + x.t0;
   x.kv_len = pos0 + x.tokens;
   x.key_lo = p.a.window <= pos0 ? pos0 - p.a.window + 1 : 0;
-  const int block0 = x.key_lo / BN, blocks = (x.kv_len + BN - 1) / BN - block0;
-  x.shares = shares_of(blocks, p.splits);
-  if (x.share >= x.shares) return false;
-  x.block_first = block0 + static_cast<int>(static_cast<int64_t>(x.share) * blocks / x.shares);
-  x.nblocks = block0 + static_cast<int>(static_cast<int64_t>(x.share + 1) * blocks / x.shares) - x.block_first;
+  x.block_first = x.key_lo / BN;
+  x.nblocks = (x.kv_len + BN - 1) / BN - x.block_first;
+  x.slot = -1;
   return true;
 }
+// Blocks before place `at` of `places` of a tile with `blocks` blocks.
+__device__ __forceinline__ int blocks_before(int at, int places, int blocks) {
+  return static_cast<int>(static_cast<int64_t>(at) * blocks / places);
+}
+__device__ __forceinline__ void tile_cut(Tile& x, int at, int end, int places, int slot) {
+  const int lo = blocks_before(at, places, x.nblocks), hi = blocks_before(end, places, x.nblocks);
+  x.block_first += lo;
+  x.nblocks = hi - lo;
+  x.slot = slot;
+}
+// Parts of a split tile: at least kMinBlocks blocks each.
+__device__ __forceinline__ int parts_of(const PrefillArgs& p, int blocks) { return max(1, min(p.split, blocks / kMinBlocks)); }
 
-// A warp's (or, for the MMA thread, a thread's) way through the tiles of its CTA: the
-// CTA's own first, then what it claims. The MMA thread asks for the next one as soon as
-// a tile begins; every warp reads the answers. Two answers alternate; a slot is asked
-// for again once all `readers` have left it.
-struct TileWalk {
+// A sequence in the list of shares: for each KV head its tiles in the order first, last,
+// second, last but one, ..., each with `weight` places.
+struct SeqShare {
+  int tiles, weight;
+};
+__device__ __forceinline__ SeqShare seq_share(const PrefillArgs& p, const SeqRows& rows) {
+  SeqShare s{0, 1};
+  if (rows.n == 0) return s;
+  s.tiles = (rows.n + p.tile_tokens - 1) / p.tile_tokens;
+  const int middle = rows.past + (rows.n + p.tile_tokens) / 2;  // its last key, and one
+  s.weight = (static_cast<int>(min(static_cast<int64_t>(middle), static_cast<int64_t>(p.a.window) + p.tile_tokens)) + BN - 1) / BN;
+  return s;
+}
+__device__ __forceinline__ int fold(int rank, int tiles) { return rank & 1 ? tiles - 1 - (rank >> 1) : rank >> 1; }
+
+// The one warp that finds the CTA's next tile: what the grid or the hardware scheduler
+// names, or the next of the CTA's share.
+struct Scheduler {
   const PrefillArgs& p;
-  uint8_t* answers;
-  uint64_t* full;
-  uint64_t* empty;
-  bool asks, single;  // single: one thread walks, not a warp
-  int n = 0;          // answers read
-  bool open = false;  // (asks) an answer is outstanding
+  uint8_t* answer;
+  uint64_t* claimed;
+  int lane;
+  int claims = 0;        // asked for
+  bool begun = false, open = false;
+  int w = 0, w0 = 0, w_end = 0;  // shared: places in the list: here, begin and end of the share
+  int base = 0, work = 0, b = 0; // of the sequence: its begin, its places
+  SeqRows rows{0, 0, 0};
+  SeqShare sh{0, 1};
 
+  __device__ __forceinline__ void enter() {
+    rows = seq_rows(p.a.seqs, b, false);
+    sh = seq_share(p, rows);
+    work = p.a.hkv * sh.tiles * sh.weight;
+  }
+  // The CTA's share, and the sequence it begins in.
+  __device__ void begin_share() {
+    const int batch = p.a.seqs.batch;
+    int total = 0;
+    for (int c = 0; c < batch; c += 32) {
+      if (c + lane < batch) {
+        const SeqShare s = seq_share(p, seq_rows(p.a.seqs, c + lane, blockIdx.x == 0));
+        total += p.a.hkv * s.tiles * s.weight;
+      }
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    const Shares shares(total, p.ctas, kMinBlocks);
+    w0 = w = shares.begin(blockIdx.x);
+    w_end = shares.begin(blockIdx.x + 1);
+    if (w >= w_end) return;
+    for (int c = 0; c < batch; c += 32) {
+      int mine = 0;
+      if (c + lane < batch) {
+        const SeqShare s = seq_share(p, seq_rows(p.a.seqs, c + lane, false));
+        mine = p.a.hkv * s.tiles * s.weight;
+      }
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const int k = __popc(__ballot_sync(0xffffffffu, base + upto <= w));  // sequences that end before w
+      if (k < 32) {
+        base += __shfl_sync(0xffffffffu, upto - mine, k);
+        b = c + k;
+        enter();
+        return;
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  __device__ bool next_of_share(Tile& x) {
+    if (!begun) begin_share();
+    begun = true;
+    while (w < w_end) {
+      while (w >= base + work) {
+        base += work;
+        ++b;
+        enter();
+      }
+      const int unit = (w - base) / sh.weight, at = w - base - unit * sh.weight;
+      const int len = min(sh.weight - at, w_end - w), kvh = unit / sh.tiles;
+      tile_set(p, rows, b, kvh, fold(unit - kvh * sh.tiles, sh.tiles), x);
+      if (len < sh.weight) tile_cut(x, at, at + len, sh.weight, 2 * static_cast<int>(blockIdx.x) + (w == w0 ? 0 : 1));
+      w += len;
+      if (x.nblocks > 0) return true;
+    }
+    return false;
+  }
+  // Item `at` of the grid's list; false when there is nothing to do in it. Order: parts,
+  // groups of pairs, the longest tiles first, the pairs of the group.
+  __device__ __forceinline__ bool item(int at, Tile& x) {
+    const int pairs = p.a.hkv * p.a.seqs.batch, units = pairs * p.tiles;
+    const int part = at / units, unit = at - part * units;
+    const int group = unit / p.tiles / p.pairs_group;
+    const int first = group * p.pairs_group, size = min(p.pairs_group, pairs - first);
+    const int in_group = unit - first * p.tiles;
+    const int rank = in_group / size, pair = first + in_group - rank * size;
+    const int seq = pair / p.a.hkv, tile = p.tiles - 1 - rank;
+    rows = seq_rows(p.a.seqs, seq, lane == 0 && tile == 0);
+    if (!tile_set(p, rows, seq, pair - seq * p.a.hkv, tile, x)) return false;
+    const int parts = parts_of(p, x.nblocks);
+    if (part >= parts) return false;
+    if (parts > 1) tile_cut(x, part, part + 1, parts, (pair * p.tiles + tile) * p.split + part);
+    return true;
+  }
+  // Asks for another item: a few key blocks before a tile's end (not earlier: what is
+  // claimed waits for this CTA, while another may be idle).
   __device__ __forceinline__ void ask() {
-    if (!asks) return;
-    if (!mbar_wait(&empty[n & 1], ((n >> 1) & 1) ^ 1)) return;  // the wait below then runs out
-    mbar_arrive_expect_tx(&full[n & 1], 16);
-    claim_next_cta(answers + 16 * (n & 1), &full[n & 1]);
+    if (p.shared) return;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(claimed, 16);
+      claim_next_cta(answer, claimed);
+    }
     open = true;
   }
-  // The CTA index of the next tile, -1 at the end, -2 when a wait ran out.
-  __device__ __forceinline__ int claim(volatile int* abort_flag) {
+  __device__ bool next(Tile& x, bool& ok) {
+    if (p.shared) return next_of_share(x);
+    while (true) {
+      int at = static_cast<int>(blockIdx.x);
+      if (begun) {
+        if (!__all_sync(0xffffffffu, mbar_wait(claimed, claims & 1))) {
+          ok = false;
+          return false;
+        }
+        at = claimed_cta(answer);
+        open = false;
+        ++claims;
+        fence_proxy_async_smem();  // read before it is written again
+        __syncwarp();
+        if (at < 0) return false;
+      }
+      begun = true;
+      if (item(at, x)) return true;
+      ask();
+    }
+  }
+};
+
+// The tiles as the scheduling warp passes them to the others, through two slots.
+struct TileQueue {
+  uint8_t* slots;
+  uint64_t* full;
+  uint64_t* empty;
+  int n = 0;
+  // By the scheduling warp; x.nblocks = 0 at the end.
+  __device__ __forceinline__ bool put(const Tile& x, int lane) {
+    const bool free_slot = mbar_wait(&empty[n & 1], ((n >> 1) & 1) ^ 1);
+    if (!__all_sync(0xffffffffu, free_slot)) return false;
+    if (lane == 0) {
+      const uint4* from = reinterpret_cast<const uint4*>(&x);
+      uint4* to = reinterpret_cast<uint4*>(slots + 48 * (n & 1));
+      to[0] = from[0];
+      to[1] = from[1];
+      to[2] = from[2];
+      mbar_arrive(&full[n & 1]);
+    }
+    __syncwarp();
+    ++n;
+    return true;
+  }
+  // By another warp, or by one thread of it (single). False at the end, and with ok
+  // false when the wait ran out.
+  __device__ __forceinline__ bool get(Tile& x, bool single, volatile int* abort_flag, bool& ok) {
     bool got = mbar_wait(&full[n & 1], (n >> 1) & 1) && *abort_flag == 0;
     if (!single) got = __all_sync(0xffffffffu, got);
-    if (!got) return -2;
-    const int at = claimed_cta(answers + 16 * (n & 1));
-    open = false;
-    fence_proxy_async_smem();  // read before the slot is written again
+    if (!got) {
+      ok = false;
+      return false;
+    }
+    const uint4* from = reinterpret_cast<const uint4*>(slots + 48 * (n & 1));
+    uint4* to = reinterpret_cast<uint4*>(&x);
+    to[0] = from[0];
+    to[1] = from[1];
+    to[2] = from[2];
     if (!single) __syncwarp();
     if (single || (threadIdx.x & 31) == 0) mbar_arrive(&empty[n & 1]);
     ++n;
-    return at;
-  }
-  // Advances to the next tile with work. `at`: -1 before the first call.
-  __device__ __forceinline__ bool next(Tile& x, int& at, bool report, volatile int* abort_flag, bool& ok) {
-    while (true) {
-      at = at == -1 ? static_cast<int>(blockIdx.x) : claim(abort_flag);
-      if (at < 0) {
-        ok = ok && at == -1;
-        return false;
-      }
-      ask();
-      if (tile_at(p, at, x, report)) return true;
-    }
+    return x.nblocks > 0;
   }
 };
 
@@ -234,7 +378,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     if (threadIdx.x == 0) set_device_error(a.seqs.err, kDevErrAttentionTimeout);
     return;  // uniform for the CTA, nothing was started
   }
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff + L::kClaims);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff + L::kTiles);
   uint64_t* q_empty = q_full + 1;
   uint64_t* k_full = q_empty + 1;
   uint64_t* k_empty = k_full + KST;
@@ -246,9 +390,11 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   uint64_t* o_full = o_done + 1;
   uint64_t* o_empty = o_full + 1;
   uint64_t* mma_done = o_empty + 1;
-  uint64_t* claim_full = mma_done + 1;
-  uint64_t* claim_empty = claim_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(claim_empty + 2);
+  uint64_t* claimed = mma_done + 1;
+  uint64_t* near_end = claimed + 1;
+  uint64_t* tile_full = near_end + 1;
+  uint64_t* tile_empty = tile_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tile_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -272,9 +418,11 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     mbar_init(o_full, 1);
     mbar_init(o_empty, 4);
     mbar_init(mma_done, 1);
+    mbar_init(claimed, 1);
+    mbar_init(near_end, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&claim_full[s], 1);
-      mbar_init(&claim_empty[s], kFp4 ? 9 : 6);  // the warps that walk
+      mbar_init(&tile_full[s], 1);
+      mbar_init(&tile_empty[s], kFp4 ? 9 : 5);  // the MMA thread, softmax warps, converters
     }
     *abort_flag = 0;
     mbar_fence_init();
@@ -289,9 +437,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_trigger();
-  TileWalk walk{p, smem + L::kBarOff, claim_full, claim_empty, warp == W::kMma, warp == W::kMma};
+  TileQueue tiles{smem + L::kBarOff + 16, tile_full, tile_empty};
   Tile x;
-  int at = -1;
   bool ok = true;
   int g0 = 0;    // key blocks of the tiles before this one: stages and phases run on
   int tile_n = 0;  // tiles before this one
@@ -302,7 +449,11 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     const int box_rows = min(page_rows, BN), boxes = BN / box_rows;
     const int none = static_cast<int>(a.seqs.num_pages);  // outside the map: reads as zeros
     int k_issued = 0, v_issued = 0, q_issued = 0;
-    while (ok && walk.next(x, at, lane == 0, abort_flag, ok)) {
+    Scheduler scheduler{p, smem + L::kBarOff, claimed, lane};
+    while (ok) {
+      if (!scheduler.next(x, ok)) x.nblocks = 0;
+      ok = tiles.put(x, lane) && ok;
+      if (!ok || x.nblocks == 0) break;
       const int32_t* ids = a.seqs.page_table + x.b * a.seqs.max_pages;
       const int last_page = (x.kv_len - 1) >> shift;
       auto page_for = [&](int j) {  // of lane's box of step j
@@ -349,11 +500,12 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         mbar_arrive_expect_tx(q_full, p.q_bytes);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(smem + c * L::kBox, &tq, c * 64, x.kvh * a.group, static_cast<int>(x.rows.row0) + x.t0, 0, q_full);
+          tma_load_4d(smem + c * L::kBox, &tq, c * 64, x.kvh * a.group, x.row0 + x.t0, 0, q_full);
       }
       __syncwarp();
       q_issued = tile_n + 1;
       for (int j = 0; j < x.nblocks && ok; ++j) {
+        if (j == max(0, x.nblocks - 2)) scheduler.ask();
         const int page3 = page_for(j + 3);
         if (j + 1 < x.nblocks) ok = load(j + 1, page1, true);
         if (ok) ok = load(j, page0, false);
@@ -369,6 +521,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       *abort_flag = 1;
     }
     // no copy may still be writing shared memory when the CTA exits
+    if (scheduler.open) mbar_wait(claimed, scheduler.claims & 1);
     if (q_issued > 0) mbar_wait(q_full, (q_issued - 1) & 1);
     for (int g = max(0, k_issued - KST); g < k_issued; ++g) mbar_wait(&k_full[g % KST], (g / KST) & 1);
     for (int g = max(0, v_issued - VST); g < v_issued; ++g) mbar_wait(&v_full[g % VST], (g / VST) & 1);
@@ -377,7 +530,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       constexpr uint32_t idesc_s = umma_idesc_f16(kBf16, BM, BN);
       constexpr uint32_t idesc_o = umma_idesc_f16_bmn(kBf16, BM, D);
       const uint32_t q_addr = smem_u32(smem);
-      while (ok && walk.next(x, at, false, abort_flag, ok)) {
+      while (ok && tiles.get(x, true, abort_flag, ok)) {
         auto qk = [&](int j) -> bool {
           const int g = g0 + j, s = g % KST, sb = g & 1;
           if (!mbar_wait(&k_full[s], (g / KST) & 1)) return false;
@@ -429,12 +582,31 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         set_device_error(a.seqs.err, kDevErrAttentionTimeout);
         *abort_flag = 1;
       }
-      // every issued MMA has finished before the CTA releases tensor memory, and no
-      // answer is still to be written
+      // every issued MMA has finished before the CTA releases tensor memory
       umma_commit(mma_done);
       mbar_wait(mma_done, 0);
-      if (walk.open) mbar_wait(&claim_full[walk.n & 1], (walk.n >> 1) & 1);
     }
+  } else if (kFp4 && warp == W::kSchedule) {
+    Scheduler scheduler{p, smem + L::kBarOff, claimed, lane};
+    while (ok) {
+      if (!scheduler.next(x, ok)) x.nblocks = 0;
+      ok = tiles.put(x, lane) && ok;
+      if (!ok || x.nblocks == 0) break;
+      if (!p.shared) {
+        // a whole tile may take longer than one wait lasts: as long as its blocks may take
+        bool near = false;
+        for (int tries = 0; !near && tries <= x.nblocks && *abort_flag == 0; ++tries) near = mbar_wait(near_end, tile_n & 1);
+        ok = __all_sync(0xffffffffu, near);
+        if (!ok) break;
+        scheduler.ask();
+      }
+      ++tile_n;
+    }
+    if (!ok && lane == 0) {
+      set_device_error(a.seqs.err, kDevErrAttentionTimeout);
+      *abort_flag = 1;
+    }
+    if (scheduler.open) mbar_wait(claimed, scheduler.claims & 1);  // no answer is still to be written
   } else if (kFp4 && warp >= W::kConvert) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W::kConvertRegs));
     // ---- converters: thread = half a key row; loads a block ahead, then K0, K1, V0, ...
@@ -460,7 +632,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     };
-    while (ok && walk.next(x, at, lane == 0, abort_flag, ok)) {
+    while (ok && tiles.get(x, false, abort_flag, ok)) {
       const int32_t* ids = a.seqs.page_table + x.b * a.seqs.max_pages;
       auto page_for = [&](int j) {
         const int key = j < x.nblocks ? x.key_of(j) + key_row : -1;
@@ -494,6 +666,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       // V of step j is converted after K of step j + 1: the order of the MMAs
       for (int j = 0; j <= x.nblocks; ++j) {
         const int page2 = page_for(j + 2);
+        if (ct == 0 && j == max(0, x.nblocks - 2)) mbar_arrive(near_end);
         if (j < x.nblocks) {
           const int g = g0 + j, st = g % KST;
           ok = warp_wait(&k_empty[st], ((g / KST) & 1) ^ 1, abort_flag);
@@ -526,9 +699,9 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
     const int tok = row / a.group, in_group = row - tok * a.group;
     const bool cap = a.softcap > 0.f, bias = a.slopes != nullptr;
     const float cap_out = a.softcap * kLog2e;
-    while (ok && walk.next(x, at, false, abort_flag, ok)) {
+    while (ok && tiles.get(x, false, abort_flag, ok)) {
       const int rows = x.tokens * a.group;  // of the 128
-      const int pos0 = x.rows.past + x.t0;
+      const int pos0 = x.past + x.t0;
       const int head = x.kvh * a.group + in_group;
       const int pos = row < rows ? pos0 + tok : -1;  // rows past the tile compute what nobody reads
       const int lo = max(-1, pos - a.window);        // sees the keys in (lo, pos]
@@ -537,7 +710,7 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       if constexpr (kFp4) {
         // this thread's row of the Q tile (every S of the tile before has been read, so
         // its Q has too), scaled by 2^-e with 2^e <= max|q| < 2^(e+1)
-        const T* q = static_cast<const T*>(a.q) + ((x.rows.row0 + x.t0 + tok) * a.hq + head) * D;
+        const T* q = static_cast<const T*>(a.q) + (static_cast<int64_t>(x.row0 + x.t0 + tok) * a.hq + head) * D;
         float big = 0.f;
         if (row < rows) {
 #pragma unroll 4
@@ -683,12 +856,12 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         break;
       }
       tc_fence_after();
-      const bool whole = x.shares == 1;
+      const bool whole = x.slot < 0;
       const float inv = l > 0.f ? a.v_scale / l : 0.f;
-      T* dst = static_cast<T*>(a.out) + ((x.rows.row0 + x.t0 + tok) * a.hq + head) * D;
-      // the share's O, unnormalised, its maximum and sum
-      const int64_t part = ((static_cast<int64_t>(x.b) * a.hkv + x.kvh) * p.tiles + x.tile) * p.splits + x.share;
-      float* part_dst = p.part_o + (part * BM + row) * D;
+      T* dst = static_cast<T*>(a.out) + (static_cast<int64_t>(x.row0 + x.t0 + tok) * a.hq + head) * D;
+      // the part's O, unnormalised, its maximum and sum
+      const int64_t part = whole ? 0 : static_cast<int64_t>(x.slot);
+      float* part_dst = p.part_o + (part * (D / 4) * BM + row) * 4;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t r[32];
@@ -716,7 +889,8 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(part_dst + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(part_dst + (c + i) * BM) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
         }
       }
       if (!whole && row < rows) p.part_ml[part * BM + row] = make_float2(m_used, l);
@@ -737,63 +911,110 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   }
 }
 
-// Merges the shares of a tile in order. grid = (tiles x (128 x D / 1024), KV heads,
-// sequences); thread = 4 elements of a row. Which shares there are is worked out while
-// the main kernel still runs: positions and starts were final before that began.
+// Merges the parts of the tiles that were cut, in order. Shared list: the first part's
+// slot is its CTA's first or second, the others are the first slots of the CTAs after
+// it; parts without blocks were not written. Split tiles: the tile's own slots. grid =
+// (tiles x D / 16, KV heads, sequences); a warp's lanes are rows, a thread takes 4
+// elements of two chunks. Which parts there are is worked out while the main kernel
+// still runs: positions and starts were final before that began.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_paged_prefill_combine_kernel(const PrefillArgs p) {
-  constexpr int CHUNKS = BM * D / 1024;
+  constexpr int CHUNKS = D / 16;  // of 16 dims
   const PagedAttnArgs& a = p.a;
-  const int tile = blockIdx.x / CHUNKS, chunk = blockIdx.x % CHUNKS, kvh = blockIdx.y, b = blockIdx.z;
-  const SeqRows sr = seq_rows(a.seqs, b, false);
-  const int t0 = tile * p.tile_tokens, tokens = min(p.tile_tokens, sr.n - t0);
-  const int pos0 = sr.past + t0, key_lo = a.window <= pos0 ? pos0 - a.window + 1 : 0;
-  const int shares = shares_of((pos0 + tokens + BN - 1) / BN - key_lo / BN, p.splits);
-  const int c = chunk * 256 + threadIdx.x;
-  const int r = c / (D / 4), d = (c - r * (D / 4)) * 4;
-  pdl_wait();
-  pdl_trigger();
-  if (tokens <= 0 || shares == 1 || r >= tokens * a.group) return;
-  const int64_t at = ((static_cast<int64_t>(b) * a.hkv + kvh) * p.tiles + tile) * p.splits * BM + r;
-  float top = -INFINITY, den = 0.f;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < shares; s0 += 4) {
-    float2 ml[4];
-    float4 v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      ml[k] = make_float2(-INFINITY, 0.f);
-      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (s0 + k < shares) {
-        ml[k] = p.part_ml[at + (s0 + k) * BM];
-        v[k] = *reinterpret_cast<const float4*>(p.part_o + (at + (s0 + k) * BM) * D + d);
+  const int chunk = blockIdx.x % CHUNKS, rank = blockIdx.x / CHUNKS, kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
+  const SeqRows rows = seq_rows(a.seqs, b, false);
+  const SeqShare sh = seq_share(p, rows);
+  Tile x;
+  int parts = 1, places = 1, first = 0, begin = 0;
+  int64_t slot0 = 0, slot_step = 1;  // slots: slot0, then slot1, slot1 + slot_step, ...
+  int64_t slot1 = 0;
+  Shares shares(0, 1, 1);
+  if (p.shared) {
+    int total = 0, base = 0;
+    for (int c = 0; c < a.seqs.batch; c += 32) {
+      if (c + lane < a.seqs.batch) {
+        const SeqShare s = seq_share(p, seq_rows(a.seqs, c + lane, false));
+        const int work = a.hkv * s.tiles * s.weight;
+        total += work;
+        if (c + lane < b) base += work;
       }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (ml[k].x == -INFINITY) continue;  // a share in which the row sees no key
-      const float m = fmaxf(top, ml[k].x);
-      const float f = exp2_approx(top - m), f2 = exp2_approx(ml[k].x - m);  // top = -inf: 0
-      top = m;
-      den = den * f + ml[k].y * f2;
-      sum.x = sum.x * f + v[k].x * f2;
-      sum.y = sum.y * f + v[k].y * f2;
-      sum.z = sum.z * f + v[k].z * f2;
-      sum.w = sum.w * f + v[k].w * f2;
+    total = __reduce_add_sync(0xffffffffu, total);
+    base = __reduce_add_sync(0xffffffffu, base);
+    shares = Shares(total, p.ctas, kMinBlocks);
+    if (rank < sh.tiles) {
+      tile_set(p, rows, b, kvh, fold(rank, sh.tiles), x);
+      places = sh.weight;
+      begin = base + (kvh * sh.tiles + rank) * places;
+      first = shares.cta_of(begin);
+      parts = shares.cta_of(begin + places - 1) - first + 1;
+      slot0 = begin == shares.begin(first) ? 2 * first : 2 * first + 1;
+      slot1 = 2ll * (first + 1);
+      slot_step = 2;
     }
+  } else if (tile_set(p, rows, b, kvh, rank, x)) {
+    places = parts = parts_of(p, x.nblocks);
+    slot0 = (static_cast<int64_t>(b * a.hkv + kvh) * p.tiles + rank) * p.split;
+    slot1 = slot0 + 1;
   }
+  pdl_wait();
+  pdl_trigger();
+  if (parts == 1) return;
+  const int r = threadIdx.x & (BM - 1);
+  if (r >= x.tokens * a.group) return;
   const int tok = r / a.group, head = kvh * a.group + r - tok * a.group;
-  const float inv = a.v_scale / den;
-  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + ((sr.row0 + t0 + tok) * a.hq + head) * D + d) =
-      make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
+  T* dst = static_cast<T*>(a.out) + (static_cast<int64_t>(x.row0 + x.t0 + tok) * a.hq + head) * D;
+#pragma unroll
+  for (int d4 = chunk * 4 + threadIdx.x / BM; d4 < chunk * 4 + 4; d4 += 2) {
+    float top = -INFINITY, den = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < parts; s0 += 4) {
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int i = s0 + k;
+        if (i >= parts) continue;
+        if (p.shared) {
+          const int from = i == 0 ? 0 : shares.begin(first + i) - begin;
+          const int to = i == parts - 1 ? places : shares.begin(first + i + 1) - begin;
+          if (blocks_before(from, places, x.nblocks) == blocks_before(to, places, x.nblocks)) continue;
+        }
+        const int64_t slot = i == 0 ? slot0 : slot1 + (i - 1) * slot_step;
+        ml[k] = p.part_ml[slot * BM + r];
+        v[k] = *reinterpret_cast<const float4*>(p.part_o + ((slot * (D / 4) + d4) * BM + r) * 4);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (ml[k].x == -INFINITY) continue;  // a part in which the row sees no key
+        const float m = fmaxf(top, ml[k].x);
+        const float f = exp2_approx(top - m), f2 = exp2_approx(ml[k].x - m);  // top = -inf: 0
+        top = m;
+        den = den * f + ml[k].y * f2;
+        sum.x = sum.x * f + v[k].x * f2;
+        sum.y = sum.y * f + v[k].y * f2;
+        sum.z = sum.z * f + v[k].z * f2;
+        sum.w = sum.w * f + v[k].w * f2;
+      }
+    }
+    const float inv = a.v_scale / den;
+    *reinterpret_cast<uint2*>(dst + d4 * 4) = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
+  }
 }
 
 // ---- host ------------------------------------------------------------------------
 struct PrefillPlan {
   int64_t tiles, pairs, units;
-  int tile_tokens, splits, pairs_group;
+  int tile_tokens, pairs_group, ctas, split;
+  bool shared;
   size_t part_o, workspace;
 };
+
+// Tiles for each place of a CTA up to which their list is shared out equally. With more,
+// whole tiles balance as well and nothing passes through the workspace.
+constexpr int kSharedTiles = 4;
 
 PrefillPlan plan_prefill(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys) {
   PrefillPlan p{};
@@ -803,13 +1024,13 @@ PrefillPlan plan_prefill(int64_t batch, int64_t hkv, int64_t group, int64_t max_
   p.units = p.tiles * p.pairs;
   // pairs of a group: their K and V (2 x 2 bytes an element) within about a quarter of L2
   p.pairs_group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.pairs, (32ll << 20) / (4 * head_dim * std::max<int64_t>(1, max_keys)))));
-  // as many shares of the keys as keep every CTA resident at once, at least 256 keys each
-  const int64_t slots = 2ll * sm_count();
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({slots / std::max<int64_t>(1, p.units), max_keys / (4 * BN), 64})));
-  if (p.splits > 1) {
-    p.part_o = static_cast<size_t>(p.units * p.splits * BM * head_dim) * 4;
-    p.workspace = p.part_o + static_cast<size_t>(p.units * p.splits * BM) * 8;
-  }
+  p.ctas = 2 * sm_count();
+  p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({p.ctas / std::max<int64_t>(1, p.units), max_keys / (kMinBlocks * BN), 64})));
+  p.shared = p.split == 1 && p.units <= kSharedTiles * static_cast<int64_t>(p.ctas) && max_keys >= 2 * kMinBlocks * BN &&
+             p.units * (max_keys / BN + 2) < INT_MAX;
+  const int64_t slots = p.shared ? 2ll * p.ctas : p.split > 1 ? p.units * p.split : 0;
+  p.part_o = static_cast<size_t>(slots * BM * head_dim) * 4;
+  p.workspace = p.part_o + static_cast<size_t>(slots * BM) * 8;
   return p;
 }
 
@@ -831,12 +1052,15 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
   PrefillArgs p{};
   p.a = a;
   p.tile_tokens = plan.tile_tokens;
-  p.splits = plan.splits;
+  p.shared = plan.shared ? 1 : 0;
   p.tiles = static_cast<int>(plan.tiles);
-  p.pairs_group = plan.splits > 1 ? static_cast<int>(std::min<int64_t>(plan.pairs, INT_MAX)) : plan.pairs_group;
+  p.ctas = plan.ctas;
+  p.split = plan.split;
+  p.pairs_group = plan.pairs_group;
   p.wide_out = aligned(a.out, 32);
   p.q_bytes = static_cast<unsigned>(plan.tile_tokens * a.group * D * 2);
-  if (plan.splits > 1) {
+  const bool parts = plan.shared || plan.split > 1;
+  if (parts) {
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.part_o);
   }
@@ -851,13 +1075,14 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
     }();
     if (regs < Roles<true>::kLaunchRegs) return fail(DLI_ERR_UNSUPPORTED, "attention_paged: built with too few registers a thread");
   }
-  launch_pdl(kern, dim3(static_cast<unsigned>(plan.units * plan.splits)), dim3(Roles<kFp4>::kThreads), L::kBytes, stream, p, tq, tk, tv);
-  if (plan.splits > 1)
+  launch_pdl(kern, dim3(static_cast<unsigned>(plan.shared ? plan.ctas : plan.units * plan.split)), dim3(Roles<kFp4>::kThreads), L::kBytes,
+             stream, p, tq, tk, tv);
+  if (parts)
     launch_pdl(attn_paged_prefill_combine_kernel<T, D>,
-               dim3(static_cast<unsigned>(plan.tiles * (BM * D / 1024)), static_cast<unsigned>(a.hkv),
+               dim3(static_cast<unsigned>(plan.tiles * (D / 16)), static_cast<unsigned>(a.hkv),
                     static_cast<unsigned>(a.seqs.batch)),
                dim3(256), 0, stream, p);
-  return check_launch("attention_paged", plan.splits > 1 ? 2 : 1);
+  return check_launch("attention_paged", parts ? 2 : 1);
 }
 
 int64_t keys_of(const PagedAttnArgs& a) {
