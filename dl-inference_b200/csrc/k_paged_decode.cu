@@ -104,6 +104,18 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int b, bool 
   return w;
 }
 
+// The equal shares of `total` blocks among the CTAs that get any.
+struct Shares {
+  int total, ctas, q, r;
+  __device__ __forceinline__ Shares(int total_blocks, int grid, int min_blocks) : total(total_blocks) {
+    ctas = max(1, min(grid, (total + min_blocks - 1) / min_blocks));
+    q = total / ctas;
+    r = total - q * ctas;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c >= ctas ? total : c * q + min(c, r); }
+  __device__ __forceinline__ int cta_of(int at) const { return at < r * (q + 1) ? at / (q + 1) : r + (at - r * (q + 1)) / max(q, 1); }
+};
+
 // The blocks of all sequences (a whole warp).
 template <int BN, int R>
 __device__ __forceinline__ int list_total(const PagedAttnArgs& a, int lane, bool report) {

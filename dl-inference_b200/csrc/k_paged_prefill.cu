@@ -12,11 +12,9 @@
 // from the hardware scheduler (cluster launch control) while it computes, so two CTAs
 // per SM stay for the whole call, one tile's end overlaps the next one's start, and a
 // ragged batch is balanced as it runs (which CTA computes a tile changes nothing in it).
-// Few tiles: with room for several CTAs per tile, each tile's keys are split evenly;
-// else the tiles are one list, a tile counting as its sequence's mean number of key
-// blocks and short tiles taking turns with long ones, of which every CTA takes an equal
-// share. Tiles that are cut store their parts' (max, sum, O) in the workspace, and a
-// second kernel merges them in order.
+// Few tiles: each tile's keys are split evenly into parts, which are items of the list
+// like tiles; they store their (max, sum, O) in the workspace, and a second kernel merges
+// them in order.
 // 192 threads:
 //   warp 0     loads each Q tile (a box of group x tokens of q by TMA), walks the page
 //              table and loads 64-key K and V blocks (a box per page; boxes past the
@@ -62,7 +60,7 @@ struct Roles {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // log2: P <= 2^8 before O is rescaled
 constexpr int BM = 128, BN = 64;
-constexpr int kMinBlocks = 4;  // shared: no CTA takes fewer key blocks (but the last)
+
 
 template <int D>
 struct PrefillLayout {
@@ -88,13 +86,12 @@ struct PrefillArgs {
   PagedAttnArgs a;
   int tile_tokens;  // 128 / group
   int tiles;        // of a sequence of max_new tokens
-  int ctas;         // of the main kernel, when shared or split
-  int split;        // few tiles, several CTAs each: parts of a tile's keys (else 1)
-  int shared;       // few tiles: equal shares of their list
+  int split;        // parts of a tile's keys, at most
+  int min_part;     // key blocks of a part, at least
   int pairs_group;  // (sequence, KV head) pairs whose tiles are interleaved
   int wide_out;     // out is 32-byte aligned
-  float* part_o;    // [slots][D / 4][128][4]
-  float2* part_ml;  // [slots][128]
+  float* part_o;    // [tiles x split][D / 4][128][4]
+  float2* part_ml;  // [tiles x split][128]
   unsigned q_bytes; // of the Q box
 };
 
@@ -129,108 +126,19 @@ __device__ __forceinline__ bool tile_set(const PrefillArgs& p, const SeqRows& ro
   x.slot = -1;
   return true;
 }
-// Blocks before place `at` of `places` of a tile with `blocks` blocks.
-__device__ __forceinline__ int blocks_before(int at, int places, int blocks) {
-  return static_cast<int>(static_cast<int64_t>(at) * blocks / places);
-}
-__device__ __forceinline__ void tile_cut(Tile& x, int at, int end, int places, int slot) {
-  const int lo = blocks_before(at, places, x.nblocks), hi = blocks_before(end, places, x.nblocks);
-  x.block_first += lo;
-  x.nblocks = hi - lo;
-  x.slot = slot;
-}
-// Parts of a split tile: at least kMinBlocks blocks each.
-__device__ __forceinline__ int parts_of(const PrefillArgs& p, int blocks) { return max(1, min(p.split, blocks / kMinBlocks)); }
+// The parts of a tile with `blocks` blocks, by its sequence's length.
+__device__ __forceinline__ int parts_of(const PrefillArgs& p, int blocks) { return max(1, min(p.split, blocks / p.min_part)); }
 
-// A sequence in the list of shares: for each KV head its tiles in the order first, last,
-// second, last but one, ..., each with `weight` places.
-struct SeqShare {
-  int tiles, weight;
-};
-__device__ __forceinline__ SeqShare seq_share(const PrefillArgs& p, const SeqRows& rows) {
-  SeqShare s{0, 1};
-  if (rows.n == 0) return s;
-  s.tiles = (rows.n + p.tile_tokens - 1) / p.tile_tokens;
-  const int middle = rows.past + (rows.n + p.tile_tokens) / 2;  // its last key, and one
-  s.weight = (static_cast<int>(min(static_cast<int64_t>(middle), static_cast<int64_t>(p.a.window) + p.tile_tokens)) + BN - 1) / BN;
-  return s;
-}
-__device__ __forceinline__ int fold(int rank, int tiles) { return rank & 1 ? tiles - 1 - (rank >> 1) : rank >> 1; }
-
-// The one warp that finds the CTA's next tile: what the grid or the hardware scheduler
-// names, or the next of the CTA's share.
+// The one warp that finds the CTA's next item: its own of the grid, then what the
+// hardware scheduler grants.
 struct Scheduler {
   const PrefillArgs& p;
   uint8_t* answer;
   uint64_t* claimed;
   int lane;
-  int claims = 0;        // asked for
+  int claims = 0;  // answered
   bool begun = false, open = false;
-  int w = 0, w0 = 0, w_end = 0;  // shared: places in the list: here, begin and end of the share
-  int base = 0, work = 0, b = 0; // of the sequence: its begin, its places
-  SeqRows rows{0, 0, 0};
-  SeqShare sh{0, 1};
 
-  __device__ __forceinline__ void enter() {
-    rows = seq_rows(p.a.seqs, b, false);
-    sh = seq_share(p, rows);
-    work = p.a.hkv * sh.tiles * sh.weight;
-  }
-  // The CTA's share, and the sequence it begins in.
-  __device__ void begin_share() {
-    const int batch = p.a.seqs.batch;
-    int total = 0;
-    for (int c = 0; c < batch; c += 32) {
-      if (c + lane < batch) {
-        const SeqShare s = seq_share(p, seq_rows(p.a.seqs, c + lane, blockIdx.x == 0));
-        total += p.a.hkv * s.tiles * s.weight;
-      }
-    }
-    total = __reduce_add_sync(0xffffffffu, total);
-    const Shares shares(total, p.ctas, kMinBlocks);
-    w0 = w = shares.begin(blockIdx.x);
-    w_end = shares.begin(blockIdx.x + 1);
-    if (w >= w_end) return;
-    for (int c = 0; c < batch; c += 32) {
-      int mine = 0;
-      if (c + lane < batch) {
-        const SeqShare s = seq_share(p, seq_rows(p.a.seqs, c + lane, false));
-        mine = p.a.hkv * s.tiles * s.weight;
-      }
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      const int k = __popc(__ballot_sync(0xffffffffu, base + upto <= w));  // sequences that end before w
-      if (k < 32) {
-        base += __shfl_sync(0xffffffffu, upto - mine, k);
-        b = c + k;
-        enter();
-        return;
-      }
-      base += __shfl_sync(0xffffffffu, upto, 31);
-    }
-  }
-  __device__ bool next_of_share(Tile& x) {
-    if (!begun) begin_share();
-    begun = true;
-    while (w < w_end) {
-      while (w >= base + work) {
-        base += work;
-        ++b;
-        enter();
-      }
-      const int unit = (w - base) / sh.weight, at = w - base - unit * sh.weight;
-      const int len = min(sh.weight - at, w_end - w), kvh = unit / sh.tiles;
-      tile_set(p, rows, b, kvh, fold(unit - kvh * sh.tiles, sh.tiles), x);
-      if (len < sh.weight) tile_cut(x, at, at + len, sh.weight, 2 * static_cast<int>(blockIdx.x) + (w == w0 ? 0 : 1));
-      w += len;
-      if (x.nblocks > 0) return true;
-    }
-    return false;
-  }
   // Item `at` of the grid's list; false when there is nothing to do in it. Order: parts,
   // groups of pairs, the longest tiles first, the pairs of the group.
   __device__ __forceinline__ bool item(int at, Tile& x) {
@@ -241,17 +149,22 @@ struct Scheduler {
     const int in_group = unit - first * p.tiles;
     const int rank = in_group / size, pair = first + in_group - rank * size;
     const int seq = pair / p.a.hkv, tile = p.tiles - 1 - rank;
-    rows = seq_rows(p.a.seqs, seq, lane == 0 && tile == 0);
+    const SeqRows rows = seq_rows(p.a.seqs, seq, lane == 0 && tile == 0);
     if (!tile_set(p, rows, seq, pair - seq * p.a.hkv, tile, x)) return false;
     const int parts = parts_of(p, x.nblocks);
     if (part >= parts) return false;
-    if (parts > 1) tile_cut(x, part, part + 1, parts, (pair * p.tiles + tile) * p.split + part);
+    if (parts > 1) {
+      const int64_t blocks = x.nblocks;
+      const int lo = static_cast<int>(part * blocks / parts);
+      x.nblocks = static_cast<int>((part + 1) * blocks / parts) - lo;
+      x.block_first += lo;
+      x.slot = (pair * p.tiles + tile) * p.split + part;
+    }
     return true;
   }
   // Asks for another item: a few key blocks before a tile's end (not earlier: what is
   // claimed waits for this CTA, while another may be idle).
   __device__ __forceinline__ void ask() {
-    if (p.shared) return;
     if (lane == 0) {
       mbar_arrive_expect_tx(claimed, 16);
       claim_next_cta(answer, claimed);
@@ -259,7 +172,6 @@ struct Scheduler {
     open = true;
   }
   __device__ bool next(Tile& x, bool& ok) {
-    if (p.shared) return next_of_share(x);
     while (true) {
       int at = static_cast<int>(blockIdx.x);
       if (begun) {
@@ -592,14 +504,12 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       if (!scheduler.next(x, ok)) x.nblocks = 0;
       ok = tiles.put(x, lane) && ok;
       if (!ok || x.nblocks == 0) break;
-      if (!p.shared) {
-        // a whole tile may take longer than one wait lasts: as long as its blocks may take
-        bool near = false;
-        for (int tries = 0; !near && tries <= x.nblocks && *abort_flag == 0; ++tries) near = mbar_wait(near_end, tile_n & 1);
-        ok = __all_sync(0xffffffffu, near);
-        if (!ok) break;
-        scheduler.ask();
-      }
+      // a whole tile may take longer than one wait lasts: as long as its blocks may take
+      bool near = false;
+      for (int tries = 0; !near && tries <= x.nblocks && *abort_flag == 0; ++tries) near = mbar_wait(near_end, tile_n & 1);
+      ok = __all_sync(0xffffffffu, near);
+      if (!ok) break;
+      scheduler.ask();
       ++tile_n;
     }
     if (!ok && lane == 0) {
@@ -911,52 +821,18 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
   }
 }
 
-// Merges the parts of the tiles that were cut, in order. Shared list: the first part's
-// slot is its CTA's first or second, the others are the first slots of the CTAs after
-// it; parts without blocks were not written. Split tiles: the tile's own slots. grid =
-// (tiles x D / 16, KV heads, sequences); a warp's lanes are rows, a thread takes 4
-// elements of two chunks. Which parts there are is worked out while the main kernel
-// still runs: positions and starts were final before that began.
+// Merges the parts of the tiles that were cut, in order. grid = (tiles x D / 16, KV heads,
+// sequences); a warp's lanes are rows, a thread takes 4 elements of two chunks. Which
+// parts there are is worked out while the main kernel still runs: positions and starts
+// were final before that began.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) attn_paged_prefill_combine_kernel(const PrefillArgs p) {
   constexpr int CHUNKS = D / 16;  // of 16 dims
   const PagedAttnArgs& a = p.a;
-  const int chunk = blockIdx.x % CHUNKS, rank = blockIdx.x / CHUNKS, kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-  const SeqRows rows = seq_rows(a.seqs, b, false);
-  const SeqShare sh = seq_share(p, rows);
+  const int chunk = blockIdx.x % CHUNKS, tile = blockIdx.x / CHUNKS, kvh = blockIdx.y, b = blockIdx.z;
   Tile x;
-  int parts = 1, places = 1, first = 0, begin = 0;
-  int64_t slot0 = 0, slot_step = 1;  // slots: slot0, then slot1, slot1 + slot_step, ...
-  int64_t slot1 = 0;
-  Shares shares(0, 1, 1);
-  if (p.shared) {
-    int total = 0, base = 0;
-    for (int c = 0; c < a.seqs.batch; c += 32) {
-      if (c + lane < a.seqs.batch) {
-        const SeqShare s = seq_share(p, seq_rows(a.seqs, c + lane, false));
-        const int work = a.hkv * s.tiles * s.weight;
-        total += work;
-        if (c + lane < b) base += work;
-      }
-    }
-    total = __reduce_add_sync(0xffffffffu, total);
-    base = __reduce_add_sync(0xffffffffu, base);
-    shares = Shares(total, p.ctas, kMinBlocks);
-    if (rank < sh.tiles) {
-      tile_set(p, rows, b, kvh, fold(rank, sh.tiles), x);
-      places = sh.weight;
-      begin = base + (kvh * sh.tiles + rank) * places;
-      first = shares.cta_of(begin);
-      parts = shares.cta_of(begin + places - 1) - first + 1;
-      slot0 = begin == shares.begin(first) ? 2 * first : 2 * first + 1;
-      slot1 = 2ll * (first + 1);
-      slot_step = 2;
-    }
-  } else if (tile_set(p, rows, b, kvh, rank, x)) {
-    places = parts = parts_of(p, x.nblocks);
-    slot0 = (static_cast<int64_t>(b * a.hkv + kvh) * p.tiles + rank) * p.split;
-    slot1 = slot0 + 1;
-  }
+  const int parts = tile_set(p, seq_rows(a.seqs, b, false), b, kvh, tile, x) ? parts_of(p, x.nblocks) : 1;
+  const int64_t slot0 = (static_cast<int64_t>(b * a.hkv + kvh) * p.tiles + tile) * p.split;
   pdl_wait();
   pdl_trigger();
   if (parts == 1) return;
@@ -977,12 +853,7 @@ __global__ void __launch_bounds__(256) attn_paged_prefill_combine_kernel(const P
         v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         const int i = s0 + k;
         if (i >= parts) continue;
-        if (p.shared) {
-          const int from = i == 0 ? 0 : shares.begin(first + i) - begin;
-          const int to = i == parts - 1 ? places : shares.begin(first + i + 1) - begin;
-          if (blocks_before(from, places, x.nblocks) == blocks_before(to, places, x.nblocks)) continue;
-        }
-        const int64_t slot = i == 0 ? slot0 : slot1 + (i - 1) * slot_step;
+        const int64_t slot = slot0 + i;
         ml[k] = p.part_ml[slot * BM + r];
         v[k] = *reinterpret_cast<const float4*>(p.part_o + ((slot * (D / 4) + d4) * BM + r) * 4);
       }
@@ -1007,14 +878,9 @@ __global__ void __launch_bounds__(256) attn_paged_prefill_combine_kernel(const P
 // ---- host ------------------------------------------------------------------------
 struct PrefillPlan {
   int64_t tiles, pairs, units;
-  int tile_tokens, pairs_group, ctas, split;
-  bool shared;
+  int tile_tokens, pairs_group, split, min_part;
   size_t part_o, workspace;
 };
-
-// Tiles for each place of a CTA up to which their list is shared out equally. With more,
-// whole tiles balance as well and nothing passes through the workspace.
-constexpr int kSharedTiles = 4;
 
 PrefillPlan plan_prefill(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys) {
   PrefillPlan p{};
@@ -1024,13 +890,25 @@ PrefillPlan plan_prefill(int64_t batch, int64_t hkv, int64_t group, int64_t max_
   p.units = p.tiles * p.pairs;
   // pairs of a group: their K and V (2 x 2 bytes an element) within about a quarter of L2
   p.pairs_group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(p.pairs, (32ll << 20) / (4 * head_dim * std::max<int64_t>(1, max_keys)))));
-  p.ctas = 2 * sm_count();
-  p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({p.ctas / std::max<int64_t>(1, p.units), max_keys / (kMinBlocks * BN), 64})));
-  p.shared = p.split == 1 && p.units <= kSharedTiles * static_cast<int64_t>(p.ctas) && max_keys >= 2 * kMinBlocks * BN &&
-             p.units * (max_keys / BN + 2) < INT_MAX;
-  const int64_t slots = p.shared ? 2ll * p.ctas : p.split > 1 ? p.units * p.split : 0;
-  p.part_o = static_cast<size_t>(slots * BM * head_dim) * 4;
-  p.workspace = p.part_o + static_cast<size_t>(slots * BM) * 8;
+  // Places for CTAs left over: parts until all have one, of at least 4 key blocks (256
+  // keys). With up to two tiles for each place, parts of 1792 keys or more, so that the
+  // tiles of the longest sequences do not run on alone: us whole -> in parts, 28/4 heads,
+  // 16 x 60 tokens over 16,000 keys 322 -> 206, over 4,000 88 -> 79, 2 x 500 over 10,000
+  // 211 -> 127, 64/8 heads 4 x 200 over 20,000 407 -> 371. Smaller parts or more tiles
+  // cost more than they level: 4 x 301 over 3,001 65 -> 76, 64 x 60 over 4,000 205 -> 223.
+  const int64_t places = 2ll * sm_count();
+  p.split = 1;
+  p.min_part = 4;
+  if (2 * p.units <= places) {
+    p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({places / std::max<int64_t>(1, p.units), max_keys / (4 * BN), 64})));
+  } else if (p.units <= 2 * places) {
+    p.min_part = 28;
+    p.split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, max_keys / (28 * BN))));
+  }
+  if (p.split > 1) {
+    p.part_o = static_cast<size_t>(p.units * p.split * BM * head_dim) * 4;
+    p.workspace = p.part_o + static_cast<size_t>(p.units * p.split * BM) * 8;
+  }
   return p;
 }
 
@@ -1052,15 +930,13 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
   PrefillArgs p{};
   p.a = a;
   p.tile_tokens = plan.tile_tokens;
-  p.shared = plan.shared ? 1 : 0;
   p.tiles = static_cast<int>(plan.tiles);
-  p.ctas = plan.ctas;
   p.split = plan.split;
+  p.min_part = plan.min_part;
   p.pairs_group = plan.pairs_group;
   p.wide_out = aligned(a.out, 32);
   p.q_bytes = static_cast<unsigned>(plan.tile_tokens * a.group * D * 2);
-  const bool parts = plan.shared || plan.split > 1;
-  if (parts) {
+  if (plan.split > 1) {
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + plan.part_o);
   }
@@ -1075,14 +951,14 @@ dli_status launch_prefill(const PagedAttnArgs& a, const PrefillPlan& plan, void*
     }();
     if (regs < Roles<true>::kLaunchRegs) return fail(DLI_ERR_UNSUPPORTED, "attention_paged: built with too few registers a thread");
   }
-  launch_pdl(kern, dim3(static_cast<unsigned>(plan.shared ? plan.ctas : plan.units * plan.split)), dim3(Roles<kFp4>::kThreads), L::kBytes,
+  launch_pdl(kern, dim3(static_cast<unsigned>(plan.units * plan.split)), dim3(Roles<kFp4>::kThreads), L::kBytes,
              stream, p, tq, tk, tv);
-  if (parts)
+  if (plan.split > 1)
     launch_pdl(attn_paged_prefill_combine_kernel<T, D>,
                dim3(static_cast<unsigned>(plan.tiles * (D / 16)), static_cast<unsigned>(a.hkv),
                     static_cast<unsigned>(a.seqs.batch)),
                dim3(256), 0, stream, p);
-  return check_launch("attention_paged", parts ? 2 : 1);
+  return check_launch("attention_paged", plan.split > 1 ? 2 : 1);
 }
 
 int64_t keys_of(const PagedAttnArgs& a) {

@@ -10,18 +10,6 @@ namespace dli_sm100 {
 // 128 bytes of one (page, head).
 dli_status make_page_maps(const PagedAttnArgs& a, dli_dtype dtype, int d, int box_rows, CUtensorMap* tk, CUtensorMap* tv);
 
-// The equal shares of `total` blocks among the CTAs that get any.
-struct Shares {
-  int total, ctas, q, r;
-  __device__ __forceinline__ Shares(int total_blocks, int grid, int min_blocks) : total(total_blocks) {
-    ctas = max(1, min(grid, (total + min_blocks - 1) / min_blocks));
-    q = total / ctas;
-    r = total - q * ctas;
-  }
-  __device__ __forceinline__ int begin(int c) const { return c >= ctas ? total : c * q + min(c, r); }
-  __device__ __forceinline__ int cta_of(int at) const { return at < r * (q + 1) ? at / (q + 1) : r + (at - r * (q + 1)) / max(q, 1); }
-};
-
 // Few query rows per KV head, and every float32 call (k_paged_decode.cu): head_dim 64
 // or 128, 16-byte aligned tensors.
 bool paged_decode_serves(const PagedAttnArgs& a, dli_dtype dtype);
