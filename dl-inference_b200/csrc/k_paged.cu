@@ -500,10 +500,14 @@ dli_status launch_attn_general(const PagedAttnArgs& a, cudaStream_t stream) {
   return check_launch("attention_paged");
 }
 
-// Calls of the decode kernel (the others go to the tcgen05 kernel): up to 32 query rows
-// per KV head, float32, and more heads per KV head than a tcgen05 tile has rows.
-bool few_rows(dli_dtype dtype, int64_t group, int64_t max_new) {
-  return dtype == DLI_DTYPE_F32 || group > 128 || group * max_new <= 32;
+// Calls of the decode kernel (the others go to the tcgen05 kernel): float32, more heads
+// per KV head than a tcgen05 tile has rows, and up to 16 query rows per KV head over
+// 16-bit pages or 32 over 4-bit ones, which the tcgen05 kernel has to convert. us, decode
+// | tcgen05, over 1 x 30,000 keys and 32 x 2,304: 14 rows 28 | 35 and 30 | 36; 28 rows
+// 33 | 35 and 38 | 35; 32 rows 48 | 38 and 65 | 53; 4 bits: 28 rows 32 | 38 and 43 | 43;
+// 56 rows 48 | 38 and 73 | 45.
+bool few_rows(dli_dtype dtype, bool fp4, int64_t group, int64_t max_new) {
+  return dtype == DLI_DTYPE_F32 || group > 128 || group * max_new <= (fp4 ? 32 : 16);
 }
 
 // ---- argument checks -----------------------------------------------------------------
@@ -683,7 +687,7 @@ extern "C" size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64
   if (!is_float_dtype(dtype) || (head_dim != 64 && head_dim != 128)) return 0;
   const int64_t group = q_heads / kv_heads, max_keys = max_pages * page_size;
   (void)kv_dtype;
-  if (few_rows(dtype, group, max_new)) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys, dtype);
+  if (few_rows(dtype, kv_dtype == DLI_DTYPE_FP4, group, max_new)) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys, dtype);
   return paged_prefill_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
 }
 
@@ -724,7 +728,7 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
   a.scale = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim))) * (fp4 ? k_scale : 1.f);
   a.softcap = softcap;
   a.v_scale = fp4 ? v_scale : 1.f;
-  if (few_rows(dtype, a.group, max_new)) {
+  if (few_rows(dtype, fp4, a.group, max_new)) {
     if (paged_decode_serves(a, dtype)) return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
   } else if (paged_prefill_serves(a, dtype, kv_dtype)) {
     return run_paged_prefill(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
