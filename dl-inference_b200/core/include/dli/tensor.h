@@ -5,7 +5,8 @@
 // PyTorch caching allocator provides device memory), or a non-owning external
 // CUDA pointer; `deviceData()` returns the raw device pointer and throws
 // std::logic_error for host tensors. DType keeps the reference's Float32 = 0 and
-// Int64 = 1 and appends BFloat16, Float16 and Int32.
+// Int64 = 1 and appends BFloat16, Float16, Int32 and UInt8 (bytes of 4-bit cache
+// pages).
 #pragma once
 
 #include <ATen/ATen.h>
@@ -20,7 +21,7 @@
 namespace dli {
 
 enum class DeviceType { Cpu, Cuda };
-enum class DType { Float32, Int64, BFloat16, Float16, Int32 };
+enum class DType { Float32, Int64, BFloat16, Float16, Int32, UInt8 };
 
 std::string toString(DeviceType device);
 DeviceType deviceFromString(const std::string& device);

@@ -44,6 +44,7 @@ void KVCache::append(const std::string& name, const Tensor& key, const Tensor& v
   auto it = entries_.find(name);
   if (it != entries_.end()) {
     const KVCacheEntry& e = it->second;
+    if (e.page_size != 0) throw std::invalid_argument("KV cache entry " + name + " is paged");
     if (e.key.dim(0) != b || e.key.dim(1) != h || e.key.dim(3) != d || e.key.dtype() != key.dtype())
       throw std::invalid_argument("KV cache append shape mismatch");
   }
@@ -100,6 +101,7 @@ KVCacheEntry& KVCache::reserve(const std::string& name, std::int64_t batch, std:
   auto it = entries_.find(name);
   if (it != entries_.end()) {
     const KVCacheEntry& e = it->second;
+    if (e.page_size != 0) throw std::invalid_argument("KV cache entry " + name + " is paged");
     if (e.key.dim(0) == batch && e.key.dim(1) == heads && e.key.dim(3) == head_dim &&
         e.key.dtype() == dtype && e.capacity() >= capacity)
       return it->second;
@@ -110,6 +112,31 @@ KVCacheEntry& KVCache::reserve(const std::string& name, std::int64_t batch, std:
   e.value = Tensor(at::zeros({batch, heads, capacity, head_dim},
                              at::TensorOptions().dtype(torchDType(dtype)).device(at::kCUDA, device_id)));
   e.length = 0;
+  entries_[name] = std::move(e);
+  return entries_[name];
+}
+
+KVCacheEntry& KVCache::reservePaged(const std::string& name, std::int64_t num_pages, std::int64_t heads,
+                                    std::int64_t page_size, std::int64_t head_dim, DType dtype, bool fp4,
+                                    int device_id) {
+  const dli_dtype kind = fp4 ? DLI_DTYPE_FP4 : cDtype(dtype);
+  const auto bytes = static_cast<std::int64_t>(dli_sm100_paged_kv_page_bytes(heads, page_size, head_dim, kind));
+  if (num_pages <= 0 || bytes == 0) throw std::invalid_argument("KV cache: bad size of pages for " + name);
+  const std::vector<std::int64_t> shape =
+      fp4 ? std::vector<std::int64_t>{num_pages, heads, bytes / heads} : std::vector<std::int64_t>{num_pages, heads, page_size, head_dim};
+  const DType held = fp4 ? DType::UInt8 : dtype;
+  auto it = entries_.find(name);
+  if (it != entries_.end()) {
+    const KVCacheEntry& e = it->second;
+    if (e.page_size != page_size || e.key.shape() != shape || e.key.dtype() != held || e.key.deviceId() != device_id)
+      throw std::invalid_argument("KV cache entry " + name + " exists in another form");
+    return it->second;
+  }
+  KVCacheEntry e;
+  const auto options = at::TensorOptions().dtype(torchDType(held)).device(at::kCUDA, device_id);
+  e.key = Tensor(at::zeros(shape, options));
+  e.value = Tensor(at::zeros(shape, options));
+  e.page_size = page_size;
   entries_[name] = std::move(e);
   return entries_[name];
 }

@@ -46,6 +46,7 @@ std::string toString(DType dtype) {
     case DType::BFloat16: return "bfloat16";
     case DType::Float16: return "float16";
     case DType::Int32: return "int32";
+    case DType::UInt8: return "uint8";
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -56,6 +57,7 @@ DType dtypeFromString(const std::string& dtype) {
   if (dtype == "bfloat16") return DType::BFloat16;
   if (dtype == "float16") return DType::Float16;
   if (dtype == "int32") return DType::Int32;
+  if (dtype == "uint8") return DType::UInt8;
   throw std::invalid_argument("unknown dtype: " + dtype);
 }
 
@@ -66,6 +68,7 @@ std::size_t byteSize(DType dtype) {
     case DType::BFloat16: return 2;
     case DType::Float16: return 2;
     case DType::Int32: return 4;
+    case DType::UInt8: return 1;
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -81,6 +84,7 @@ at::ScalarType torchDType(DType dtype) {
     case DType::BFloat16: return at::kBFloat16;
     case DType::Float16: return at::kHalf;
     case DType::Int32: return at::kInt;
+    case DType::UInt8: return at::kByte;
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -92,6 +96,7 @@ DType dtypeFromTorch(at::ScalarType dtype) {
     case at::kBFloat16: return DType::BFloat16;
     case at::kHalf: return DType::Float16;
     case at::kInt: return DType::Int32;
+    case at::kByte: return DType::UInt8;
     default: break;
   }
   throw std::invalid_argument("unsupported torch tensor dtype");

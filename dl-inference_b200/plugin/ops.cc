@@ -7,7 +7,8 @@
 // add, mul, silu, relu, softmax, max_pool2d, batch_norm2d, reshape, transpose)
 // plus additive fused operators for the batched Qwen2 graphs (add_rms_norm,
 // silu_mul, qkv_rotary_cache, attention_kvcache, last_token, argmax, cast,
-// all_reduce, all_reduce_add_rms_norm, tp_argmax, linear_silu_mul).
+// all_reduce, all_reduce_add_rms_norm, tp_argmax, linear_silu_mul) and the paged
+// cache (qkv_rotary_paged, attention_paged).
 //
 // Every operator validates arity/dtype/shape on the host and throws
 // std::invalid_argument like the reference templates
@@ -50,6 +51,7 @@ dli_dtype cdt(DType d) {
     case DType::BFloat16: return DLI_DTYPE_BF16;
     case DType::Float16: return DLI_DTYPE_F16;
     case DType::Int32: return DLI_DTYPE_I32;
+    case DType::UInt8: break;  // bytes of 4-bit pages, no operand of a kernel by themselves
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -637,6 +639,7 @@ class AttentionKvCacheOp final : public dli::Operator {
     if (ctx.kv_cache == nullptr) throw std::invalid_argument("attention_kvcache missing KV cache");
     const dli::KVCacheEntry* e = ctx.kv_cache->get(attrs.require<std::string>("kv_cache"));
     if (e == nullptr) throw std::invalid_argument("attention_kvcache: unknown cache entry");
+    if (e->page_size != 0) throw std::invalid_argument("attention_kvcache: the cache entry is paged");
     const std::int64_t b = q.dim(0), s = q.dim(1), hq = q.dim(2), d = q.dim(3);
     const std::int64_t hkv = e->key.dim(1), cap = e->capacity();
     if (e->key.dim(0) != b || e->key.dim(3) != d || hq % hkv != 0)
@@ -648,6 +651,107 @@ class AttentionKvCacheOp final : public dli::Operator {
     check(dli_sm100_attention_kvcache(dli::ptr(q), e->key.deviceData(), e->value.deviceData(),
                                       static_cast<const std::int64_t*>(dli::ptr(pos)), out[0]->deviceData(), b, s,
                                       hq, hkv, cap, d, scale, dt, wsPtr(ws), wsBytes(ws), ctx.cuda_stream),
+          type());
+  }
+};
+
+// Page table of the paged operators: int32 [B, max_pages].
+void requirePageTable(const Tensor& table, std::int64_t b, const std::string& op) {
+  if (table.dtype() != DType::Int32 || table.rank() != 2 || table.dim(0) != b)
+    throw std::invalid_argument(op + " expects an int32 page table [B, max_pages]");
+}
+
+// qkv_rotary_paged: (qkv [B,S,(Hq+2Hkv)*D], cos, sin, positions int64 [B], page_table
+// int32 [B, max_pages]) -> rotated q [B,S,Hq,D]; rotated k and v go to the pages of the
+// cache entry. Attributes as qkv_rotary_cache, with page_size and num_pages instead of
+// capacity, and kv_dtype = "fp4" (with k_scale, v_scale) for 4-bit pages.
+class QkvRotaryPagedOp final : public dli::Operator {
+ public:
+  std::string type() const override { return "qkv_rotary_paged"; }
+  void compute(const Inputs& in, const Outputs& out, const Attributes& attrs, ExecutionContext& ctx) const override {
+    arity(in, out, 5, 5, 1, type());
+    dli::requireCudaInputs(in, type());
+    const Tensor& qkv = *in[0];
+    dli::requireFloat(qkv, type());
+    const Tensor& cos = *in[1];
+    const Tensor& sin = *in[2];
+    const Tensor& pos = *in[3];
+    const Tensor& table = *in[4];
+    if (cos.dtype() != DType::Float32 || sin.dtype() != DType::Float32 || cos.shape() != sin.shape() || cos.rank() != 2)
+      throw std::invalid_argument(type() + " expects float32 cos/sin [max_pos, pairs]");
+    if (pos.dtype() != DType::Int64) throw std::invalid_argument(type() + " positions must be int64");
+    const std::int64_t hq = requireIntAttr(attrs, "q_heads", type());
+    const std::int64_t hkv = requireIntAttr(attrs, "kv_heads", type());
+    const std::int64_t d = requireIntAttr(attrs, "head_dim", type());
+    const std::int64_t page = requireIntAttr(attrs, "page_size", type());
+    const std::int64_t pages = requireIntAttr(attrs, "num_pages", type());
+    const std::string kind = attrs.value_or<std::string>("kv_dtype", "");
+    if (!kind.empty() && kind != "fp4") throw std::invalid_argument(type() + ": kv_dtype is \"fp4\" or absent");
+    const std::string& name = attrs.require<std::string>("kv_cache");
+    if (hq <= 0 || hkv <= 0 || d <= 0 || qkv.rank() != 3 || qkv.shape().back() != (hq + 2 * hkv) * d)
+      throw std::invalid_argument(type() + " expects qkv [B,S,(Hq+2Hkv)*D]");
+    const std::int64_t b = qkv.dim(0), s = qkv.dim(1);
+    if (static_cast<std::int64_t>(pos.numel()) != b) throw std::invalid_argument(type() + " positions must be [B]");
+    requirePageTable(table, b, type());
+    if (ctx.kv_cache == nullptr) throw std::invalid_argument(type() + " missing KV cache");
+    dli::KVCacheEntry& e =
+        ctx.kv_cache->reservePaged(name, pages, hkv, page, d, qkv.dtype(), kind == "fp4", qkv.deviceId());
+    *out[0] = Tensor::cuda(qkv.dtype(), {b, s, hq, d}, qkv.deviceId());
+    check(dli_sm100_qkv_rotary_paged(
+              dli::ptr(qkv), static_cast<const float*>(dli::ptr(cos)), static_cast<const float*>(dli::ptr(sin)),
+              static_cast<const std::int64_t*>(dli::ptr(pos)), nullptr, static_cast<const std::int32_t*>(dli::ptr(table)),
+              out[0]->deviceData(), e.key.deviceData(), e.value.deviceData(), b * s, b, s, hq, hkv, d, cos.dim(1),
+              cos.dim(0), page, pages, table.dim(1), static_cast<float>(dli::attrDouble(attrs, "k_scale", 1.0)),
+              static_cast<float>(dli::attrDouble(attrs, "v_scale", 1.0)), cdt(qkv.dtype()),
+              kind == "fp4" ? DLI_DTYPE_FP4 : cdt(qkv.dtype()), ctx.cuda_stream),
+          type());
+  }
+};
+
+// attention_paged: (q [B,S,Hq,D], positions int64 [B], page_table int32 [B, max_pages]
+// (, slopes float32 [Hq])) -> [B,S,Hq*D] over the pages that qkv_rotary_paged wrote.
+// Attributes kv_cache, and optionally scale, softcap, window, k_scale, v_scale.
+class AttentionPagedOp final : public dli::Operator {
+ public:
+  std::string type() const override { return "attention_paged"; }
+  void compute(const Inputs& in, const Outputs& out, const Attributes& attrs, ExecutionContext& ctx) const override {
+    arity(in, out, 3, 4, 1, type());
+    dli::requireCudaInputs(in, type());
+    const Tensor& q = *in[0];
+    const Tensor& pos = *in[1];
+    const Tensor& table = *in[2];
+    dli::requireFloat(q, type());
+    if (q.rank() != 4) throw std::invalid_argument(type() + " expects q [B,S,Hq,D]");
+    const std::int64_t b = q.dim(0), s = q.dim(1), hq = q.dim(2), d = q.dim(3);
+    if (pos.dtype() != DType::Int64 || static_cast<std::int64_t>(pos.numel()) != b)
+      throw std::invalid_argument(type() + " positions must be int64 [B]");
+    requirePageTable(table, b, type());
+    const Tensor* slopes = in.size() == 4 ? in[3] : nullptr;
+    if (slopes != nullptr && (slopes->dtype() != DType::Float32 || static_cast<std::int64_t>(slopes->numel()) != hq))
+      throw std::invalid_argument(type() + " slopes must be float32 [Hq]");
+    if (ctx.kv_cache == nullptr) throw std::invalid_argument(type() + " missing KV cache");
+    const dli::KVCacheEntry* e = ctx.kv_cache->get(attrs.require<std::string>("kv_cache"));
+    if (e == nullptr) throw std::invalid_argument(type() + ": unknown cache entry");
+    if (e->page_size == 0) throw std::invalid_argument(type() + ": the cache entry is not paged");
+    const bool fp4 = e->key.dtype() == DType::UInt8;
+    const std::int64_t pages = e->key.dim(0), hkv = e->key.dim(1), row = e->key.dim(2) / (fp4 ? e->page_size : 1);
+    if (hq % hkv != 0 || (fp4 ? row != d / 16 * 9 || d % 16 != 0 : e->key.dim(3) != d || e->key.dtype() != q.dtype()))
+      throw std::invalid_argument(type() + " q/cache shape mismatch");
+    *out[0] = Tensor::cuda(q.dtype(), {b, s, hq * d}, q.deviceId());
+    const dli_dtype dt = cdt(q.dtype()), kind = fp4 ? DLI_DTYPE_FP4 : dt;
+    at::Tensor ws = workspace(dli_sm100_attention_paged_workspace_size(b * s, b, s, hq, hkv, d, e->page_size,
+                                                                       table.dim(1), dt, kind),
+                              q.deviceId());
+    check(dli_sm100_attention_paged(
+              dli::ptr(q), e->key.deviceData(), e->value.deviceData(), static_cast<const std::int64_t*>(dli::ptr(pos)),
+              nullptr, static_cast<const std::int32_t*>(dli::ptr(table)),
+              slopes == nullptr ? nullptr : static_cast<const float*>(dli::ptr(*slopes)), out[0]->deviceData(), b * s,
+              b, s, hq, hkv, d, e->page_size, pages, table.dim(1),
+              static_cast<float>(dli::attrDouble(attrs, "scale", 0.0)),
+              static_cast<float>(dli::attrDouble(attrs, "softcap", 0.0)), attrs.value_or<std::int64_t>("window", 0),
+              static_cast<float>(dli::attrDouble(attrs, "k_scale", 1.0)),
+              static_cast<float>(dli::attrDouble(attrs, "v_scale", 1.0)), dt, kind, wsPtr(ws), wsBytes(ws),
+              ctx.cuda_stream),
           type());
   }
 };
@@ -946,6 +1050,8 @@ extern "C" bool dli_register_operators(dli::OperatorRegistry* registry) {
   reg<LinearSiluMulOp>(registry, "linear_silu_mul");
   reg<QkvRotaryCacheOp>(registry, "qkv_rotary_cache");
   reg<AttentionKvCacheOp>(registry, "attention_kvcache");
+  reg<QkvRotaryPagedOp>(registry, "qkv_rotary_paged");
+  reg<AttentionPagedOp>(registry, "attention_paged");
   reg<LastTokenOp>(registry, "last_token");
   reg<ArgmaxOp>(registry, "argmax");
   reg<CastOp>(registry, "cast");

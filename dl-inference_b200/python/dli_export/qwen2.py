@@ -10,7 +10,9 @@ fp32, to what the plugin serves:
   cache row of each sequence's first token), so one graph serves prefill and
   every decode step (the reference bakes start_pos at 0, export.py:350-356);
 * a preallocated KV cache addressed by position (fused `qkv_rotary_cache`
-  writes rotated k and v into the rows, `attention_kvcache` reads them);
+  writes rotated k and v into the rows, `attention_kvcache` reads them), or a
+  pool of 16-bit or 4-bit pages addressed through a `page_table` input
+  (`qkv_rotary_paged`, `attention_paged`);
 * fused QKV and gate/up projections, `add_rms_norm` for residual + norm,
   `silu_mul` for SwiGLU, and an LM head over the last token only;
 * bf16/fp16 weights (the reference casts every weight to fp32, weights.py:39-40);
@@ -186,7 +188,8 @@ def build_graph(shape: Qwen2Shape, capacity: int, tp_size: int = 1, model_type: 
                 weights_file: str = "", with_argmax: bool = True, fused_glu: bool = True,
                 logits_dtype: str | None = "float32",
                 residual_dtype: str | None = "float32", fused_exchange: bool = True,
-                fused_qkv_rotary: bool = True) -> dict[str, Any]:
+                fused_qkv_rotary: bool = True, page_size: int = 0, num_pages: int = 0,
+                kv_dtype: str | None = None) -> dict[str, Any]:
     """dli.graph.v1 dict for one rank. Inputs: input_ids [B,S] int64, positions [B]
     int64, rotary_cos/rotary_sin, and the weights of transform_weights() (made
     with the same `fused_glu`: one linear_silu_mul node instead of linear +
@@ -203,7 +206,13 @@ def build_graph(shape: Qwen2Shape, capacity: int, tp_size: int = 1, model_type: 
     GEMM pushes its partial rows into the group's exchange buffers itself.
     `fused_qkv_rotary` makes the q|k|v projection and its rotary + KV-cache
     write one `linear_qkv_rotary_cache` node (decode GEMMs rotate and scatter
-    in their epilogue)."""
+    in their epilogue). `page_size` > 0 keeps the cache in a pool of `num_pages`
+    pages of that many rows, of the weights' dtype or with kv_dtype = "fp4" of 4
+    bits: the graph then has a third input, page_table (int32 [B, max_pages])."""
+    if page_size < 0 or (page_size > 0) != (num_pages > 0):
+        raise ValueError("a paged cache needs page_size and num_pages")
+    if kv_dtype not in (None, "fp4") or (kv_dtype and not page_size):
+        raise ValueError('kv_dtype is None, or "fp4" with a paged cache')
     hq, hkv, d = shape.q_heads // tp_size, shape.kv_heads // tp_size, shape.head_dim
     nodes: list[dict[str, Any]] = []
 
@@ -239,7 +248,13 @@ def build_graph(shape: Qwen2Shape, capacity: int, tp_size: int = 1, model_type: 
             resid = f"{L}.h_in"
         rot_attrs = {"q_heads": hq, "kv_heads": hkv, "head_dim": d, "capacity": int(capacity),
                      "kv_cache": f"layer_{i}"}
-        if fused_qkv_rotary:
+        if page_size:
+            pool = {"kv_cache": f"layer_{i}", "page_size": int(page_size), "num_pages": int(num_pages)}
+            node(f"{L}.qkv_proj", "linear", [f"{L}.x", f"{L}.wqkv", f"{L}.bqkv"], [f"{L}.qkv"])
+            node(f"{L}.rotary_cache", "qkv_rotary_paged",
+                 [f"{L}.qkv", "rotary_cos", "rotary_sin", "positions", "page_table"], [f"{L}.q"],
+                 {"q_heads": hq, "kv_heads": hkv, "head_dim": d, **pool, **({"kv_dtype": kv_dtype} if kv_dtype else {})})
+        elif fused_qkv_rotary:
             node(f"{L}.qkv_proj", "linear_qkv_rotary_cache",
                  [f"{L}.x", f"{L}.wqkv", f"{L}.bqkv", "rotary_cos", "rotary_sin", "positions"], [f"{L}.q"],
                  rot_attrs)
@@ -247,8 +262,12 @@ def build_graph(shape: Qwen2Shape, capacity: int, tp_size: int = 1, model_type: 
             node(f"{L}.qkv_proj", "linear", [f"{L}.x", f"{L}.wqkv", f"{L}.bqkv"], [f"{L}.qkv"])
             node(f"{L}.rotary_cache", "qkv_rotary_cache",
                  [f"{L}.qkv", "rotary_cos", "rotary_sin", "positions"], [f"{L}.q"], rot_attrs)
-        node(f"{L}.attention", "attention_kvcache", [f"{L}.q", "positions"], [f"{L}.attn"],
-             {"kv_cache": f"layer_{i}"})
+        if page_size:
+            node(f"{L}.attention", "attention_paged", [f"{L}.q", "positions", "page_table"], [f"{L}.attn"],
+                 {"kv_cache": f"layer_{i}"})
+        else:
+            node(f"{L}.attention", "attention_kvcache", [f"{L}.q", "positions"], [f"{L}.attn"],
+                 {"kv_cache": f"layer_{i}"})
         project_add_norm(f"{L}.post_attention_layernorm", resid, f"{L}.attn", f"{L}.wo", f"{L}.ln_post",
                          [f"{L}.x2", f"{L}.h_mid"], f"{L}.o_proj", f"{L}.o_part")
         resid = f"{L}.h_mid"
@@ -269,7 +288,8 @@ def build_graph(shape: Qwen2Shape, capacity: int, tp_size: int = 1, model_type: 
         node("greedy", "tp_argmax" if vocab_parallel(shape, tp_size) else "argmax", ["logits"], ["next_ids"])
         outputs.append("next_ids")
     return {"format": "dli.graph.v1", "model_type": model_type, "weights": weights_file,
-            "inputs": ["input_ids", "positions"], "outputs": outputs, "nodes": nodes}
+            "inputs": ["input_ids", "positions"] + (["page_table"] if page_size else []), "outputs": outputs,
+            "nodes": nodes}
 
 
 def random_state(shape: Qwen2Shape, device="cpu", dtype=torch.bfloat16, seed: int = 0,
@@ -333,9 +353,11 @@ def write_weights(tensors: dict[str, torch.Tensor], out_dir: Path, stem: str) ->
 
 def export_qwen2(model_or_state: Any, out_dir: str | Path, stem: str = "qwen2",
                  shape: Qwen2Shape | None = None, capacity: int = 4096, tp_size: int = 1,
-                 tp_rank: int = 0, dtype: torch.dtype = torch.bfloat16) -> tuple[Path, Path]:
+                 tp_rank: int = 0, dtype: torch.dtype = torch.bfloat16, page_size: int = 0,
+                 num_pages: int = 0, kv_dtype: str | None = None) -> tuple[Path, Path]:
     """Writes <stem>.dli.json and <stem>.dli.weights.{json,bin} for one TP rank.
-    `model_or_state` is an HF Qwen2ForCausalLM or its state dict."""
+    `model_or_state` is an HF Qwen2ForCausalLM or its state dict. page_size,
+    num_pages and kv_dtype choose a paged cache, as in build_graph."""
     out = Path(out_dir)
     if hasattr(model_or_state, "state_dict"):
         shape = shape or Qwen2Shape.from_hf(model_or_state.config)
@@ -349,7 +371,8 @@ def export_qwen2(model_or_state: Any, out_dir: str | Path, stem: str = "qwen2",
     cos, sin = rotary_tables(shape, capacity)
     weights["rotary_cos"], weights["rotary_sin"] = cos, sin
     wpath = write_weights(weights, out, stem)
-    graph = build_graph(shape, capacity, tp_size, weights_file=wpath.name, fused_glu=fused)
+    graph = build_graph(shape, capacity, tp_size, weights_file=wpath.name, fused_glu=fused,
+                        page_size=page_size, num_pages=num_pages, kv_dtype=kv_dtype)
     gpath = out / f"{stem}.dli.json"
     gpath.write_text(json.dumps(graph, indent=1), encoding="utf-8")
     meta = {"shape": asdict(shape), "capacity": capacity, "tp_size": tp_size, "tp_rank": tp_rank}

@@ -4,7 +4,8 @@ Executes a graph dict node by node with the numpy oracle (float64), keeping a
 position-addressed KV cache for the fused `qkv_rotary_cache` /
 `attention_kvcache` operators and an appending cache for the reference's
 `attention` with a `kv_cache` attribute (python/dli_ops/aot/attention/
-template.cc:10-18). Used to check exported graphs against the source model on
+template.cc:10-18). The paged operators keep rows per page, found through the
+page table; 4-bit pages hold the values the codes stand for. Used to check exported graphs against the source model on
 CPU; never used by the product path.
 """
 from __future__ import annotations
@@ -12,6 +13,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import ops as O
+from . import paged as P
 
 
 class GraphOracle:
@@ -85,6 +87,10 @@ class GraphOracle:
             return [self._qkv_rotary_cache([O.linear(x[0], x[1], x[2])] + list(x[3:]), a)]
         if op == "attention_kvcache":
             return [self._attention_kvcache(x, a)]
+        if op == "qkv_rotary_paged":
+            return [self._qkv_rotary_paged(x, a)]
+        if op == "attention_paged":
+            return [self._attention_paged(x, a)]
         if op in ("add", "mul", "silu", "relu", "softmax"):
             return [getattr(O, op)(*x)]
         if op == "reshape":
@@ -109,6 +115,39 @@ class GraphOracle:
             entry["k"][i, :, p:p + s] = rk[i]
             entry["v"][i, :, p:p + s] = v[i]
         return rq.transpose(0, 2, 1, 3)
+
+    def _qkv_rotary_paged(self, x, a):
+        qkv, cos, sin, pos, table = (np.asarray(t) for t in x)
+        hq, hkv, d, size = a["q_heads"], a["kv_heads"], a["head_dim"], a["page_size"]
+        b, s = qkv.shape[:2]
+        t = qkv.astype(np.float64).reshape(b, s, hq + 2 * hkv, d)
+        pool = self.cache.setdefault(a["kv_cache"], {"k": np.zeros((a["num_pages"], size, hkv, d)),
+                                                     "v": np.zeros((a["num_pages"], size, hkv, d))})
+        out = np.empty((b, s, hq, d))
+        for i in range(b):
+            p = int(pos[i]) + np.arange(s)
+            rot = P.rotate(t[i, :, :hq + hkv], cos[p], sin[p])
+            out[i], k, v = rot[:, :hq], rot[:, hq:], t[i, :, hq + hkv:]
+            if a.get("kv_dtype") == "fp4":
+                sk, sv = a.get("k_scale", 1.0), a.get("v_scale", 1.0)
+                k, v = P.fp4_values(*P.fp4_codes(k, sk), sk), P.fp4_values(*P.fp4_codes(v, sv), sv)
+            pool["k"][table[i, p // size], p % size] = k
+            pool["v"][table[i, p // size], p % size] = v
+        return out
+
+    def _attention_paged(self, x, a):
+        q, pos, table = np.asarray(x[0], dtype=np.float64), np.asarray(x[1]), np.asarray(x[2])
+        pool = self.cache[a["kv_cache"]]
+        b, s, hq, d = q.shape
+        size = pool["k"].shape[1]
+        out = np.zeros((b, s, hq * d))
+        for i in range(b):
+            rows = np.arange(int(pos[i]) + s)
+            k, v = (pool[n][table[i, rows // size], rows % size].transpose(1, 0, 2) for n in ("k", "v"))
+            o, _, _ = P.attention(q[i], k, v, int(pos[i]), a.get("scale") or d ** -0.5, a.get("softcap", 0.0),
+                                  a.get("window", 0), np.asarray(x[3]) if len(x) > 3 else None)
+            out[i] = o.reshape(s, hq * d)
+        return out
 
     def _attention_kvcache(self, x, a):
         q, pos = np.asarray(x[0], dtype=np.float64), np.asarray(x[1])
