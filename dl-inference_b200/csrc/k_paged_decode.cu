@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
     bool alive = true;
     while (alive && walk.get(seg)) {
       const int32_t* ids = a.seqs.page_table + seg.b * a.seqs.max_pages;
-      const int last_page = (seg.w.kv_len - 1) >> shift;
+      const int first_page = seg.w.key_lo >> shift, last_page = (seg.w.kv_len - 1) >> shift;  // others may be gone
       const int none = static_cast<int>(a.seqs.num_pages);  // outside the map: reads as zeros
       auto fetch = [&](int chunk) {
         const int i = chunk * 32 + lane;
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
           nxt = fetch(chunk + 1);
         }
         int page = __shfl_sync(0xffffffffu, cur, (first + lane) & 31);
-        if (first + lane > last_page) page = none;
+        if (first + lane < first_page || first + lane > last_page) page = none;
         else if (lane < boxes && (page < 0 || page >= none)) {
           set_device_error(a.seqs.err, kDevErrPageIndex);
           page = none;

@@ -367,11 +367,11 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
       ok = tiles.put(x, lane) && ok;
       if (!ok || x.nblocks == 0) break;
       const int32_t* ids = a.seqs.page_table + x.b * a.seqs.max_pages;
-      const int last_page = (x.kv_len - 1) >> shift;
+      const int first_page = x.key_lo >> shift, last_page = (x.kv_len - 1) >> shift;  // others may be gone
       auto page_for = [&](int j) {  // of lane's box of step j
         int page = none;
         const int i = j < x.nblocks ? (x.key_of(j) >> shift) + lane : 0;
-        if (lane < boxes && j < x.nblocks && i <= last_page) {
+        if (lane < boxes && j < x.nblocks && i >= first_page && i <= last_page) {
           page = ids[i];
           if (page < 0 || page >= none) {
             set_device_error(a.seqs.err, kDevErrPageIndex);
