@@ -686,7 +686,6 @@ extern "C" size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64
   if (page_shift_of(page_size) < 0 || max_pages <= 0 || max_pages > (1ll << 30) / page_size) return 0;
   if (!is_float_dtype(dtype) || (head_dim != 64 && head_dim != 128)) return 0;
   const int64_t group = q_heads / kv_heads, max_keys = max_pages * page_size;
-  (void)kv_dtype;
   if (few_rows(dtype, kv_dtype == DLI_DTYPE_FP4, group, max_new)) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys, dtype);
   return paged_prefill_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
 }

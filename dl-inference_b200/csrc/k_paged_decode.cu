@@ -57,17 +57,19 @@ struct DecodeArgs {
 };
 
 // W consumer warps: 4, or 8 where the ring's entries are small enough. Two CTAs per
-// SM (float32 and two row tiles of 4-bit pages: one).
+// SM, one works while the other waits (float32, 32 x 1501 keys, 16/4 heads: one CTA of 8
+// warps 43.4 us, two of 4 39.2, although a few registers spill);
+// 4-bit pages three, or one with two row tiles or split float32 operands.
 template <typename T, typename KV, int D, int NT>
 struct DecodeLayout {
   static constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
   static constexpr bool kF32 = std::is_same<KV, float>::value;
-  static constexpr int W = kF32 || (!kFp4 && D == 64 && NT == 1) ? 8 : 4;
+  static constexpr int W = !kFp4 && !kF32 && D == 64 && NT == 1 ? 8 : 4;
   static constexpr int SUB = kFp4 ? 2 : 1;  // 16-key groups of a warp per block
   static constexpr int kThreads = 32 * W + 32;
   static constexpr int R = 8 * NT;
   static constexpr int BN = 16 * W * SUB;  // keys per block
-  static constexpr int kCtas = kF32 || (kFp4 && (NT == 2 || std::is_same<T, float>::value)) ? 1 : kFp4 ? 3 : 2;
+  static constexpr int kCtas = kFp4 && (NT == 2 || std::is_same<T, float>::value) ? 1 : kFp4 ? 3 : 2;
   static constexpr int kRowBytes = kFp4 ? D / 2 : kF32 ? D * 4 : D * 2;
   static constexpr int kBox = BN * 128;          // bytes of one 128-byte-wide column of boxes
   static constexpr int kCodes = BN * kRowBytes;  // code or element bytes of a K (or V) block
@@ -1037,10 +1039,12 @@ struct DecodePlan {
   size_t part_o, part_ml, workspace;
 };
 
-// Shares of a split call are at least kMinKeys keys; a call whose sequences cannot
-// exceed kWholeKeys runs one CTA per unit.
+// Shares of a split call are at least kMinKeys keys (1 x 1501 keys, us with 64 | 128 |
+// 256 | 512: 28/4 heads 16 bits 8.3 | 8.4 | 9.9 | 13.5, 4 bits 8.5 | 8.5 | 9.6 | 11.9,
+// float32 16/4 heads 11.7 | 11.6 | 14.9 | 21.4; nothing changes where every CTA has
+// more); a call whose sequences cannot exceed kWholeKeys runs one CTA per unit.
 constexpr int kWholeKeys = 512;
-constexpr int kMinKeys = 256;
+constexpr int kMinKeys = 128;
 constexpr int kMaxCtasPerSm = 3;
 
 DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys,
