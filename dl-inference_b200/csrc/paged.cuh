@@ -38,7 +38,7 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedSeqs& s, int b, bool repo
     return r;
   }
   const int64_t past = s.positions[b];
-  if (past < 0 || past + (s1 - s0) > (s.max_pages << s.page_shift)) {
+  if (past < 0 || past > (s.max_pages << s.page_shift) - (s1 - s0)) {
     if (report && s1 > s0) set_device_error(s.err, kDevErrKvCapacity);
     return r;
   }

@@ -520,7 +520,7 @@ def qkv_rotary_paged(qkv, cos, sin, positions, page_table, k_pages, v_pages, q_h
     if cos.shape != sin.shape or cos.dim() != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("qkv_rotary_paged: cos and sin must be float32 [rows, pairs]")
     if q_out is None:
-        q_out = torch.empty((tokens, q_heads, d), dtype=qkv.dtype, device=qkv.device)
+        q_out = qkv.new_empty((tokens, q_heads, d))
     elif q_out.dtype != qkv.dtype or q_out.numel() != tokens * q_heads * d:
         raise ValueError("qkv_rotary_paged: q_out must be [rows, q_heads, head_dim] of qkv's dtype")
     dev = _device(what, qkv, cos, sin, positions, page_table, k_pages, v_pages, starts, q_out)
@@ -579,7 +579,7 @@ def paged_gather(k_pages, v_pages, page_table, count, head_dim, dtype, first=Non
         if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or t.numel() != b):
             raise ValueError("paged_gather: first and lengths must be int64 [batch]")
     dev = _device(what, k_pages, v_pages, page_table, first, lengths)
-    both = torch.empty((2, b, hkv, count, head_dim), dtype=dtype, device=k_pages.device)
+    both = k_pages.new_empty((2, b, hkv, count, head_dim), dtype=dtype)
     k, v = both.unbind(0)
     _launch(what, dev, lib().dli_sm100_paged_gather, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
             _at(first), _at(lengths), k.data_ptr(), v.data_ptr(), b, count, hkv, head_dim, page_size, num_pages,

@@ -339,3 +339,42 @@ def test_gather_and_append_on_another_stream_and_many_pages():
     for (a, b) in results:
         for x, y in zip(a, b):
             assert torch.equal(x, y) and torch.isfinite(x).all()
+
+
+@pytest.mark.parametrize("fp4", [False, True], ids=["rows16", "rows4"])
+def test_positions_and_lengths_at_the_ends_of_their_type(fp4):
+    """The largest and smallest int64 as positions or lengths: reported, nothing written, the other sequences served."""
+    hkv, d, page, hq = 2, 64, 16, 4
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    one = torch.ones(64, 1, device="cuda")
+    qkv = torch.randn(2, (hq + 2 * hkv) * d, device="cuda").to(BF)
+    for far in (2 ** 63 - 1, 2 ** 63 - 2, -2 ** 63, 2 ** 32, 2 ** 31 - 1):
+        k, v = C.paged_kv_pages(4, hkv, page, d, "fp4" if fp4 else BF)
+        k.fill_(1), v.fill_(1)
+        kept = k[2:].clone()
+        pos = torch.tensor([3, far], device="cuda")
+        q = torch.full((2, hq, d), 7.0, dtype=BF, device="cuda")
+        C.qkv_rotary_paged(qkv, one, one * 0, pos, table, k, v, hq, q_out=q)
+        with pytest.raises(RuntimeError):
+            C.check_device_error()
+        assert torch.equal(k[2:], kept) and (q[1] == 7).all() and torch.equal(q[0], qkv[0, :hq * d].view(hq, d))
+        for rows in (1, 40):  # the decode kernel, the tcgen05 kernel
+            out = torch.full((2 * rows, hq, d), 7.0, dtype=BF, device="cuda")
+            big = torch.tensor([[0, 1, 0, 1], [2, 3, 2, 3]], dtype=torch.int32, device="cuda")
+            C.attention_paged(torch.zeros_like(out), k, v, pos, big, out=out)
+            with pytest.raises(RuntimeError):
+                C.check_device_error()
+            assert (out[rows:] == 7).all() and torch.isfinite(out[:rows]).all() and (out[:rows] != 7).all()
+        # past every row: zeros, with an error only where a bound is outside the table's
+        kk, vv = C.paged_gather(k, v, table, 5, d, BF, first=pos)
+        assert (kk[1] == 0).all() and (vv[1] == 0).all() and kk[0].abs().sum() > 0
+        if far < 0:
+            with pytest.raises(RuntimeError):
+                C.check_device_error()
+        C.check_device_error()
+        kk, _ = C.paged_gather(k, v, table, 32, d, BF, lengths=pos)
+        assert kk[0, :, :3].abs().sum() > 0 and (kk[0, :, 3:] == 0).all()
+        if far > 0:
+            with pytest.raises(RuntimeError):
+                C.check_device_error()
+        C.check_device_error()
