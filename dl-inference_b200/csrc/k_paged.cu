@@ -422,34 +422,75 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
 }
 
 // ---- attention, any head dim up to 256, any type --------------------------------------
-// One warp per (packed row, query head): lane j scores key j of a 32-key chunk
-// against the row's q (shared memory), the online softmax runs across the warp,
-// and for O += p V each lane owns the elements lane, lane + 32, ... In fp32.
+// One CTA per (packed row, query head), in fp32. Its warps take 32-key chunks in turn:
+// lane j scores key j against the row's q (shared memory), the online softmax runs across
+// the warp, and for O += p V each lane owns the elements lane, lane + 32, ...; the warps'
+// (max, sum, O) are merged in order. It serves what the tensor-core kernels do not (other
+// head dims, tensors off their alignment) and is bound by issue and by K and V rows that
+// are fetched per query head: 8 x 1 token over 1000 keys, 16/4 heads of 80, bf16, 61 us
+// (one warp per row and head 476 us), of 256 77 us, 4-bit pages of 96 83 us.
+constexpr int kGeneralWarps = 8;
+
+// sum of q[c] * K[c] over the row pr of a block at `block` (of one head of a page)
 template <typename T, typename KV>
-__global__ void __launch_bounds__(128) attn_paged_general_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ float general_dot(const float* sq, const void* pages, int64_t block, int page_rows, int d, int pr,
+                                             bool vec) {
+  float dot = 0.f;
+  if constexpr (std::is_same<KV, Fp4>::value) {
+    const uint8_t* base = static_cast<const uint8_t*>(pages) + block * fp4_block_bytes(page_rows, d);
+    for (int c = 0; c < d; c += 16) {
+      const uint2 w = *reinterpret_cast<const uint2*>(base + pr * (d / 2) + c / 2);
+      const float s = e4m3_value(base[page_rows * (d / 2) + pr * (d / 16) + c / 16]) * 16384.f;
+      float part = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) part = fmaf(sq[c + j], e2m1_small(((j < 8 ? w.x : w.y) >> (4 * (j & 7))) & 15u), part);
+      dot = fmaf(part, s, dot);
+    }
+  } else {
+    const T* k = static_cast<const T*>(pages) + (block * page_rows + pr) * d;
+    int c = 0;
+    if (vec) {
+      constexpr int N = Vec16<T>::N;
+#pragma unroll 4
+      for (; c + N <= d; c += N) {
+        const Vec16<T> v = load16(k + c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) dot = fmaf(sq[c + j], to_f32(v.e[j]), dot);
+      }
+    }
+    for (; c < d; ++c) dot = fmaf(sq[c], to_f32(k[c]), dot);
+  }
+  return dot;
+}
+
+template <typename T, typename KV>
+__global__ void __launch_bounds__(32 * kGeneralWarps) attn_paged_general_kernel(const PagedAttnArgs a, bool vec) {
   DLI_PDL_ENTRY();
   constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
-  extern __shared__ float sq_all[];
+  constexpr int W = kGeneralWarps;
+  extern __shared__ float general_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.y, d = a.head_dim;
-  const SeqRows sr = seq_rows(a.seqs, b, threadIdx.x == 0);
+  float* sq = general_smem;  // [d]
+  float* so = sq + d;        // [W][d]
+  float* sm = so + W * d;    // [W], then the sums [W]
+  const SeqRows sr = seq_rows(a.seqs, b, threadIdx.x == 0 && blockIdx.x == 0);
   const int page_rows = 1 << a.seqs.page_shift;
-  float* sq = sq_all + warp * d;
-  for (int64_t i = blockIdx.x * 4ll + warp; i < static_cast<int64_t>(sr.n) * a.hq; i += gridDim.x * 4ll) {
+  for (int64_t i = blockIdx.x; i < static_cast<int64_t>(sr.n) * a.hq; i += gridDim.x) {
     const int t = static_cast<int>(i / a.hq), h = static_cast<int>(i - static_cast<int64_t>(t) * a.hq);
     const int kvh = h / a.group, pos = sr.past + t;
     const int64_t at = ((sr.row0 + t) * a.hq + h) * d;
-    __syncwarp();
-    for (int c = lane; c < d; c += 32) sq[c] = to_f32(static_cast<const T*>(a.q)[at + c]);
-    __syncwarp();
+    __syncthreads();
+    for (int c = threadIdx.x; c < d; c += 32 * W) sq[c] = to_f32(static_cast<const T*>(a.q)[at + c]);
+    __syncthreads();
     const float slope = a.slopes ? a.slopes[h] : 0.f;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     const int key_lo = max(0, pos - a.window + 1);
-    for (int j0 = key_lo; j0 <= pos; j0 += 32) {
+    for (int j0 = key_lo + 32 * warp; j0 <= pos; j0 += 32 * W) {
       const int j = j0 + lane;
       float x = -INFINITY;
-      int64_t row = -1;  // element (or byte block) index of this lane's key row
+      int64_t row = -1;  // (page, head) block of this lane's key
       int pr = 0;
       if (j <= pos) {
         const int page = page_of(a.seqs, b, j);
@@ -457,13 +498,7 @@ __global__ void __launch_bounds__(128) attn_paged_general_kernel(const PagedAttn
         float dot = 0.f;
         if (page >= 0) {
           row = static_cast<int64_t>(page) * a.hkv + kvh;
-          if constexpr (kFp4) {
-            const uint8_t* base = static_cast<const uint8_t*>(a.k_pages) + row * fp4_block_bytes(page_rows, d);
-            for (int c = 0; c < d; ++c) dot = fmaf(sq[c], fp4_element(base, page_rows, d, pr, c), dot);
-          } else {
-            const T* k = static_cast<const T*>(a.k_pages) + (row * page_rows + pr) * d;
-            for (int c = 0; c < d; ++c) dot = fmaf(sq[c], to_f32(k[c]), dot);
-          }
+          dot = general_dot<T, KV>(sq, a.k_pages, row, page_rows, d, pr, vec);
         }
         x = dot * a.scale;
         if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
@@ -477,6 +512,7 @@ __global__ void __launch_bounds__(128) attn_paged_general_kernel(const PagedAttn
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] *= alpha;
       const int keys = min(32, pos + 1 - j0);
+#pragma unroll 4
       for (int k = 0; k < keys; ++k) {
         const float pk = __shfl_sync(0xffffffffu, p, k);
         const int64_t rk = __shfl_sync(0xffffffffu, row, k);
@@ -495,20 +531,41 @@ __global__ void __launch_bounds__(128) attn_paged_general_kernel(const PagedAttn
         }
       }
     }
-    const float inv = a.v_scale / l;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (lane + 32 * e < d) static_cast<T*>(a.out)[at + lane + 32 * e] = from_f32<T>(o[e] * inv);
+      if (lane + 32 * e < d) so[warp * d + lane + 32 * e] = o[e];
+    if (lane == 0) {
+      sm[warp] = m;
+      sm[W + warp] = l;
+    }
+    __syncthreads();
+    // a warp without keys has m = -inf, l = 0 and O = 0
+    float top = sm[0], sum = 0.f, w[W];
+#pragma unroll
+    for (int k = 1; k < W; ++k) top = sm[k] > top || isnan(sm[k]) ? sm[k] : top;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      w[k] = sm[W + k] == 0.f ? 0.f : expf(sm[k] - top);
+      sum += sm[W + k] * w[k];
+    }
+    const float inv = a.v_scale / sum;
+    for (int c = threadIdx.x; c < d; c += 32 * W) {
+      float x = 0.f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) x = fmaf(so[k * d + c], w[k], x);
+      static_cast<T*>(a.out)[at + c] = from_f32<T>(x * inv);
+    }
   }
 }
 
 template <typename T, typename KV>
 dli_status launch_attn_general(const PagedAttnArgs& a, cudaStream_t stream) {
-  const int64_t per_seq = ceil_div(static_cast<int64_t>(a.seqs.max_new) * a.hq, 4);
+  const int64_t per_seq = static_cast<int64_t>(a.seqs.max_new) * a.hq;
   const int64_t walkers = std::min<int64_t>(per_seq, std::max<int64_t>(1, ceil_div(64ll * sm_count(), a.seqs.batch)));
+  const bool vec = a.head_dim % Vec16<T>::N == 0 && aligned(a.k_pages, 16);
   launch_pdl(attn_paged_general_kernel<T, KV>,
-             dim3(static_cast<unsigned>(walkers), static_cast<unsigned>(a.seqs.batch)), dim3(128),
-             4 * a.head_dim * sizeof(float), stream, a);
+             dim3(static_cast<unsigned>(walkers), static_cast<unsigned>(a.seqs.batch)), dim3(32 * kGeneralWarps),
+             ((kGeneralWarps + 1) * a.head_dim + 2 * kGeneralWarps) * sizeof(float), stream, a, vec);
   return check_launch("attention_paged");
 }
 
