@@ -316,8 +316,15 @@ dli_status dli_sm100_qkv_rotary_paged(const void* qkv, const float* cos_table, c
  * window > 0 only i - window < j. Score of (i, j) in head h: x = scale * q . k;
  * softcap > 0: x = softcap * tanh(x / softcap); slopes (float [Hq], NULL = none):
  * x += slopes[h] * (j - i). scale <= 0 selects 1/sqrt(D). Hq must be a multiple
- * of Hkv. The workspace is scratch: nothing in it has to be
- * initialised or kept, but calls that may overlap on the GPU need their own. */
+ * of Hkv. Pages whose rows no query of the sequence sees (behind its window, or
+ * past its last row) are not looked up; their table entries may be anything.
+ * Non-finite values: in a row of q they reach only that row's heads; a cached v
+ * row reaches the rows that see it and, where it is not finite, may also reach
+ * the earlier new tokens of the same call (0 * NaN in a shared tile). out may be
+ * q itself. The workspace is scratch: nothing in it has to be initialised or
+ * kept, but calls that may overlap on the GPU need their own.
+ * Head dims 64 and 128 with 16-byte aligned tensors run on tensor cores, others on
+ * a slower general kernel. */
 size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64_t batch, int64_t max_new, int64_t q_heads,
                                                 int64_t kv_heads, int64_t head_dim, int64_t page_size,
                                                 int64_t max_pages, dli_dtype dtype, dli_dtype kv_dtype);

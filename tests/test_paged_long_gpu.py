@@ -378,3 +378,13 @@ def test_positions_and_lengths_at_the_ends_of_their_type(fp4):
             with pytest.raises(RuntimeError):
                 C.check_device_error()
         C.check_device_error()
+
+
+@pytest.mark.parametrize("name", ["tiles-bf16", "tiles-fp4", "parts", "long-parts", "decode", "decode-many", "decode-fp4",
+                                  "decode-f32", "rows-f32"])
+def test_the_output_may_be_q_itself(name):
+    c = case(name)
+    want = c.run()
+    q = c.q.clone()
+    assert torch.equal(c.run(q=q, out=q), want)
+    C.check_device_error()
