@@ -794,7 +794,9 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
   a.window = window > 0 && window < INT_MAX ? static_cast<int>(window) : INT_MAX;
   const bool fp4 = kv_dtype == DLI_DTYPE_FP4;
   a.scale = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(head_dim))) * (fp4 ? k_scale : 1.f);
-  a.softcap = softcap;
+  // caps beyond 2^64 or below 2^-64 bend nothing more (scores past 2^51 keep one key, those
+  // within 2^-64 weigh all alike), and their reciprocals stay normal
+  a.softcap = softcap > 0.f ? std::max(std::min(softcap, 0x1p64f), 0x1p-64f) : 0.f;
   a.v_scale = fp4 ? v_scale : 1.f;
   if (few_rows(dtype, fp4, a.group, max_new)) {
     if (paged_decode_serves(a, dtype)) return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));

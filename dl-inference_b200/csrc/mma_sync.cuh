@@ -88,6 +88,24 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// cap tanh(x / cap), times log2(e), from z = 2 log2(e) x / cap; cap2 = 2 cap log2(e).
+// tanh = 1 - 2 / (1 + 2^z) is off by some 2^-22 of the cap, which would drown scores far
+// below it: those (|z| < 1) take tanh's series, y - y^3/3 + 2y^5/15 - 17y^7/315 +
+// 62y^9/2835 with y = z ln(2) / 2, whose next term is below 2^-22 of the sum.
+constexpr float kHalfLn2 = 0.34657359f, kHalfLn2Sq = kHalfLn2 * kHalfLn2;
+constexpr float kTanh0 = 0.5f * kHalfLn2, kTanh1 = -kHalfLn2Sq / 3.f, kTanh2 = kHalfLn2Sq * kHalfLn2Sq * (2.f / 15.f),
+                kTanh3 = -kHalfLn2Sq * kHalfLn2Sq * kHalfLn2Sq * (17.f / 315.f),
+                kTanh4 = kHalfLn2Sq * kHalfLn2Sq * kHalfLn2Sq * kHalfLn2Sq * (62.f / 2835.f);
+__device__ __forceinline__ float capped_score(float z, float cap2) {
+  const float s = z * z;
+  float t = fmaf(s, kTanh4, kTanh3);
+  t = fmaf(s, t, kTanh2);
+  t = fmaf(s, t, kTanh1);
+  t = fmaf(s, t, 1.f) * (z * (kTanh0 * cap2));
+  const float e = fmaf(-cap2, rcp_approx(1.f + exp2_approx(z)), 0.5f * cap2);
+  return fabsf(z) < 1.f ? t : e;
+}
 // Byte I of `w` (two E2M1 codes) as two halves, the low code in the low half.
 template <int I>
 __device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t w) {

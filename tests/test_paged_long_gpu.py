@@ -388,3 +388,57 @@ def test_the_output_may_be_q_itself(name):
     q = c.q.clone()
     assert torch.equal(c.run(q=q, out=q), want)
     C.check_device_error()
+
+
+@pytest.mark.parametrize("name", ["parts", "decode", "decode-fp4", "tiles-fp4", "decode-f32", "rows-f32"])
+@pytest.mark.parametrize("softcap", [2.0 ** -130, 1e-3, 0.7, 3.0, 1e4, 1e9, 1e38])
+def test_caps_of_any_size(name, softcap):
+    """Caps far below the scores (all keys alike), around them, and far above (no cap at all): the error is one of
+    the scores' size, not of the cap's."""
+    c = case(name, softcap=softcap)
+    out = c.run()
+    C.check_device_error()
+    c.check(out)
+
+
+@pytest.mark.parametrize("name", ["tiles-bf16", "parts", "decode", "decode-fp4", "parts-fp4", "decode-f32"])
+def test_a_window_of_one_and_a_window_past_everything(name):
+    c = case(name, window=1)
+    c.check(c.run())
+    c = case(name, window=2 ** 40)
+    plain = case(name, window=0)
+    assert torch.equal(c.run(), plain.run())
+    C.check_device_error()
+
+
+@pytest.mark.parametrize("name", ["decode", "decode-fp4", "parts", "long-parts", "decode-f32"])
+def test_a_bound_on_new_rows_that_is_too_large(name):
+    """max_new may be more than any sequence has (here: all rows of the batch); rows behind the last sequence stay."""
+    c = case(name)
+    q = torch.cat([c.q, c.q[:3]])
+    out = torch.full_like(q, 5.0)
+    C.attention_paged(q, c.k, c.v, c.positions, c.table, starts=c.starts, slopes=c.slopes, out=out, **c.options)
+    C.check_device_error()
+    c.check(out)
+    assert (out[c.tokens:] == 5).all()
+    # no rows at all in a batch that has some behind it
+    out.fill_(5.0)
+    C.attention_paged(q, c.k, c.v, c.positions, c.table, starts=torch.zeros_like(c.starts), out=out)
+    C.check_device_error()
+    assert (out == 5).all()
+
+
+@pytest.mark.parametrize("fp4", [False, True], ids=["rows16", "rows4"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_sequences_that_share_their_first_pages(fp4, new):
+    """A common prefix cached once: the same bits as with a copy of it for every sequence."""
+    c = Case(HF, fp4, 8, 2, 64, 32, [320, 320, 320], [new] * 3, seed=9)
+    shared = c.table.clone()
+    shared[1:, :10] = shared[0, :10]
+    for t in (c.k, c.v):
+        for b in (1, 2):
+            t[c.table[b, :10].long()] = t[c.table[0, :10].long()]
+    want = c.run()
+    assert torch.equal(c.run(table=shared), want)
+    C.check_device_error()
+    c.check(want)
