@@ -35,8 +35,9 @@
 // Every wait is bounded; one that runs out sets the device error word and winds the
 // CTA down.
 //
-// Bound by the chain S -> softmax -> P with two softmax warps per scheduler, no pipe above
-// half: 16 prompts of up to 2048 tokens, 28/4 heads of 128, bf16: 365 us = 787 TFLOP/s
+// Bound by the chain S -> softmax -> P V -> next S of each CTA (tensor unit busy 59% of the
+// time, MUFU 39%, issue 39%, L2 26%; two threads per row, 96 registers each, 402 us
+// instead of 365): 16 prompts of up to 2048 tokens, 28/4 heads of 128, bf16: 365 us = 787 TFLOP/s
 // (466 when a grid of whole tiles had no claiming; 64 keys a block keep two CTAs in an
 // SM's tensor memory). 2 chunks of up to 383 tokens over 8000 keys, window 4096, bias, 16
 // heads of 64: 39 us (issue 40%, MUFU 35%, tensor 34% busy). 4-bit pages, 4 chunks of up
