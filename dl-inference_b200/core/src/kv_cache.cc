@@ -1,5 +1,6 @@
 #include "dli/kv_cache.h"
 
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
@@ -132,6 +133,9 @@ KVCacheEntry& KVCache::reservePaged(const std::string& name, std::int64_t num_pa
       throw std::invalid_argument("KV cache entry " + name + " exists in another form");
     return it->second;
   }
+  // a pool made under capture would be zeroed by every replay
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    throw std::runtime_error("KV cache entry " + name + " has to exist before a capture: run the graph once first");
   KVCacheEntry e;
   const auto options = at::TensorOptions().dtype(torchDType(held)).device(at::kCUDA, device_id);
   e.key = Tensor(at::zeros(shape, options));

@@ -33,7 +33,7 @@
 // chains: scores are summed in four, O in one per 16 keys, and added up in fp32.
 //
 // Bound by memory when the cache is long (3 sequences of up to 60001 keys, 64/8 heads of
-// 128: 100 us = 6.1 TB/s), by its start, the second kernel and the ragged ends when it is
+// 128: 102 us = 6.1 TB/s), by its start, the second kernel and the ragged ends when it is
 // not (32 x up to 2304 keys, 28/4 heads: 26.7 us = 4.2 TB/s; 1 x 333 keys 6 us). 4-bit
 // pages: the conversion (24 x up to 8192 keys, 28/4 heads: 34 us; ALU 51% busy, issue 57%
 // with 12 consumer warps per SM; eight per CTA spilled). float32: 32 x up to 1501 keys,

@@ -106,6 +106,27 @@ def test_cache_entries_keep_their_form():
                   {"q": bad, "pos": pos, "table": table})
 
 
+def test_a_pool_is_not_made_under_capture():
+    d = 64
+    e = _engine()
+    g = _graph([("qkv_rotary_paged", ["qkv", "cos", "sin", "pos", "table"], ["q"], _pool_attrs(1, 1, d, 16, 2, False))],
+               ["qkv", "cos", "sin", "pos", "table"], ["q"])
+    one = torch.ones(32, d // 2, device="cuda")
+    feed = {"qkv": torch.zeros(1, 1, 3 * d, device="cuda", dtype=torch.bfloat16), "cos": one, "sin": one,
+            "pos": torch.zeros(1, dtype=torch.int64, device="cuda"),
+            "table": torch.zeros(1, 2, dtype=torch.int32, device="cuda")}
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="before a capture"):
+            e.run(g, feed)
+    assert e.kv_cache_size() == 0
+    e.run(g, feed)
+    captured = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(captured):
+        e.run(g, feed)
+    captured.replay()
+    torch.cuda.synchronize()
+
+
 def _small(head_dim=64):
     from dli_export.qwen2 import Qwen2Shape
 
