@@ -159,10 +159,10 @@ struct Row {
 // loads. A thread owns V elements of a token's head and takes NP heads a step, whose loads
 // are asked for together: 24 ragged prompts of up to 2048 tokens, 14/2 heads of 64, 157 MB
 // in 31 us = 5.1 TB/s (one head a step 45 us); a step of 32 sequences, 28/4 heads of 128,
-// 2.3 us in a graph of launches. Into 4-bit pages the quantisation of k and v bounds it:
-// exact, through doubles for k (products of two floats) and a division per value, 16
-// ragged prompts of up to 2048 tokens, 28/4 heads of 128, 121 us (205 with one kind of CTA
-// and comparisons for codes).
+// 2.3 us in a graph of launches. Into 4-bit pages k and v are
+// quantised exactly, through doubles for k (products of two floats) and a division per
+// value: 16 ragged prompts of up to 2048 tokens, 28/4 heads of 128, 121 us (180 with one
+// kind of CTA and comparisons for codes; 110 without the doubles, 102 without any of it).
 template <typename T, typename KV, int V, int NP>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, const HeadSplit& hs, int walker, int walkers, int part,
                                             int parts) {
@@ -369,20 +369,24 @@ struct GatherArgs {
   int64_t count;
 };
 
+constexpr int kGatherRows = 2;  // of a thread, in flight
+
 // A thread owns elements [vi * V, vi * V + V) of a row and walks rows; grid = (row
-// walkers, sequences x heads, K and V). Bound by memory: the dense rows are written, and
-// read from 16-bit pages or from 4-bit ones a quarter of that; 16 ragged prompts of up to
-// 2048 tokens, 4 heads of 128 out of 4-bit pages in 25 us.
+// walkers, sequences x heads, K and V), no larger CTAs than the rows want. Bound by memory
+// (the dense rows are written, and read from 16-bit pages, or from 4-bit ones a quarter of
+// that) and by conversion: 16 ragged prompts of up to 2048 tokens, 4 heads of 128 out of
+// 4-bit pages 21.6 us (four rows in flight 23.3, half the elements a thread 26 to 30); one
+// row of 128 sequences, 8 heads, 2.9 us (4.7 with 256 threads a CTA).
 template <typename T, typename KV, int V>
 __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
   DLI_PDL_ENTRY();
   constexpr bool kFp4 = std::is_same<KV, Fp4>::value;
-  constexpr int U = 2;  // rows in flight
+  constexpr int U = kGatherRows;
   const int b = blockIdx.y / a.hkv, h = blockIdx.y - b * a.hkv;
   const void* pages = blockIdx.z ? a.v_pages : a.k_pages;
   const float scale = blockIdx.z ? a.v_scale : a.k_scale;
   const int d = a.head_dim, ipr = d / V, page_rows = 1 << a.seqs.page_shift;
-  const int per_cta = 256 / ipr;  // rows
+  const int per_cta = blockDim.x / ipr;  // rows
   const int vi = threadIdx.x % ipr, rl = threadIdx.x / ipr;
   if (rl >= per_cta) return;
   const int64_t rows_max = a.seqs.max_pages << a.seqs.page_shift;
@@ -395,24 +399,41 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
   T* out = static_cast<T*>(blockIdx.z ? a.v_out : a.k_out) + static_cast<int64_t>(blockIdx.y) * a.count * d + vi * V;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * per_cta;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per_cta + rl; r0 < a.count; r0 += U * stride) {
-    Row<T, V> x[U];
+    // all rows' pages, then all their bytes, then the stores
+    int page[U], pr[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int64_t p = first + r0 + k * stride;
+      const bool there = r0 + k * stride < a.count && p >= 0 && p < end;
+      pr[k] = static_cast<int>(p) & (page_rows - 1);
+      page[k] = there ? page_of(a.seqs, b, static_cast<int>(p)) : -1;
+    }
+    Row<T, V> x[U];
+    if constexpr (kFp4) {
+      uint2 w[U];
+      unsigned char sb[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k].e[j] = from_f32<T>(0.f);
-      const int page = r0 + k * stride < a.count && p >= 0 && p < end ? page_of(a.seqs, b, static_cast<int>(p)) : -1;
-      if (page < 0) continue;
-      const int64_t block = static_cast<int64_t>(page) * a.hkv + h;
-      const int pr = static_cast<int>(p) & (page_rows - 1);
-      if constexpr (kFp4) {
-        const uint8_t* base = static_cast<const uint8_t*>(pages) + block * fp4_block_bytes(page_rows, d);
-        const uint2 w = *reinterpret_cast<const uint2*>(base + pr * (d / 2) + vi * 8);
-        const float s = e4m3_value(base[page_rows * (d / 2) + pr * (d / 16) + vi]) * 16384.f;  // exact
+      for (int k = 0; k < U; ++k) {
+        w[k] = make_uint2(0u, 0u);
+        sb[k] = 0;
+        if (page[k] >= 0) {
+          const uint8_t* base = static_cast<const uint8_t*>(pages) + (static_cast<int64_t>(page[k]) * a.hkv + h) * fp4_block_bytes(page_rows, d);
+          w[k] = *reinterpret_cast<const uint2*>(base + pr[k] * (d / 2) + vi * 8);
+          sb[k] = base[page_rows * (d / 2) + pr[k] * (d / 16) + vi];
+        }
+      }
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[k].e[j] = from_f32<T>(e2m1_small(((j < 8 ? w.x : w.y) >> (4 * (j & 7))) & 15u) * s * scale);
-      } else {
-        x[k].load(static_cast<const T*>(pages) + (block * page_rows + pr) * d + vi * V);
+      for (int k = 0; k < U; ++k) {
+        const float s = e4m3_value(sb[k]) * 16384.f;  // exact
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[k].e[j] = from_f32<T>(e2m1_small(((j < 8 ? w[k].x : w[k].y) >> (4 * (j & 7))) & 15u) * s * scale);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[k].e[j] = from_f32<T>(0.f);
+        if (page[k] >= 0) x[k].load(static_cast<const T*>(pages) + ((static_cast<int64_t>(page[k]) * a.hkv + h) * page_rows + pr[k]) * d + vi * V);
       }
     }
 #pragma unroll
@@ -730,18 +751,18 @@ extern "C" dli_status dli_sm100_paged_gather(const void* k_pages, const void* v_
   if (head_dim > 256) return fail(DLI_ERR_UNSUPPORTED, "paged_gather: head_dim > 256");
   st = dispatch_float(dtype, what, [&](auto tag) {
     using T = decltype(tag);
-    auto grid = [&](int64_t elements) {  // of a thread
-      const int64_t per_cta = 256 / (head_dim / elements);
-      const int64_t walkers = std::min<int64_t>(ceil_div(count, per_cta),
+    auto launch = [&](auto kernel, int64_t elements) {  // of a thread
+      // no more threads than the rows want
+      const int64_t per_row = head_dim / elements, threads = std::max<int64_t>(per_row, std::min<int64_t>(256, count * per_row));
+      const int64_t per_cta = std::min<int64_t>(256, ceil_div(threads, 32) * 32) / per_row;
+      const int64_t walkers = std::min<int64_t>(ceil_div(count, kGatherRows * per_cta),
                                                 std::max<int64_t>(1, ceil_div(32ll * sm_count(), batch * kv_heads)));
-      return dim3(static_cast<unsigned>(walkers), static_cast<unsigned>(batch * kv_heads), 2u);
+      launch_pdl(kernel, dim3(static_cast<unsigned>(walkers), static_cast<unsigned>(batch * kv_heads), 2u),
+                 dim3(static_cast<unsigned>(std::min<int64_t>(256, ceil_div(threads, 32) * 32))), 0, as_stream(stream), a);
     };
-    if (kv_dtype == DLI_DTYPE_FP4)
-      launch_pdl(paged_gather_kernel<T, Fp4, 16>, grid(16), dim3(256), 0, as_stream(stream), a);
-    else if (al && head_dim % Vec16<T>::N == 0)
-      launch_pdl(paged_gather_kernel<T, T, Vec16<T>::N>, grid(Vec16<T>::N), dim3(256), 0, as_stream(stream), a);
-    else
-      launch_pdl(paged_gather_kernel<T, T, 1>, grid(1), dim3(256), 0, as_stream(stream), a);
+    if (kv_dtype == DLI_DTYPE_FP4) launch(paged_gather_kernel<T, Fp4, 16>, 16);
+    else if (al && head_dim % Vec16<T>::N == 0) launch(paged_gather_kernel<T, T, Vec16<T>::N>, Vec16<T>::N);
+    else launch(paged_gather_kernel<T, T, 1>, 1);
   });
   if (st != DLI_OK) return st;
   return check_launch(what);
