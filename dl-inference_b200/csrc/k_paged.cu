@@ -158,11 +158,11 @@ struct Row {
 // read once per token and pass), and for a decode step by the latency of one chain of
 // loads. A thread owns V elements of a token's head and takes NP heads a step, whose loads
 // are asked for together: 24 ragged prompts of up to 2048 tokens, 14/2 heads of 64, 157 MB
-// in 31 us = 5.1 TB/s (one head a step 45 us); a step of 32 sequences, 28/4 heads of 128,
+// in 29.5 us = 5.3 TB/s (three heads a step 31 us, one 45); a step of 32 sequences, 28/4 heads of 128,
 // 2.3 us in a graph of launches. Into 4-bit pages k and v are
 // quantised exactly, through doubles for k (products of two floats) and a division per
-// value: 16 ragged prompts of up to 2048 tokens, 28/4 heads of 128, 121 us (180 with one
-// kind of CTA and comparisons for codes; 110 without the doubles, 102 without any of it).
+// value: 16 ragged prompts of up to 2048 tokens, 28/4 heads of 128, 99 us (180 with one
+// kind of CTA and comparisons for codes).
 template <typename T, typename KV, int V, int NP>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, const HeadSplit& hs, int walker, int walkers, int part,
                                             int parts) {
@@ -304,15 +304,16 @@ __global__ void __launch_bounds__(256, NP == 1 ? 2 : 4) qkv_rotary_paged_kernel(
   append_rows<T, KV, V, NP>(a, a.all, blockIdx.x, gridDim.x, blockIdx.z, gridDim.z);
 }
 
-// Many tokens into 4-bit pages: every other CTA streams q, three heads a thread, while
-// its neighbours quantise k and v, whose arithmetic (ALU half busy) then hides under the
+// Many tokens into 4-bit pages: every other CTA streams q, four heads a thread, while its
+// neighbours quantise k and v, two rows a thread (16 prompts, q heads | rows of k and v:
+// 3 | 1 121 us, 3 | 2 113, 4 | 2 99, 3 | 4 120, 2 | 2 114), whose arithmetic (ALU half busy) then hides under the
 // streaming. grid = (2 x token walkers, sequences).
 template <typename T>
 __global__ void __launch_bounds__(256, 4) qkv_rotary_paged_fp4_kernel(const AppendArgs a) {
   DLI_PDL_ENTRY();
   const int walker = blockIdx.x >> 1, walkers = gridDim.x >> 1;
-  if (blockIdx.x & 1) append_rows<T, Fp4, 8, 1>(a, a.kv, walker, walkers, 0, 1);
-  else append_rows<T, T, 8, 3>(a, a.q, walker, walkers, 0, 1);
+  if (blockIdx.x & 1) append_rows<T, Fp4, 8, 2>(a, a.kv, walker, walkers, 0, 1);
+  else append_rows<T, T, 8, 4>(a, a.q, walker, walkers, 0, 1);
 }
 
 template <typename T, typename KV, int V>
@@ -348,12 +349,13 @@ void launch_append(AppendArgs a, cudaStream_t stream) {
                dim3(static_cast<unsigned>(a.seqs.max_new), batch, static_cast<unsigned>(a.all.passes)),
                dim3(threads(a.all)), 0, stream, a);
   } else if constexpr (kFp4) {
-    a.q = split(0, a.hq, 3);
-    a.kv = split(a.hq, heads, 1);
+    a.q = split(0, a.hq, 4);
+    a.kv = split(a.hq, heads, 2);
     launch_pdl(qkv_rotary_paged_fp4_kernel<T>, dim3(2u * std::max(walkers(a.q), walkers(a.kv)), batch),
                dim3(std::max(threads(a.q), threads(a.kv))), 0, stream, a);
   } else {
-    launch_pdl(qkv_rotary_paged_kernel<T, KV, V, 3>, dim3(walkers(a.all), batch), dim3(threads(a.all)), 0, stream, a);
+    a.all = split(0, heads, 5);
+    launch_pdl(qkv_rotary_paged_kernel<T, KV, V, 5>, dim3(walkers(a.all), batch), dim3(threads(a.all)), 0, stream, a);
   }
 }
 
