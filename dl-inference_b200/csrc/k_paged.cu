@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(256, NP == 1 ? 2 : 4) qkv_rotary_paged_kernel(
 
 // Many tokens into 4-bit pages: every other CTA streams q, four heads a thread, while its
 // neighbours quantise k and v, two rows a thread (16 prompts, q heads | rows of k and v:
-// 3 | 1 121 us, 3 | 2 113, 4 | 2 99, 3 | 4 120, 2 | 2 114), whose arithmetic (ALU half busy) then hides under the
-// streaming. grid = (2 x token walkers, sequences).
+// 3 | 1 121 us, 3 | 2 113, 4 | 2 99, 3 | 4 120, 2 | 2 114), whose arithmetic then hides
+// under the streaming. grid = (2 x token walkers, sequences).
 template <typename T>
 __global__ void __launch_bounds__(256, 4) qkv_rotary_paged_fp4_kernel(const AppendArgs a) {
   DLI_PDL_ENTRY();
@@ -655,7 +655,7 @@ PagedSeqs make_seqs(const int64_t* positions, const int64_t* starts, const int32
   s.num_pages = num_pages;
   s.max_pages = max_pages;
   s.batch = static_cast<int>(batch);
-  s.max_new = static_cast<int>(max_new);
+  s.max_new = static_cast<int>(std::min(max_new, tokens));  // no sequence has more rows than there are
   s.page_shift = page_shift_of(page_size);
   s.err = device_error_word();
   return s;
@@ -777,6 +777,7 @@ extern "C" size_t dli_sm100_attention_paged_workspace_size(int64_t tokens, int64
   if (tokens <= 0 || batch <= 0 || max_new <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0) return 0;
   if (page_shift_of(page_size) < 0 || max_pages <= 0 || max_pages > (1ll << 30) / page_size) return 0;
   if (!is_float_dtype(dtype) || (head_dim != 64 && head_dim != 128)) return 0;
+  max_new = std::min(max_new, tokens);
   const int64_t group = q_heads / kv_heads, max_keys = max_pages * page_size;
   if (few_rows(dtype, kv_dtype == DLI_DTYPE_FP4, group, max_new)) return paged_decode_workspace(batch, kv_heads, group, max_new, head_dim, max_keys, dtype);
   return paged_prefill_workspace(batch, kv_heads, group, max_new, head_dim, max_keys);
@@ -821,7 +822,7 @@ extern "C" dli_status dli_sm100_attention_paged(const void* q, const void* k_pag
   // within 2^-64 weigh all alike), and their reciprocals stay normal
   a.softcap = softcap > 0.f ? std::max(std::min(softcap, 0x1p64f), 0x1p-64f) : 0.f;
   a.v_scale = fp4 ? v_scale : 1.f;
-  if (few_rows(dtype, fp4, a.group, max_new)) {
+  if (few_rows(dtype, fp4, a.group, a.seqs.max_new)) {
     if (paged_decode_serves(a, dtype)) return run_paged_decode(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));
   } else if (paged_prefill_serves(a, dtype, kv_dtype)) {
     return run_paged_prefill(a, dtype, kv_dtype, workspace, workspace_bytes, as_stream(stream));

@@ -421,6 +421,15 @@ def test_a_bound_on_new_rows_that_is_too_large(name):
     C.check_device_error()
     c.check(out)
     assert (out[c.tokens:] == 5).all()
+    out.fill_(5.0)  # a bound beyond any buffer costs nothing
+    C.attention_paged(q, c.k, c.v, c.positions, c.table, starts=c.starts, max_new=2 ** 30, slopes=c.slopes, out=out, **c.options)
+    C.check_device_error()
+    c.check(out)
+    hkv = c.k.shape[1]
+    qkv = torch.zeros(c.tokens, (c.hq + 2 * hkv) * c.d, dtype=c.dtype, device="cuda")
+    one = torch.ones(int(c.lengths.max()), 1, device="cuda")
+    C.qkv_rotary_paged(qkv, one, one * 0, c.positions, c.table, c.k, c.v, c.hq, starts=c.starts, max_new=2 ** 30)
+    C.check_device_error()
     # no rows at all in a batch that has some behind it
     out.fill_(5.0)
     C.attention_paged(q, c.k, c.v, c.positions, c.table, starts=torch.zeros_like(c.starts), out=out)
