@@ -566,8 +566,13 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
           if constexpr (L::kFp4) {
             const bool copy = lane < boxes && page != none;
             uint8_t* block = dst + lane * block_bytes;
-            if (lane < boxes && page == none && first + lane <= last_page)  // a bad page
+            // a bad page, or one behind the window: zeros, ordered before the arrival below
+            // (for the consumers) and before a later copy into the entry (another proxy)
+            if (lane < boxes && page == none && first + lane <= last_page) {
               for (int i = 0; i < block_bytes; i += 16) *reinterpret_cast<uint4*>(block + i) = make_uint4(0u, 0u, 0u, 0u);
+              fence_proxy_async_smem();
+            }
+            __syncwarp();
             const int copies = __popc(__ballot_sync(0xffffffffu, copy));
             if (lane == 0) mbar_arrive_expect_tx(&full[e], static_cast<uint32_t>(copies * block_bytes));
             __syncwarp();
