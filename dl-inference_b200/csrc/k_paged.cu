@@ -629,7 +629,8 @@ dli_status check_pages(const std::string& what, int64_t batch, int64_t kv_heads,
   if (batch > 65535 || kv_heads > 65535) return fail(DLI_ERR_UNSUPPORTED, what + ": more than 65535 sequences or heads");
   if (num_pages > INT_MAX || max_pages > (1ll << 30) / page_size)
     return fail(DLI_ERR_UNSUPPORTED, what + ": more than 2^30 rows per sequence or 2^31 pages");
-  if (batch > 0 && (k_pages == nullptr || v_pages == nullptr || page_table == nullptr) && num_pages > 0 && max_pages > 0)
+  // the kernels look rows up in the table before they compare its entries with num_pages
+  if (batch > 0 && max_pages > 0 && (page_table == nullptr || (num_pages > 0 && (k_pages == nullptr || v_pages == nullptr))))
     return fail(DLI_ERR_INVALID_ARGUMENT, what + ": pages and page_table required");
   return DLI_OK;
 }
