@@ -293,14 +293,14 @@ __device__ __forceinline__ void qk_f32(float (&sc)[NT][4], const uint8_t* sk, in
     const float4 k0 = *reinterpret_cast<const float4*>(col + r0 * 128 + ((ch ^ (r0 & 7)) << 4));
     const float4 k1 = *reinterpret_cast<const float4*>(col + r1 * 128 + ((ch ^ (r1 & 7)) << 4));
     uint32_t hi[2][4], lo[2][4];
-    split_tf32(k0.x, hi[0][0], lo[0][0]);
-    split_tf32(k1.x, hi[0][1], lo[0][1]);
-    split_tf32(k0.y, hi[0][2], lo[0][2]);
-    split_tf32(k1.y, hi[0][3], lo[0][3]);
-    split_tf32(k0.z, hi[1][0], lo[1][0]);
-    split_tf32(k1.z, hi[1][1], lo[1][1]);
-    split_tf32(k0.w, hi[1][2], lo[1][2]);
-    split_tf32(k1.w, hi[1][3], lo[1][3]);
+    split_tf32<true>(k0.x, hi[0][0], lo[0][0]);
+    split_tf32<true>(k1.x, hi[0][1], lo[0][1]);
+    split_tf32<true>(k0.y, hi[0][2], lo[0][2]);
+    split_tf32<true>(k1.y, hi[0][3], lo[0][3]);
+    split_tf32<true>(k0.z, hi[1][0], lo[1][0]);
+    split_tf32<true>(k1.z, hi[1][1], lo[1][1]);
+    split_tf32<true>(k0.w, hi[1][2], lo[1][2]);
+    split_tf32<true>(k1.w, hi[1][3], lo[1][3]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float(&acc)[4] = part[nt][kk & 3];
@@ -348,14 +348,14 @@ __device__ __forceinline__ void pv_f32(float (&o)[NT][D / 16][4], const float (&
       const float4 va = *reinterpret_cast<const float4*>(col + ra * 128 + ((chunk ^ (ra & 7)) << 4));
       const float4 vb = *reinterpret_cast<const float4*>(col + rb * 128 + ((chunk ^ (rb & 7)) << 4));
       uint32_t hi[2][4], lo[2][4];
-      split_tf32(va.x, hi[0][0], lo[0][0]);
-      split_tf32(va.y, hi[0][1], lo[0][1]);
-      split_tf32(vb.x, hi[0][2], lo[0][2]);
-      split_tf32(vb.y, hi[0][3], lo[0][3]);
-      split_tf32(va.z, hi[1][0], lo[1][0]);
-      split_tf32(va.w, hi[1][1], lo[1][1]);
-      split_tf32(vb.z, hi[1][2], lo[1][2]);
-      split_tf32(vb.w, hi[1][3], lo[1][3]);
+      split_tf32<true>(va.x, hi[0][0], lo[0][0]);
+      split_tf32<true>(va.y, hi[0][1], lo[0][1]);
+      split_tf32<true>(vb.x, hi[0][2], lo[0][2]);
+      split_tf32<true>(vb.y, hi[0][3], lo[0][3]);
+      split_tf32<true>(va.z, hi[1][0], lo[1][0]);
+      split_tf32<true>(va.w, hi[1][1], lo[1][1]);
+      split_tf32<true>(vb.z, hi[1][2], lo[1][2]);
+      split_tf32<true>(vb.w, hi[1][3], lo[1][3]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         mma_1688_f32(part[nt][0], low[nt][0], hi[0], lo[0], pb[nt][2 * h], pb[nt][2 * h + 1]);

@@ -34,11 +34,22 @@ __device__ __forceinline__ void mma_1688_tf32(float (&d)[4], uint32_t a0, uint32
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// x = hi + lo to 2^-24: both rounded to nearest (ties away) at TF32's 11 significant
-// bits. lo is left for the MMA to cut off: half a unit is added to its magnitude.
+// x = hi + lo: hi rounded to nearest (ties away) at TF32's 11 significant bits, lo the
+// rest of at most 12, whose last the MMA cuts off (2^-23 of x at most). No bits of lo are
+// touched: it carries a NaN, and one of all ones (the GPU's own) plus a rounding unit
+// would be -0. An infinity, and a value that rounds up to one, becomes a NaN, as the row
+// of q or P would that has it; CACHED values keep hi at the largest TF32 number, and lo
+// is the rest, an infinity included (an infinite k may count for nothing, an infinite v
+// is an infinity): two more instructions of five.
+template <bool CACHED = false>
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
-  lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
+  if constexpr (CACHED) {
+    constexpr float kMost = 0x1.ffcp127f;
+    hi = ((__float_as_uint(fminf(fabsf(x), kMost)) + 0x1000u) & 0x7FFFE000u) | (__float_as_uint(x) & 0x80000000u);
+  } else {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  }
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 // A B to fp32's accuracy as three TF32 products, lo * lo (2^-24 of it) left out. The
 // MMA cuts its sums off instead of rounding them, so the caller keeps its chains

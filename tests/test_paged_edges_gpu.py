@@ -11,6 +11,8 @@ import test_paged_long_gpu as long
 
 pytestmark = pytest.mark.gpu
 
+FL = torch.float32
+
 
 @pytest.mark.parametrize("name", ["decode-fp4", "decode-fp4-many", "decode-f32-fp4"])
 @pytest.mark.parametrize("window", [0, 1000])
@@ -40,3 +42,82 @@ def test_four_bit_rings_over_bad_and_forgotten_pages(name, window):
         for _ in range(20):
             assert torch.equal(c.run(), want)
         C.check_device_error()
+
+
+def put_nan(c, pages, b, head, rows, dims, bits=None):
+    """NaN (of the given float32 bits) in some dims of rows of sequence b; over 4-bit pages in the whole rows."""
+    table = c.table[b].tolist()
+    page = pages.shape[2] // (c.d * 9 // 16) if pages.dtype == torch.uint8 else pages.shape[2]
+    for r in rows:
+        block, r0 = pages[table[r // page], head], r % page
+        if pages.dtype == torch.uint8:
+            at = page * c.d // 2 + r0 * (c.d // 16)
+            block[at:at + c.d // 16] = 0x7F
+        elif bits is None:
+            block[r0, dims] = float("nan")
+        else:
+            block.view(torch.int32)[r0, dims] = bits
+
+
+SHORT = (FL, False, 6, 2, 64, 16, [70, 4, 333], [1, 1, 1])
+
+
+@pytest.mark.parametrize("bits", [0x7FFFFFFF, 0xFFFFFFFF, 0x7F800001, 0x7FC00000], ids=hex)
+@pytest.mark.parametrize("name", ["short", "decode-f32", "rows-f32"])
+def test_float32_nan_of_every_pattern(name, bits):
+    """A NaN in q, k or v (the GPU's own is 0x7FFFFFFF) makes NaN of what it reaches, and of nothing else."""
+    c = long.Case(*SHORT) if name == "short" else long.case(name)
+    want = c.run()
+    group, new = c.hq // c.k.shape[1], c.new[0]
+    signed = bits - (1 << 32) if bits >> 31 else bits
+    q = c.q.clone()
+    q.view(torch.int32)[0, 1, 5] = signed
+    got = c.run(q=q)
+    assert torch.isnan(got[0, 1]).all()
+    got[0, 1] = want[0, 1]
+    assert torch.equal(got, want)
+    heads = slice(group, 2 * group)  # of KV head 1
+    k = c.k.clone()
+    put_nan(c, c.k, 0, 1, [3], slice(7, 8), signed)
+    got = c.run()
+    assert torch.isnan(got[:new, heads]).all()
+    got[:new, heads] = want[:new, heads]
+    assert torch.equal(got, want)
+    c.k = k
+    put_nan(c, c.v, 0, 1, [3], slice(7, 8), signed)
+    got = c.run()
+    C.check_device_error()
+    assert torch.isnan(got[:new, heads, 7]).all()
+    got[:new, heads, 7] = want[:new, heads, 7]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["short", "decode-f32", "rows-f32"])
+def test_float32_infinities_in_the_cache(name):
+    """A k of -infinity takes its key out of the rows with a positive q there; a v of infinity makes infinities, and
+    so does a finite v next to the largest float, as it is."""
+    c = long.Case(*SHORT) if name == "short" else long.case(name)
+    group, n, past = c.hq // c.k.shape[1], c.new[0], c.past[0]
+    heads = slice(group, 2 * group)
+    c.q[:, :, 7] = c.q[:, :, 7].abs() + 0.25
+    put_nan(c, c.k, 0, 1, [3, 40], slice(7, 8), 0xFF800000 - (1 << 32))
+    got = c.run()[:n, heads]
+    k, v = C.paged_gather(c.k, c.v, c.table, past + n, c.d, FL, lengths=c.lengths)
+    s = torch.einsum("nhd,ld->nhl", c.q[:n, heads].double(), k[0, 1].double()) * c.d ** -0.5
+    i = past + torch.arange(n, device="cuda")[:, None, None]
+    s = s.masked_fill(torch.arange(past + n, device="cuda") > i, float("-inf"))
+    want = torch.softmax(s, -1) @ v[0, 1].double()
+    assert (s[..., 3] == float("-inf")).all() and torch.isfinite(want).all()
+    torch.testing.assert_close(got.double(), want, rtol=0, atol=1e-5)
+    before = c.run()
+    put_nan(c, c.v, 0, 1, [5], slice(9, 10), 0x7F800000)
+    put_nan(c, c.v, 0, 1, [5], slice(11, 12), 0x7F7FFFFF)
+    out = c.run()
+    p = torch.softmax(s, -1)[..., 5]
+    assert (out[:n, heads, 9] == float("inf")).all()
+    big = out[:n, heads, 11].double()
+    torch.testing.assert_close(big, p * torch.finfo(FL).max, rtol=1e-4, atol=0)
+    out[:n, heads, 9] = before[:n, heads, 9]
+    out[:n, heads, 11] = before[:n, heads, 11]
+    assert torch.equal(out, before)
+    C.check_device_error()
