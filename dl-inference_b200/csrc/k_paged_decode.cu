@@ -1059,15 +1059,18 @@ constexpr int kWholeKeys = 512;
 constexpr int kMinKeys = 128;
 constexpr int kMaxCtasPerSm = 3;
 
+// max_keys: that a row may see; table_keys: the table's rows. The size of the workspace is
+// asked for without a window (max_keys = table_keys), so whatever calls for one goes by
+// the table, and a window can only take the need away.
 DecodePlan plan_paged_decode(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys,
-                             bool f32) {
+                             int64_t table_keys, bool f32) {
   DecodePlan p{};
   const int64_t rows = group * max_new;
   p.nt = rows <= 8 || f32 ? 1 : 2;  // two row tiles of split operands do not fit the registers
   p.tiles_max = static_cast<int>(ceil_div(rows, 8 * p.nt));
   p.units = batch * hkv * p.tiles_max;
   // the list's length has to fit an int (a longer one is never short of CTAs)
-  p.split = max_keys > kWholeKeys && p.units * (max_keys / 64 + 2) < INT_MAX;
+  p.split = max_keys > kWholeKeys && p.units * (table_keys / 64 + 2) < INT_MAX;
   p.grid = p.split ? static_cast<int64_t>(sm_count()) * kMaxCtasPerSm : p.units;
   if (p.split) {
     const int64_t r = 8 * p.nt;
@@ -1117,9 +1120,11 @@ dli_status launch_paged_decode_nd(const PagedAttnArgs& a, const DecodePlan& plan
   return a.head_dim == 64 ? launch_paged_decode<T, KV, 64, 1>(a, plan, ws, stream) : launch_paged_decode<T, KV, 128, 1>(a, plan, ws, stream);
 }
 
-int64_t max_keys_of(const PagedAttnArgs& a) {
-  const int64_t cap = a.seqs.max_pages << a.seqs.page_shift;
-  return std::min<int64_t>(cap, static_cast<int64_t>(a.window) + a.seqs.max_new);
+DecodePlan plan_of(const PagedAttnArgs& a, dli_dtype dtype) {
+  const int64_t table_keys = a.seqs.max_pages << a.seqs.page_shift;
+  return plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim,
+                           std::min<int64_t>(table_keys, static_cast<int64_t>(a.window) + a.seqs.max_new), table_keys,
+                           dtype == DLI_DTYPE_F32);
 }
 
 }  // namespace
@@ -1155,18 +1160,17 @@ bool paged_decode_serves(const PagedAttnArgs& a, dli_dtype dtype) {
   if (a.seqs.num_pages < 1) return false;
   for (const void* p : {a.q, a.k_pages, a.v_pages, static_cast<const void*>(a.out)})
     if (!aligned(p, 16)) return false;
-  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a), dtype == DLI_DTYPE_F32);
-  return plan.units <= INT_MAX;
+  return plan_of(a, dtype).units <= INT_MAX;
 }
 
 size_t paged_decode_workspace(int64_t batch, int64_t hkv, int64_t group, int64_t max_new, int64_t head_dim, int64_t max_keys,
                               dli_dtype dtype) {
-  return plan_paged_decode(batch, hkv, group, max_new, head_dim, max_keys, dtype == DLI_DTYPE_F32).workspace;
+  return plan_paged_decode(batch, hkv, group, max_new, head_dim, max_keys, max_keys, dtype == DLI_DTYPE_F32).workspace;
 }
 
 dli_status run_paged_decode(const PagedAttnArgs& a, dli_dtype dtype, dli_dtype kv_dtype, void* workspace,
                             size_t workspace_bytes, cudaStream_t stream) {
-  const DecodePlan plan = plan_paged_decode(a.seqs.batch, a.hkv, a.group, a.seqs.max_new, a.head_dim, max_keys_of(a), dtype == DLI_DTYPE_F32);
+  const DecodePlan plan = plan_of(a, dtype);
   if (plan.workspace > 0 && (workspace == nullptr || workspace_bytes < plan.workspace || !aligned(workspace, 16)))
     return fail(DLI_ERR_WORKSPACE, "attention_paged: a 16-byte aligned workspace of " + std::to_string(plan.workspace) + " bytes is needed");
   const bool fp4 = kv_dtype == DLI_DTYPE_FP4;

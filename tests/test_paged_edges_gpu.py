@@ -121,3 +121,24 @@ def test_float32_infinities_in_the_cache(name):
     out[:n, heads, 11] = before[:n, heads, 11]
     assert torch.equal(out, before)
     C.check_device_error()
+
+
+def test_a_window_over_a_table_that_is_too_wide_to_share_out():
+    """Units times the table's blocks pass an int, units times the window's do not: the workspace is of the size that
+    was asked for, and the call is served."""
+    hq, hkv, d, page, batch = 8, 8, 64, 128, 32
+    rows, width = 8192, 4096
+    new = [rows // batch] * batch
+    g = torch.Generator("cuda").manual_seed(2)
+    q = torch.randn(rows, hq, d, device="cuda", generator=g)
+    k, v = C.paged_kv_pages(2 * batch, hkv, page, d, FL)
+    k.normal_(generator=g), v.normal_(generator=g)
+    table = torch.full((batch, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :2] = torch.randperm(2 * batch, device="cuda", generator=g).view(batch, 2)
+    starts = torch.arange(batch + 1, device="cuda") * new[0]
+    pos = torch.zeros(batch, dtype=torch.int64, device="cuda")
+    out = C.attention_paged(q, k, v, pos, table, starts=starts, window=700)  # wider than any sequence
+    want = C.attention_paged(q, k, v, pos, table[:, :2].contiguous(), starts=starts)
+    C.check_device_error()
+    assert torch.equal(out, want)
+    assert torch.equal(C.attention_paged(q, k, v, pos, table, starts=starts), want)
