@@ -328,7 +328,8 @@ void launch_append(AppendArgs a, cudaStream_t stream) {
     const int heads = head1 - head0;
     s.head0 = head0;
     s.head1 = head1;
-    s.passes = static_cast<int>(std::max<int64_t>(ceil_div(static_cast<int64_t>(heads) * ipr, 256), std::min(at_least, heads)));
+    // a CTA of 256 threads holds whole heads
+    s.passes = static_cast<int>(std::max<int64_t>(ceil_div(heads, 256 / ipr), std::min(at_least, heads)));
     s.per_pass = static_cast<int>(ceil_div(heads, s.passes));
     s.passes = static_cast<int>(ceil_div(heads, s.per_pass));
     s.tokens = std::max(1, 256 / (s.per_pass * ipr));

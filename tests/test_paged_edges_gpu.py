@@ -7,11 +7,12 @@ import pytest
 import torch
 
 import dli_sm100 as C
+import test_paged_gpu as plain
 import test_paged_long_gpu as long
 
 pytestmark = pytest.mark.gpu
 
-FL = torch.float32
+BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
 
 
 @pytest.mark.parametrize("name", ["decode-fp4", "decode-fp4-many", "decode-f32-fp4"])
@@ -142,3 +143,40 @@ def test_a_window_over_a_table_that_is_too_wide_to_share_out():
     C.check_device_error()
     assert torch.equal(out, want)
     assert torch.equal(C.attention_paged(q, k, v, pos, table, starts=starts), want)
+
+
+@pytest.mark.parametrize("dtype,fp4,hq,hkv,d,past,new", [
+    (BF, False, 48, 8, 96, [0, 5], [1, 1]),
+    (BF, False, 16, 8, 192, [31, 3], [1, 1]),
+    (FL, False, 24, 4, 96, [17], [1]),
+    (FL, False, 32, 32, 96, [3, 0], [1, 2]),
+    (FL, False, 32, 32, 96, [3, 0], [190, 30]),  # many tokens: several heads of a thread in flight
+    (BF, True, 48, 8, 96, [0, 40], [1, 1]),
+    (HF, True, 83, 1, 80, [9], [1]),
+    (BF, True, 80, 21, 80, [0, 9], [150, 60]),
+    (HF, False, 83, 1, 80, [0], [450]),
+    (BF, False, 5, 1, 172, [2], [3]),  # 43 pairs of 4 bytes a row: not by 16-byte vectors
+])
+def test_append_of_heads_that_fill_no_cta_evenly(dtype, fp4, hq, hkv, d, past, new):
+    plain.test_append(dtype, fp4, hq, hkv, d, 16, past, new, d // 2)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF, 48, 8, 96), (HF, 16, 8, 80), (FL, 7, 2, 172)])
+def test_append_of_views_off_their_alignment(dtype, hq, hkv, d):
+    """The same bits as from 16-byte aligned tensors."""
+    page, rows = 16, 7
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn(rows, (hq + 2 * hkv) * d, generator=g).to(dtype).cuda()
+    angle = (torch.rand(40, d // 2, generator=g) * 6).cuda()
+    table = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device="cuda")
+    starts, pos = torch.tensor([0, 3, 7], device="cuda"), torch.tensor([14, 5], device="cuda")
+    results = []
+    for shift in (0, 1):
+        flat = torch.empty(qkv.numel() + shift, dtype=dtype, device="cuda")[shift:]
+        flat.copy_(qkv.view(-1))
+        k, v = C.paged_kv_pages(4, hkv, page, d, dtype)
+        q = C.qkv_rotary_paged(flat.view_as(qkv), angle.cos(), angle.sin(), pos, table, k, v, hq, starts=starts, max_new=4)
+        results.append((q, k, v))
+    C.check_device_error()
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and a.abs().sum() > 0
