@@ -905,7 +905,8 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
           sum.z += v.z;
           sum.w += v.w;
           const float mw = wm[w * R + r];
-          if (mw != -INFINITY) den += wl[w * R + r] * exp2_approx(mw - top);
+          // without a score above -inf the sum is 0, or NaN
+          den += mw == -INFINITY ? wl[w * R + r] : wl[w * R + r] * exp2_approx(mw - top);
         }
         const int dim = half * DH + x;
         if (seg.whole) {
@@ -983,7 +984,8 @@ __global__ void __launch_bounds__(256) attn_paged_combine_kernel(const DecodeArg
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (ml[k].x == -INFINITY) continue;  // a part in which the row sees no key
+        // a part in which the row sees no key (the sum of one whose scores are all NaN is NaN)
+        if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;
         const float m = fmaxf(top, ml[k].x);
         const float f = exp2_approx(top - m), f2 = exp2_approx(ml[k].x - m);  // top = -inf: 0
         top = m;

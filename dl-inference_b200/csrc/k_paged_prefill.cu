@@ -893,7 +893,8 @@ __global__ void __launch_bounds__(256) attn_paged_prefill_combine_kernel(const P
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (ml[k].x == -INFINITY) continue;  // a part in which the row sees no key
+        // a part in which the row sees no key (the sum of one whose scores are all NaN is NaN)
+        if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;
         const float m = fmaxf(top, ml[k].x);
         const float f = exp2_approx(top - m), f2 = exp2_approx(ml[k].x - m);  // top = -inf: 0
         top = m;

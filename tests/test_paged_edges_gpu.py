@@ -180,3 +180,17 @@ def test_append_of_views_off_their_alignment(dtype, hq, hkv, d):
     C.check_device_error()
     for a, b in zip(*results):
         assert torch.equal(a, b) and a.abs().sum() > 0
+
+
+@pytest.mark.parametrize("dtype,fp4,d,new", [(BF, False, 128, 1), (HF, False, 64, 2), (BF, True, 128, 1), (FL, False, 128, 1),
+                                             (FL, True, 64, 1), (BF, False, 128, 60), (HF, True, 64, 60)])
+def test_nan_that_fills_whole_parts_of_the_keys(dtype, fp4, d, new):
+    """Keys 512 to 1535 of 2048, all of some shares and parts of them, score NaN in KV head 0: its rows are NaN, the
+    other head's keep their bits."""
+    c = long.Case(dtype, fp4, 16, 2, d, 64, [2048 - new], [new])
+    want = c.run()
+    put_nan(c, c.k, 0, 0, range(512, 1536), slice(0, d))
+    got = c.run()
+    C.check_device_error()
+    assert torch.isnan(got[:, :8]).all()
+    assert torch.equal(got[:, 8:], want[:, 8:])
