@@ -39,6 +39,7 @@
 // with 12 consumer warps per SM; eight per CTA spilled). float32: 32 x up to 1501 keys,
 // 16/4 heads: 39 us = 3.7 TB/s.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <map>
 #include <mutex>
@@ -707,8 +708,10 @@ __global__ void __launch_bounds__(DecodeLayout<T, KV, D, NT>::kThreads, DecodeLa
     float m[NT][2], l[NT][2], mul[NT][2];  // mul: what turns a masked score into log2 units
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      mul[nt][0] = a.softcap > 0.f || a.slopes ? 1.f : rscale[nt][0];
-      mul[nt][1] = a.softcap > 0.f || a.slopes ? 1.f : rscale[nt][1];
+      // a scale that underflows (of a q of zeros over 4-bit pages, say) must not make NaN of
+      // a masked score's -inf: no score is above 2^-100 with either
+      mul[nt][0] = a.softcap > 0.f || a.slopes ? 1.f : fmaxf(rscale[nt][0], FLT_MIN);
+      mul[nt][1] = a.softcap > 0.f || a.slopes ? 1.f : fmaxf(rscale[nt][1], FLT_MIN);
 #pragma unroll
       for (int i = 0; i < KK; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
       m[nt][0] = m[nt][1] = -INFINITY;

@@ -43,6 +43,7 @@
 // heads of 64: 39 us (issue 40%, MUFU 35%, tensor 34% busy). 4-bit pages, 4 chunks of up
 // to 301 tokens over 3001 keys, 28/4 heads: 83 us, over 16-bit pages 65.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -669,7 +670,9 @@ __global__ void __launch_bounds__(Roles<std::is_same<KV, Fp4>::value>::kThreads,
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
       }
-      const float mul = cap || bias ? 1.f : in_scale;  // what the scores still want when the maximum is taken
+      // what the scores still want when the maximum is taken; one that underflows (of a q of
+      // zeros over 4-bit pages, say) must not make NaN of a masked score's -inf
+      const float mul = cap || bias ? 1.f : fmaxf(in_scale, FLT_MIN);
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < x.nblocks; ++j) {
         const int g = g0 + j, sb = g & 1;

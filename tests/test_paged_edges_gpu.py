@@ -194,3 +194,24 @@ def test_nan_that_fills_whole_parts_of_the_keys(dtype, fp4, d, new):
     C.check_device_error()
     assert torch.isnan(got[:, :8]).all()
     assert torch.equal(got[:, 8:], want[:, 8:])
+
+
+@pytest.mark.parametrize("name", ["decode-fp4", "decode-f32-fp4", "parts-fp4", "tiles-fp4"])
+@pytest.mark.parametrize("scales", [dict(k_scale=1e-12), dict(k_scale=1e-30, scale=1e-25), dict(scale=1e-45)], ids=str)
+def test_scales_whose_product_underflows(name, scales):
+    """Scores that underflow weigh all keys alike (a row of q of zeros has nothing else), whatever masks some of them."""
+    c = long.case(name, amplitude=0.0, window=300, softcap=0.0)
+    want = c.run()
+    c.check(want)
+    c.options.update(scales)
+    assert torch.equal(c.run(), want)
+    C.check_device_error()
+
+
+@pytest.mark.parametrize("name", ["decode", "decode-f32", "parts", "tiles-bf16"])
+def test_the_smallest_scale(name):
+    c = long.case(name, amplitude=0.0)
+    want = c.run()
+    c.options.update(scale=1e-45)
+    assert torch.equal(c.run(), want)
+    C.check_device_error()
