@@ -533,8 +533,12 @@ def qkv_rotary_paged(qkv, cos, sin, positions, page_table, k_pages, v_pages, q_h
 
 
 @functools.lru_cache(maxsize=4096)
-def _attention_paged_workspace(*sizes):
-    return lib().dli_sm100_attention_paged_workspace_size(*sizes)
+def _attention_paged_workspace(dev, *sizes):
+    """Bytes for a call on device `dev` (they go by its SMs)."""
+    if torch._C._cuda_getDevice() == dev:
+        return lib().dli_sm100_attention_paged_workspace_size(*sizes)
+    with torch.cuda.device(dev):
+        return lib().dli_sm100_attention_paged_workspace_size(*sizes)
 
 
 def attention_paged(q, k_pages, v_pages, positions, page_table, starts=None, max_new=None, scale=0.0, softcap=0.0,
@@ -557,7 +561,7 @@ def attention_paged(q, k_pages, v_pages, positions, page_table, starts=None, max
         raise ValueError("attention_paged: out must be like q")
     dev = _device(what, q, k_pages, v_pages, positions, page_table, starts, slopes, out)
     dt = _dt(q)
-    ws_bytes = _attention_paged_workspace(tokens, b, max_new, hq, hkv, d, page_size, max_pages, dt, kv)
+    ws_bytes = _attention_paged_workspace(dev, tokens, b, max_new, hq, hkv, d, page_size, max_pages, dt, kv)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     _launch(what, dev, lib().dli_sm100_attention_paged, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
             positions.data_ptr(), _at(starts), page_table.data_ptr(), _at(slopes), out.data_ptr(), tokens, b, max_new,

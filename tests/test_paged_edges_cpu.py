@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 import dli_sm100 as C
 import test_paged_cpu as calls
@@ -16,3 +17,56 @@ def test_a_table_is_needed_for_a_pool_of_no_pages_too(fp4):
                      (L.dli_sm100_paged_gather, calls.gather_args)):
         assert fn(*args(table=None, pages=0, **kv)) == calls.INVALID, C.last_error()
         assert "page_table" in C.last_error()
+
+
+class _OnDevice:
+    """A tensor that says it lies on a GPU."""
+
+    def __init__(self, t, device):
+        self.t, self.index = t, device
+
+    def get_device(self):
+        return self.index
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+def test_the_workspace_is_of_the_tensors_device(monkeypatch):
+    """Its size goes by the device's SMs: asked for with that device current, and not kept for another one."""
+    current, sms = [0], {0: 148, 1: 200}
+    asked, given = [], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.held, current[0] = current[0], self.index
+
+        def __exit__(self, *a):
+            current[0] = self.held
+
+    class Lib:
+        def dli_sm100_attention_paged_workspace_size(self, *sizes):
+            asked.append(current[0])
+            return sms[current[0]] * 16
+
+        def dli_sm100_attention_paged(self, *args):
+            given.append((current[0], args[-2]))
+            return C.DLI_OK
+
+    monkeypatch.setattr(C, "lib", Lib)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    C._attention_paged_workspace.cache_clear()
+    k, v = (torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16) for _ in (0, 1))
+    q, table, pos = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int64)
+    try:
+        for device in (0, 1, 1, 0):
+            C.attention_paged(*(_OnDevice(t, device) for t in (q, k, v, pos, table)), out=_OnDevice(q.clone(), device))
+    finally:
+        C._attention_paged_workspace.cache_clear()
+    assert given == [(0, 148 * 16), (1, 200 * 16), (1, 200 * 16), (0, 148 * 16)]
+    assert asked == [0, 1] and current == [0]
