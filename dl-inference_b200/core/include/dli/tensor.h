@@ -6,7 +6,7 @@
 // CUDA pointer; `deviceData()` returns the raw device pointer and throws
 // std::logic_error for host tensors. DType keeps the reference's Float32 = 0 and
 // Int64 = 1 and appends BFloat16, Float16, Int32 and UInt8 (bytes of 4-bit cache
-// pages).
+// pages, made by the runtime only).
 #pragma once
 
 #include <ATen/ATen.h>
@@ -36,7 +36,7 @@ class Tensor {
  public:
   Tensor() = default;
   Tensor(DType dtype, std::vector<std::int64_t> shape);  // zero-filled host tensor
-  explicit Tensor(at::Tensor tensor);                       // made contiguous
+  explicit Tensor(at::Tensor tensor);                       // made contiguous; not of bytes
 
   static Tensor zeros(DType dtype, std::vector<std::int64_t> shape);
   static Tensor cuda(DType dtype, std::vector<std::int64_t> shape, int device_id = 0);

@@ -137,9 +137,10 @@ KVCacheEntry& KVCache::reservePaged(const std::string& name, std::int64_t num_pa
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     throw std::runtime_error("KV cache entry " + name + " has to exist before a capture: run the graph once first");
   KVCacheEntry e;
-  const auto options = at::TensorOptions().dtype(torchDType(held)).device(at::kCUDA, device_id);
-  e.key = Tensor(at::zeros(shape, options));
-  e.value = Tensor(at::zeros(shape, options));
+  e.key = Tensor::cuda(held, shape, device_id);
+  e.value = Tensor::cuda(held, shape, device_id);
+  e.key.torchTensor().zero_();
+  e.value.torchTensor().zero_();
   e.page_size = page_size;
   entries_[name] = std::move(e);
   return entries_[name];

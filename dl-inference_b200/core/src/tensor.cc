@@ -57,7 +57,6 @@ DType dtypeFromString(const std::string& dtype) {
   if (dtype == "bfloat16") return DType::BFloat16;
   if (dtype == "float16") return DType::Float16;
   if (dtype == "int32") return DType::Int32;
-  if (dtype == "uint8") return DType::UInt8;
   throw std::invalid_argument("unknown dtype: " + dtype);
 }
 
@@ -118,7 +117,10 @@ Tensor::Tensor(std::shared_ptr<Impl> impl) : impl_(std::move(impl)) {
   if (shape_.empty()) shape_.push_back(1);
 }
 
-Tensor::Tensor(at::Tensor tensor) : Tensor(std::make_shared<Impl>(tensor.contiguous())) {}
+Tensor::Tensor(at::Tensor tensor) : Tensor(std::make_shared<Impl>(tensor.contiguous())) {
+  // bytes are made inside the runtime only (pages of a 4-bit cache)
+  if (dtype_ == DType::UInt8) throw std::invalid_argument("unsupported torch tensor dtype");
+}
 
 Tensor::Tensor(DType dtype, std::vector<std::int64_t> shape) {
   if (shape.empty()) shape.push_back(1);

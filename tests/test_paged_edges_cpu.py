@@ -1,9 +1,12 @@
 """Paged KV cache, without a GPU: calls whose refusal, size or dtype is decided on the host alone."""
 from __future__ import annotations
 
+import json
+
 import pytest
 import torch
 
+import dli
 import dli_sm100 as C
 import test_paged_cpu as calls
 
@@ -70,3 +73,19 @@ def test_the_workspace_is_of_the_tensors_device(monkeypatch):
         C._attention_paged_workspace.cache_clear()
     assert given == [(0, 148 * 16), (1, 200 * 16), (1, 200 * 16), (0, 148 * 16)]
     assert asked == [0, 1] and current == [0]
+
+
+def test_bytes_do_not_enter_the_engine(tmp_path):
+    """uint8 is the type of a 4-bit pool's pages inside the engine: no input, constant, weight or operand has it."""
+    e = dli.Engine()
+    e.load_library(dli.PLUGIN_PATH)
+    g = dli.Graph.from_json(json.dumps({"format": "dli.graph.v1", "inputs": ["x"], "outputs": ["y"], "nodes": [
+        {"name": "n", "op": "reshape", "inputs": ["x"], "outputs": ["y"], "attrs": {"shape": [4]}}]}))
+    for call in (lambda t: e.run(g, {"x": t}), lambda t: e.set_constants({"x": t})):
+        with pytest.raises(ValueError, match="unsupported torch tensor dtype"):
+            call(torch.zeros(2, 2, dtype=torch.uint8))
+    (tmp_path / "w.bin").write_bytes(bytes(4))
+    (tmp_path / "w.json").write_text(json.dumps({"format": "dli.weights.v1", "data": "w.bin", "tensors": {
+        "a": {"dtype": "uint8", "shape": [4], "offset": 0, "nbytes": 4}}}))
+    with pytest.raises(ValueError, match="unknown dtype"):
+        dli.load_weights(str(tmp_path / "w.json"))
