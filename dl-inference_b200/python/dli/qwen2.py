@@ -14,6 +14,7 @@ stays at its address, so captured decode steps follow its contents.
 """
 from __future__ import annotations
 
+import contextlib
 import json
 from typing import Any
 
@@ -161,48 +162,48 @@ class Qwen2Runner:
         not disturbed. The markers make the step slower than the decode graph."""
         ids = torch.zeros(batch, 1, dtype=torch.int64, device=self.device)
         pos = torch.full((batch,), self.capacity - 1, dtype=torch.int64, device=self.device)
-        held = self._spare_page(batch)
-        stream = torch.cuda.Stream(self.device)
-        stream.wait_stream(torch.cuda.current_stream(self.device))
-        with torch.cuda.stream(stream):
-            self._step(ids, pos)
-        torch.cuda.current_stream(self.device).wait_stream(stream)
-        profile.reserve(len(self.graph.node_ops()))
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            self._step(ids, pos, profile=profile)
-        g.replay()
-        self._restore_table(held)
+        with self._on_spare_page(batch):
+            self._warm_up(ids, pos, 1)
+            profile.reserve(len(self.graph.node_ops()))
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                self._step(ids, pos, profile=profile)
+            g.replay()
         torch.cuda.synchronize(self.device)
         del g
 
-    def _spare_page(self, batch: int) -> torch.Tensor | None:
+    @contextlib.contextmanager
+    def _on_spare_page(self, batch: int):
         """Points a paged cache's table at the page outside the pool, for steps whose
-        rows nobody reads; returns what it held. All sequences of such a step write
-        the same row of that page with the same values."""
+        rows nobody reads, and back when they are done or have failed. All sequences of
+        such a step write the same row of that page with the same values."""
         if self.pool is None:
-            return None
+            yield
+            return
         held = self.page_table(batch).clone()
         self.page_table(batch).fill_(self.pool.num_pages)
-        return held
+        try:
+            yield
+        finally:
+            self.page_table(batch).copy_(held)
 
-    def _restore_table(self, held: torch.Tensor | None) -> None:
-        if held is not None:
-            self.page_table(held.shape[0]).copy_(held)
+    def _warm_up(self, ids: torch.Tensor, pos: torch.Tensor, steps: int) -> None:
+        stream = torch.cuda.Stream(self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(steps):
+                    self._step(ids, pos)
+        finally:
+            torch.cuda.current_stream(self.device).wait_stream(stream)
 
     def _capture(self, batch: int):
         # Warm-up and capture write one cache row per sequence; the last row is only
         # read after a later step has rewritten it, so live sequences are not disturbed.
         ids = torch.zeros(batch, 1, dtype=torch.int64, device=self.device)
         pos = torch.full((batch,), self.capacity - 1, dtype=torch.int64, device=self.device)
-        held = self._spare_page(batch)
-        stream = torch.cuda.Stream(self.device)
-        stream.wait_stream(torch.cuda.current_stream(self.device))
-        with torch.cuda.stream(stream):
-            for _ in range(2):  # warm the caching allocator and per-kernel attributes
-                self._step(ids, pos)
-        torch.cuda.current_stream(self.device).wait_stream(stream)
-        self._restore_table(held)
+        with self._on_spare_page(batch):
+            self._warm_up(ids, pos, 2)  # the caching allocator and per-kernel attributes
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             logits, next_ids = self._step(ids, pos)

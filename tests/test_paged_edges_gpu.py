@@ -215,3 +215,26 @@ def test_the_smallest_scale(name):
     c.options.update(scale=1e-45)
     assert torch.equal(c.run(), want)
     C.check_device_error()
+
+
+def test_a_warm_up_that_fails_leaves_the_open_sequences_their_pages():
+    import test_paged_model_gpu as model
+
+    shape = model._small()
+    r = model._runner(shape, page_size=16, num_pages=8)
+    r.open([40, 20])
+    held = r.page_table(2).clone()
+    step = r._step
+
+    def fail(*a, **k):
+        raise RuntimeError("out of memory")
+
+    r._step = fail
+    for call in (r.decode_graph, lambda n: r.profile_decode_step(n, None)):
+        with pytest.raises(RuntimeError, match="out of memory"):
+            call(2)
+        assert torch.equal(r.page_table(2), held)
+    r._step = step
+    r.decode_graph(2)
+    assert torch.equal(r.page_table(2), held)
+    r.release_graphs()
