@@ -238,3 +238,39 @@ def test_a_warm_up_that_fails_leaves_the_open_sequences_their_pages():
     r.decode_graph(2)
     assert torch.equal(r.page_table(2), held)
     r.release_graphs()
+
+
+@pytest.mark.parametrize("name", ["decode-many", "decode-fp4-many", "decode-f32", "parts"])
+def test_a_captured_call_follows_pages_that_move(name):
+    """Positions grow and pages move (their old places turn to NaN) between replays: the eager call's bits before the
+    move."""
+    c = long.case(name)
+    positions = c.positions.clone()
+    eager = []
+    cuts = (200, 64, 63, 1, 0)
+    for cut in cuts:
+        c.positions.copy_((positions - cut).clamp_min(0))
+        eager.append(c.run())
+    out = torch.empty_like(c.q)
+    c.run(out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.run(out=out)
+    held = set(c.table.flatten().tolist())
+    spare = [p for p in range(c.k.shape[0]) if p not in held]
+    for turn, cut in enumerate(cuts):
+        for i in range(len(spare)):
+            b, p = i % len(c.past), (turn + i) % 3 if c.past[i % len(c.past)] > 48 * 3 else 0
+            old = int(c.table[b, p])
+            if old < 0:
+                continue
+            for t in (c.k, c.v):
+                t[spare[i]] = t[old]
+                t[old] = 0xFF if t.dtype == torch.uint8 else float("nan")
+            c.table[b, p] = spare[i]
+            spare[i] = old
+        c.positions.copy_((positions - cut).clamp_min(0))
+        g.replay()
+        assert torch.equal(out, eager[turn])
+    C.check_device_error()
