@@ -274,3 +274,25 @@ def test_a_captured_call_follows_pages_that_move(name):
         g.replay()
         assert torch.equal(out, eager[turn])
     C.check_device_error()
+
+
+@pytest.mark.parametrize("fp4", [False, True], ids=["rows16", "rows4"])
+def test_a_batch_of_almost_only_idle_sequences(fp4):
+    """As many items as the grid may have, nearly all of them empty: none of the kernel's warps gives up waiting."""
+    batch, hq, rows, d = 65535, 128, 16384, 64  # a tile is one token
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = C.paged_kv_pages(4, 1, 16, d, "fp4" if fp4 else BF)
+    one = torch.ones(64, d // 2, device="cuda")
+    table = torch.zeros(batch, 2, dtype=torch.int32, device="cuda")
+    table[0], table[-1] = torch.tensor([1, 2]), torch.tensor([3, 0])
+    qkv = torch.randn(40, (hq + 2) * d, device="cuda", generator=g).to(BF)
+    starts = torch.full((batch + 1,), 20, dtype=torch.int64, device="cuda")
+    starts[0], starts[-1] = 0, 40
+    pos = torch.zeros(batch, dtype=torch.int64, device="cuda")
+    q = torch.zeros(rows, hq, d, dtype=BF, device="cuda")
+    q[:40] = C.qkv_rotary_paged(qkv, one, one * 0, pos, table, k, v, hq, starts=starts)
+    two = torch.tensor([0, batch - 1], device="cuda")
+    want = C.attention_paged(q[:40], k, v, pos[:2], table[two].contiguous(), max_new=20)
+    got = C.attention_paged(q, k, v, pos, table, starts=starts)
+    C.check_device_error()
+    assert torch.equal(got[:40], want)
