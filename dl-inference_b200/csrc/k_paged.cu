@@ -106,10 +106,6 @@ struct AppendArgs {
   int vec_tables;  // cos/sin rows can be read by 16 bytes
 };
 
-// A thread owns elements [vi * V, vi * V + V) of a head row and NP heads of a token,
-// hl, hl + heads_per_pass, ..., which it reads at once: a token's cos/sin values and
-// page are read once for all of them. A CTA holds as many tokens as it has room for.
-// Bound by memory: it reads qkv once and writes q, k and v once.
 // V elements of T as they lie in memory: 16-byte vectors where they fill any.
 template <typename T, int V>
 struct Row {
@@ -156,13 +152,17 @@ struct Row {
 // The append: out (x, y) = (x c - y s, x s + y c) for the pairs of q and k, v as it is.
 // Bound by memory (every byte of q|k|v is read once and written once, the rotary row is
 // read once per token and pass), and for a decode step by the latency of one chain of
-// loads. A thread owns V elements of a token's head and takes NP heads a step, whose loads
-// are asked for together: 24 ragged prompts of up to 2048 tokens, 14/2 heads of 64, 157 MB
+// loads. A thread owns elements [vi * V, vi * V + V) of a token's head and takes NP heads a
+// step, hl, hl + per_pass, ..., whose loads are asked for together; a CTA holds as many
+// tokens as it has room for: 24 ragged prompts of up to 2048 tokens, 14/2 heads of 64, 157 MB
 // in 29.5 us = 5.3 TB/s (three heads a step 31 us, one 45); a step of 32 sequences, 28/4 heads of 128,
-// 2.3 us in a graph of launches. Into 4-bit pages k and v are
-// quantised exactly, through doubles for k (products of two floats) and a division per
-// value: 16 ragged prompts of up to 2048 tokens, 28/4 heads of 128, 99 us (180 with one
-// kind of CTA and comparisons for codes).
+// 2.3 us in a graph of launches (a CTA for every sequence and token up to max_new: 128
+// sequences of one token 2.7 us, with a max_new of 128 57). Into 4-bit pages k and v are
+// quantised from 64 bits, k through doubles (exact products of two floats, their sum
+// rounded once) and a division per value: 16 ragged prompts of up to 2048 tokens, 28/4
+// heads of 128, 99 us (180 with one kind of CTA and comparisons for codes); with cache
+// scales other than 1, which divide every k and v in doubles, a quarter more (93 -> 116 us
+// at another draw of lengths).
 template <typename T, typename KV, int V, int NP>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, const HeadSplit& hs, int walker, int walkers, int part,
                                             int parts) {
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(const GatherArgs a) {
 // (max, sum, O) are merged in order. It serves what the tensor-core kernels do not (other
 // head dims, tensors off their alignment) and is bound by issue and by K and V rows that
 // are fetched per query head: 8 x 1 token over 1000 keys, 16/4 heads of 80, bf16, 61 us
-// (one warp per row and head 476 us), of 256 77 us, 4-bit pages of 96 83 us.
+// (one warp per row and head 476 us), of 256 114 us, 4-bit pages of 96 84 us.
 constexpr int kGeneralWarps = 8;
 
 // sum of q[c] * K[c] over the row pr of a block at `block` (of one head of a page)

@@ -23,12 +23,18 @@
 // 4-bit pages: a (page, head) block is contiguous and arrives by one untiled bulk
 // copy (tiled boxes of 64- and 16-byte rows held the TMA at 3.8 TB/s); codes
 // become halves in registers, in the order of the MMA fragments: E2M1 x E4M3 has 6 significant bits, so the
-// products are exact, and the MMA runs in f16 for every model type. q is scaled
-// by a power of two per row for that, which is exact too; a float32 q, and its P,
-// enter as two halves each (22 bits).
+// products are exact, and the MMA runs in f16 for every model type. q is scaled for that
+// by a power of two per row, its largest element to [1, 2): a half keeps all 11 bits of
+// elements down to 2^-14, smaller ones to 2^-25 of the row's maximum; a float32 q, and
+// its P, enter as two halves each (22 bits).
+//
+// P is rounded to the model's 16-bit type for its product with V (to halves over 4-bit
+// pages), sums and O stay in fp32: the error against 64 bits of a bf16 output is 2.1e-3
+// where its own rounding alone gives 1.7e-3, of f16 2.7e-4 and 2.1e-4. The exponentials
+// are ex2.approx (2^-22), the cap's reciprocal rcp.approx (2^-23).
 //
 // float32 pages: every operand is split into two TF32 numbers and three of the four
-// products are summed (2^-23 relative, like an fp32 product), so the call stays bound
+// products are summed (2^-22 relative; 2.4e-7 against 64 bits in all), so the call stays bound
 // by memory instead of by FFMA. MMAs cut their sums off, which would bias long
 // chains: scores are summed in four, O in one per 16 keys, and added up in fp32.
 //
@@ -37,7 +43,8 @@
 // not (32 x up to 2304 keys, 28/4 heads: 26.7 us = 4.2 TB/s; 1 x 333 keys 6 us). 4-bit
 // pages: the conversion (24 x up to 8192 keys, 28/4 heads: 34 us; ALU 51% busy, issue 57%
 // with 12 consumer warps per SM; eight per CTA spilled). float32: 32 x up to 1501 keys,
-// 16/4 heads: 39 us = 3.7 TB/s.
+// 16/4 heads: 40 us = 3.6 TB/s (ALU 38%, issue 40% busy); prompts in tiles of 8 rows, for
+// each of which K and V are fetched and split again: 4 x 512 tokens, 16/4 heads, 380 us.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -66,7 +73,7 @@ struct DecodeArgs {
 
 // W consumer warps: 4, or 8 where the ring's entries are small enough. Two CTAs per
 // SM, one works while the other waits (float32, 32 x 1501 keys, 16/4 heads: one CTA of 8
-// warps 43.4 us, two of 4 39.2, although a few registers spill);
+// warps took a tenth longer than two of 4, although a few registers spill);
 // 4-bit pages three, or one with two row tiles or split float32 operands.
 template <typename T, typename KV, int D, int NT>
 struct DecodeLayout {
@@ -1058,7 +1065,7 @@ struct DecodePlan {
 
 // Shares of a split call are at least kMinKeys keys (1 x 1501 keys, us with 64 | 128 |
 // 256 | 512: 28/4 heads 16 bits 8.3 | 8.4 | 9.9 | 13.5, 4 bits 8.5 | 8.5 | 9.6 | 11.9,
-// float32 16/4 heads 11.7 | 11.6 | 14.9 | 21.4; nothing changes where every CTA has
+// float32 16/4 heads 10.5 | 11.6 | 15.1 | 23.3; nothing changes where every CTA has
 // more); a call whose sequences cannot exceed kWholeKeys runs one CTA per unit.
 constexpr int kWholeKeys = 512;
 constexpr int kMinKeys = 128;

@@ -7,11 +7,15 @@
 // so a K/V block is fetched once for the whole group and a tile's rows differ by
 // few tokens: few blocks are partly masked.
 //
-// Many tiles: the grid is their list (longest first within groups of (sequence, KV
-// head) pairs whose K/V stay in L2). A CTA that works claims the next one of the list
+// Many tiles: the grid is their list, by groups of (sequence, KV head) pairs whose K/V
+// stay in L2, in a group the sequences' tiles by their index up to max_new, from the last
+// (the longest first where the sequences have as many cached rows; a single token is tile 0
+// and comes last, however long its cache). A CTA that works claims the next one of the list
 // from the hardware scheduler (cluster launch control) while it computes, so two CTAs
 // per SM stay for the whole call, one tile's end overlaps the next one's start, and a
 // ragged batch is balanced as it runs (which CTA computes a tile changes nothing in it).
+// Prompts beside single tokens suit neither rule: 1 x 2048 tokens 44 us, 31 x 1 over 8,000
+// to 32,000 keys 196 in the decode kernel, both in one call, here, 612.
 // Few tiles: each tile's keys are split evenly into parts, which are items of the list
 // like tiles; they store their (max, sum, O) in the workspace, and a second kernel merges
 // them in order.
@@ -30,18 +34,24 @@
 // 4-bit pages: no producer warp; four converter warps read codes and scales a
 // block ahead into registers and write the K and V stages as halves (E2M1 x E4M3
 // has 6 significant bits: exact), and the MMAs run in f16 for every model type. The
-// softmax warps then write the Q tile, each row scaled by a power of two (exact), and
-// undo the scale on the scores.
+// softmax warps then write the Q tile, each row scaled by a power of two so that its
+// largest element is in [1, 2) (halves keep smaller ones to 2^-25 of it), and undo the
+// scale on the scores.
+// P is rounded to the model's 16-bit type for P V (to halves over 4-bit pages); sums and O
+// stay in fp32. Against 64 bits a bf16 output is off by 2.1e-3, where its own rounding
+// gives 1.6e-3, f16 2.4e-4 and 2.1e-4.
 // Every wait is bounded; one that runs out sets the device error word and winds the
 // CTA down.
 //
-// Bound by the chain S -> softmax -> P V -> next S of each CTA (tensor unit busy 59% of the
-// time, MUFU 39%, issue 39%, L2 26%; two threads per row, 96 registers each, 402 us
-// instead of 365): 16 prompts of up to 2048 tokens, 28/4 heads of 128, bf16: 365 us = 787 TFLOP/s
-// (466 when a grid of whole tiles had no claiming; 64 keys a block keep two CTAs in an
+// Bound by the chain S -> softmax -> P V -> next S of each CTA (tensor pipe busy 38% of the
+// active cycles, MUFU 39%, issue 39%, L2 25%; two threads per row, 96 registers each, 402 us
+// instead of 365): 16 prompts of up to 2048 tokens, 28/4 heads of 128, bf16: 365 us = 787
+// TFLOP/s in a graph of 12 calls, 416 = 693 called one by one for seconds, at the clocks of
+// the power cap (466 when a grid of whole tiles had no claiming; 64 keys a block keep two CTAs in an
 // SM's tensor memory). 2 chunks of up to 383 tokens over 8000 keys, window 4096, bias, 16
-// heads of 64: 39 us (issue 40%, MUFU 35%, tensor 34% busy). 4-bit pages, 4 chunks of up
-// to 301 tokens over 3001 keys, 28/4 heads: 83 us, over 16-bit pages 65.
+// heads of 64: 39 us (issue 39%, MUFU 34%, tensor 17% busy). 4-bit pages, 4 chunks of up
+// to 301 tokens over 3001 keys, 28/4 heads: 83 us (issue 43%, ALU 35%, tensor 26% busy, the
+// converters' loads), over 16-bit pages 65.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -149,7 +159,7 @@ struct Scheduler {
   bool begun = false, open = false;
 
   // Item `at` of the grid's list; false when there is nothing to do in it. Order: parts,
-  // groups of pairs, the longest tiles first, the pairs of the group.
+  // groups of pairs, tiles from the last that max_new allows, the pairs of the group.
   __device__ __forceinline__ bool item(int at, Tile& x) {
     const int pairs = p.a.hkv * p.a.seqs.batch, units = pairs * p.tiles;
     const int part = at / units, unit = at - part * units;

@@ -1,5 +1,5 @@
 // Warp-level matrix and conversion wrappers (mma.sync, ldmatrix, movmatrix, ex2)
-// used by the paged decode attention.
+// of the paged KV-cache kernels.
 #pragma once
 
 #include <stdint.h>
@@ -51,7 +51,7 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   }
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
-// A B to fp32's accuracy as three TF32 products, lo * lo (2^-24 of it) left out. The
+// A B to fp32's accuracy as three TF32 products, lo * lo (2^-22 of it at most) left out. The
 // MMA cuts its sums off instead of rounding them, so the caller keeps its chains
 // short: the leading product goes to `main`, the small ones to `low`.
 __device__ __forceinline__ void mma_1688_f32(float (&main)[4], float (&low)[4], const uint32_t (&ah)[4],

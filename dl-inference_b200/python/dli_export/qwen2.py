@@ -208,7 +208,8 @@ def build_graph(shape: Qwen2Shape, capacity: int, tp_size: int = 1, model_type: 
     write one `linear_qkv_rotary_cache` node (decode GEMMs rotate and scatter
     in their epilogue). `page_size` > 0 keeps the cache in a pool of `num_pages`
     pages of that many rows, of the weights' dtype or with kv_dtype = "fp4" of 4
-    bits: the graph then has a third input, page_table (int32 [B, max_pages])."""
+    bits: the graph then has a third input, page_table (int32 [B, max_pages]), and the
+    q|k|v projection is a `linear` node of its own, whatever `fused_qkv_rotary` says."""
     if page_size < 0 or (page_size > 0) != (num_pages > 0):
         raise ValueError("a paged cache needs page_size and num_pages")
     if kv_dtype not in (None, "fp4") or (kv_dtype and not page_size):

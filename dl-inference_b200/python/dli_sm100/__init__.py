@@ -507,7 +507,9 @@ def qkv_rotary_paged(qkv, cos, sin, positions, page_table, k_pages, v_pages, q_h
     """Rotary embedding of a packed q|k|v projection [.., (Hq + 2 Hkv) * D], its k and
     v appended to the pages at positions[b], positions[b] + 1, ...; returns rotated q
     [rows, Hq, D]. `starts` (int64 [batch + 1]) gives the rows of every sequence, at
-    most `max_new` each; None: all sequences have the same number."""
+    most `max_new` each; None: all sequences have the same number. With `starts`, pass
+    the longest as `max_new`: without it, it is all rows, and the grid is sized for
+    sequences of that many."""
     what = "qkv_rotary_paged"
     kv_heads, width = k_pages.shape[1], qkv.shape[-1]
     heads = q_heads + 2 * kv_heads
@@ -544,7 +546,8 @@ def _attention_paged_workspace(dev, *sizes):
 def attention_paged(q, k_pages, v_pages, positions, page_table, starts=None, max_new=None, scale=0.0, softcap=0.0,
                     window=0, slopes=None, k_scale=1.0, v_scale=1.0, out=None):
     """Causal attention of packed q [rows, Hq, D] over a paged cache (after the append
-    of the rows' k and v). softcap > 0 caps the scores by a tanh, window > 0 limits a
+    of the rows' k and v). `starts` and `max_new` as in qkv_rotary_paged; max_new also
+    chooses the kernel (few new rows, or many). softcap > 0 caps the scores by a tanh, window > 0 limits a
     row to its last `window` keys, slopes (float32 [Hq]) add slope * (j - i)."""
     what = "attention_paged"
     if q.dim() != 3:

@@ -291,7 +291,9 @@ dli_status dli_sm100_attention_kvcache_noalloc(const void* q, const void* cache_
  * tokens each, none for an idle sequence), at positions positions[b],
  * positions[b]+1, ... (positions: int64 [batch], the rows cached before the
  * call). starts = NULL means max_new tokens of every sequence. `tokens` is the
- * number of rows the buffers have; rows of no sequence are not touched.
+ * number of rows the buffers have; rows of no sequence are not touched. max_new
+ * chooses the attention's kernel and sizes the grids: a bound that is far above
+ * what the sequences have costs time, not correctness.
  * A sequence whose starts or positions are outside their bounds is skipped (its
  * rows and pages are left as they were), and a page outside the pool is not
  * written and read as zeros; both set the device error word. */
@@ -302,7 +304,8 @@ size_t dli_sm100_paged_kv_page_bytes(int64_t kv_heads, int64_t page_size, int64_
 /* dli_sm100_qkv_rotary_cache for a packed batch and a paged cache: qkv[tokens,
  * (Hq + 2 Hkv) * D] holds q heads, k heads, v heads per token; rotated q goes to
  * q_out[tokens, Hq, D], rotated k and v into the pages. Into 4-bit pages k is
- * rotated and both are quantised as if exactly (one rounding, to the codes). */
+ * rotated and both are divided by their scale in 64 bits, and rounded once more,
+ * to the codes. */
 dli_status dli_sm100_qkv_rotary_paged(const void* qkv, const float* cos_table, const float* sin_table,
                                       const int64_t* positions, const int64_t* starts, const int32_t* page_table,
                                       void* q_out, void* k_pages, void* v_pages, int64_t tokens, int64_t batch,
@@ -320,7 +323,8 @@ dli_status dli_sm100_qkv_rotary_paged(const void* qkv, const float* cos_table, c
  * past its last row) are not looked up; their table entries may be anything.
  * Non-finite values: in a row of q they reach only that row's heads; a cached v
  * row reaches the rows that see it and, where it is not finite, may also reach
- * the earlier new tokens of the same call (0 * NaN in a shared tile). out may be
+ * other new tokens of the same call (earlier ones, with a window later ones too:
+ * 0 * NaN in a shared tile). out may be
  * q itself. The workspace is scratch: nothing in it has to be initialised or
  * kept, but calls that may overlap on the GPU need their own.
  * Head dims 64 and 128 with 16-byte aligned tensors run on tensor cores, others on
@@ -338,7 +342,7 @@ dli_status dli_sm100_attention_paged(const void* q, const void* k_pages, const v
 
 /* Rows first[b] .. first[b] + count - 1 (first: int64 [batch], NULL = 0) of every
  * sequence as dense k_out / v_out [batch, Hkv, count, D] of `dtype` (the values
- * 4-bit pages stand for, rounded to dtype). Rows at or past lengths[b] (int64
+ * 4-bit pages stand for, rounded to dtype through float32). Rows at or past lengths[b] (int64
  * [batch], NULL = no limit but the table's) are written as zeros. */
 dli_status dli_sm100_paged_gather(const void* k_pages, const void* v_pages, const int32_t* page_table,
                                   const int64_t* first, const int64_t* lengths, void* k_out, void* v_out,
